@@ -21,7 +21,7 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 def sources():
     """Everything the library is built from: an edit to any of it makes the built library stale."""
-    src = sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh")))
+    src = sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh", ".h")))
     return src + [os.path.join(os.path.dirname(HERE), "include", "cck_b200.h"), os.path.abspath(__file__)]
 
 
@@ -42,7 +42,7 @@ def build(force=False, verbose=False, out=None, defines=()):
     # libc and libm only at run time, as the reference's library (its CI audits that with ldd): the CUDA
     # runtime is linked statically by nvcc's default, the C++ runtime and libgcc by these flags
     cmd += ["-shared", "-Xcompiler", "-fPIC", "-Xcompiler", "-static-libstdc++", "-Xcompiler", "-static-libgcc"]
-    cmd += ["-o", OUT_, os.path.join(CSRC, "cck_b200.cu")]
+    cmd += ["--threads", "0", "-o", OUT_, os.path.join(CSRC, "cck_b200.cu"), os.path.join(CSRC, "sequence.cu")]
     ffi = os.environ.get("CCK_FFI_INCLUDE_DIR")
     if ffi:
         cmd += ["-DCCK_FFI", "-I", ffi, os.path.join(CSRC, "ffi_handler.cu")]

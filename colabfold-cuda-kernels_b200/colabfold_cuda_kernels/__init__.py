@@ -23,14 +23,18 @@ _KERNEL_TABLE = {
 }
 KERNELS = tuple(_KERNEL_TABLE)
 
+# the sequence operators, which only this library has; KERNELS stays the reference's list
+SEQUENCE_KERNELS = ("rotary", "cache_append", "cache_attention")
+_KERNEL_TABLE.update(rotary=((100,), "CckRotary"), cache_append=((100,), "CckCacheAppend"), cache_attention=((100,), "CckCacheAttention"))
+
 # plain C entry point behind each FFI target that is built, for callers without XLA
-C_ABI = {"diffusion": "cck_mk_sample"}
+C_ABI = {"diffusion": "cck_mk_sample", "rotary": "cck_rotary", "cache_append": "cck_cache_append", "cache_attention": "cck_cache_attention"}
 
 
 def symbol(kernel, cc):
     """XLA FFI target name of `kernel` at compute capability `cc` (major * 10 + minor)."""
     if kernel not in _KERNEL_TABLE:
-        raise KeyError("unknown kernel %r, expected one of %s" % (kernel, ", ".join(KERNELS)))
+        raise KeyError("unknown kernel %r, expected one of %s" % (kernel, ", ".join(_KERNEL_TABLE)))
     served, name = _KERNEL_TABLE[kernel]
     if not served:
         raise FileNotFoundError("%s is not built in the B200 library" % kernel)

@@ -4,6 +4,7 @@
 //   mk_*                 the stand-alone debug API (ctypes), same signatures as the reference's
 // Declarations with the reference interfaces they replace: include/cck_b200.h.
 #include "host.cuh"
+#include "report.h"
 
 using namespace cck;
 
@@ -94,6 +95,15 @@ __global__ void philox_test_kernel(uint32_t idx, uint32_t step, uint32_t sample,
 }
 
 } // namespace
+
+int cck::report(int code, const char* message) noexcept {
+    try {
+        g_error = message;
+    } catch (...) { // no memory for the text
+        g_error.clear();
+    }
+    return code;
+}
 
 extern "C" {
 

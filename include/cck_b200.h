@@ -68,6 +68,95 @@ int cck_mk_sample_static(void* stream, const int* ext, const void* const* in, co
                          float* out, int out_tokens, int samples, int nsteps, int flags);
 size_t cck_static_workspace_bytes(void);
 
+/* ---- Sequence operators
+ *
+ * What a sequence model needs on the GPU that it shares with the sampler: rotary positions, a cache of keys and values in 8
+ * bits and the attention that reads it. No counterpart in the reference. Same manner as cck_mk_sample: device memory of the
+ * caller's, one or two kernels enqueued on `stream` (a stream of the current device), no allocation, no synchronisation, an
+ * error code and cck_last_error(); every call can be captured into a CUDA graph. All descriptors are read before a call
+ * returns; what their pointers point to (cck_rows::data, freq, pos, first, len, table, ...) is device memory that the kernels
+ * read. Arguments that cannot be right are refused before anything is enqueued: CCK_E_SHAPE (null pointers, sizes, strides,
+ * alignment), CCK_E_FLAGS (a type that is not built), CCK_E_WORKSPACE, CCK_E_DEVICE (memory of another device, or not device
+ * memory). */
+enum { CCK_BF16 = 0, CCK_F16 = 1, CCK_F32 = 2 };
+
+/* A tensor [rows][heads][dim]: element (r, h, d) is at data + r * row_stride + h * head_stride + d, in elements. */
+typedef struct cck_rows {
+    void* data;
+    int64_t row_stride, head_stride;
+    int32_t dtype, heads;
+} cck_rows;
+
+/* Rotary positions with up to four axes. The first `dims` (even) of a head's dimensions are dims/2 pairs: (i, i + dims/2), or
+ * with `adjacent` (2i, 2i+1). The first section[0] pairs turn with axis 0, the next section[1] with axis 1, and so on; the
+ * sections add up to dims/2. Pair i of a row turns by pos[axis * pos_stride + row] * freq[i] radians; the product and its
+ * reduction are in 64 bits, cosine and sine in 32. Positions may be negative. */
+typedef struct cck_rotation {
+    int32_t dims, axes, adjacent, section[4];
+    const float* freq;   /* f32 [dims/2] */
+    const int32_t* pos;  /* i32 [axes][rows] */
+    int64_t pos_stride;
+} cck_rotation;
+
+/* A paged cache in 8 bits: `pages` pages of page_tokens tokens (16, 32, 64 or 128), heads of `dim` (32, 64, 96 or 128). For each
+ * (page, head) the keys and the values have a scale each, f32 [pages][heads]; a value is its e4m3 code times the scale.
+ *   keys    [pages][heads][page_tokens/8][dim/16][8 tokens][16 dims]
+ *   values  [pages][heads][page_tokens/16][dim][16 tokens]
+ * These are the tensor cores' own operand tiles, so that a page goes from HBM to shared memory in one copy and is used as it
+ * lies. k and v are 16-byte aligned. A scale is a power of two from 2^-40 to 2^40 where cck_cache_append wrote it; the
+ * attention takes any positive one of that range. */
+typedef struct cck_cache {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    int32_t pages, page_tokens, heads, dim;
+} cck_cache;
+
+/* The sequences of a call. Rows first[b] .. first[b+1]-1 are sequence b's newest first[b+1]-first[b] tokens (none is fine), len[b]
+ * is its length with them: both calls of a step take the same batch. Token t of it lies in page table[b * table_stride + t /
+ * page_tokens], slot t % page_tokens. first is not decreasing, from 0 up. Rows from first[sequences] on belong to nobody and are
+ * neither read nor written. */
+typedef struct cck_batch {
+    int32_t sequences, rows;    /* rows: of the tensors; first[sequences] at most */
+    int32_t max_new, max_len;   /* at least the largest first[b+1]-first[b] and len[b]; they size the launch */
+    int32_t table_pages;        /* columns of the table */
+    const int32_t *first, *len; /* i32 [sequences+1], [sequences] */
+    const int32_t* table;
+    int64_t table_stride;
+} cck_batch;
+
+/* y = R(pos) x for `rows` rows; with inverse != 0, R(-pos) x, which is also the gradient: dx = R(-pos) dy. x and y have the same
+ * heads and type (bf16, f16 or f32) and 1 <= dim <= 1024; dimensions from rotation->dims on are copied. y may be x (same data and
+ * strides); otherwise they do not overlap. Any strides and alignment of the type are taken; 16-byte ones are the fastest. */
+int cck_rotary(void* stream, const cck_rotation* rotation, int rows, int dim, const cck_rows* x, const cck_rows* y, int inverse);
+
+/* Puts the batch's rows of k and v (heads and dim of the cache; bf16, f16 or f32; data and strides multiples of 16 bytes) into the
+ * cache, the keys rotated if `rotation` is given. q (may be null; any number of heads) is rotated into q_out (which may be q) by
+ * the same launch.
+ * A page's scale is the smallest power of two that holds the values put into it, at least the one it has if older tokens of the
+ * sequence share the page: those are then brought to the new scale. Rounded to nearest even; magnitudes over 448 * 2^40 saturate,
+ * what is far below 2^-40 is lost. A token that holds NaN or an infinity in a head's key or value becomes NaN in whole: its key's
+ * codes are NaN, its value's are zero, and the rows of that head that attend to it come out as NaN, the others untouched.
+ * Pages that a call writes to belong to one sequence of the batch; full pages may be shared. Slots past len[b] keep their codes.
+ * status (may be null): set to 1 on the device where something was left out: a page id outside the cache, a sequence longer than
+ * its row of the table or max_new, rows past batch->rows. */
+int cck_cache_append(void* stream, const cck_cache* cache, const cck_batch* batch, const cck_rows* k, const cck_rows* v,
+                     const cck_rotation* rotation, const cck_rows* q, const cck_rows* q_out, int32_t* status);
+
+/* out = softmax(softmax_scale * q K^T) V over the cache, for the batch's rows; q heads are a multiple of the cache's heads (head j
+ * reads cache head j / (q heads / heads)); q and out are bf16 or f16, both the same, data and strides multiples of 16 bytes.
+ * Row i of n of sequence b stands at place len[b]-n+i. causal: it sees places up to its own, else all len[b]; window > 0: of
+ * those only the ones later than its place - window. A row that sees nothing gives 0, and -inf in lse. lse (may be null):
+ * f32 [rows][q heads], the natural log of the sum of exponentials. Scores, maxima, sums and outputs are accumulated in f32; q is
+ * rounded to 11 bits relative to a power of two at the row's largest (bf16 and f16 lose nothing above 2^-14 of it), the
+ * probabilities to f16.
+ * Rows that need a page id outside the cache or past the table's row are NaN. Slots past len[b] may hold anything.
+ * ws: cck_cache_attention_workspace_bytes(cache, batch, q_heads) bytes (0 if none is needed, also for arguments that the call
+ * refuses), 16-byte aligned, may be uninitialised; its contents mean nothing between calls. Calls that overlap on the GPU, or graphs that may
+ * run at the same time, need one each. */
+size_t cck_cache_attention_workspace_bytes(const cck_cache* cache, const cck_batch* batch, int q_heads);
+int cck_cache_attention(void* stream, const cck_cache* cache, const cck_batch* batch, const cck_rows* q, const cck_rows* out, float* lse,
+                        float softmax_scale, int causal, int window, void* ws, size_t ws_bytes);
+
 /* Workspace size for a shape bucket; 0 if the sizes do not describe a supported model
  * (src/diffusion/host.cuh:376-379). */
 size_t mk_workspace_bytes(int S, int Nb, int NSb, int nsteps, int flags, const size_t* bytes);
