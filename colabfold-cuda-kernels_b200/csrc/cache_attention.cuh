@@ -6,13 +6,20 @@
 // The values' scale rides in the exponent: p stays in [0, 1] whatever the scales of the pages are, goes to the tensor cores as f16
 // and what it loses there (below 2^-24) is small against the largest term of the sum. One pass with running maximum and sum.
 //
-// Bound by memory: 2 * dim bytes a key and head, read once. Every warp runs on its own: it takes granules of 32 keys, which lie in one
-// piece in a page, through a ring of bulk copies into its own shared memory, and multiplies with mma.m16n8k16 in f16 (codes are f16
-// exactly). 16 query rows (the heads that share the keys, times the new tokens) fill a tile; a tcgen05 tile of 128 rows would be
-// empty but for those. The cache's layout is such that both products read their operand as it lies, four codes a word, with the
-// k index permuted alike on both sides:
-//   q.k: lane (n = lane / 4, c = lane % 4) holds dims 16 k + 4 c .. + 3 of key n
-//   p.v: lane (n, c) holds keys 16 s + 4 c .. + 3 of dim n; so score tile 2 s + j has keys 16 s + 4 (n / 2) + 2 j + n % 2 in its columns
+// Bound by memory: 2 * dim bytes a key and head, read once. Every warp runs on its own: it takes granules of 32 or 64 keys, which lie in one
+// piece in a page, through a ring of bulk copies into its own shared memory. Keys are the 16 rows of its tiles, the 8 columns are query
+// rows (the heads that share the keys, times the new tokens): a tcgen05 tile of 128 rows would be empty but for those, and a warp
+// that waits for nobody hides its copies better. What then counts is the number of instructions, whose fetch a warp pays for
+// anew in every granule; so the codes go to the tensor cores as they lie:
+//   K q^T   mma.m16n8k32 on e4m3. ldmatrix brings four 8 keys x 16 dims pieces at once. q, scaled to 256 at its row's largest, is split into
+//           terms of 4 bits, each the e4m3 rounding of 16 times what the one before left: two terms hold a bf16, three an f16, exactly
+//           down to 2^-13 of the row's largest. Sums of a term are f32 (checked: nothing is cut off in the tensor core).
+//   V^T p   mma.m16n8k16 on f16, to which the codes convert exactly. p needs the range: in terms of e4m3 a key of probability
+//           2^-16 would vanish beside one of 1, and a long tail of such keys can outweigh it.
+// Score rows i and i + 8 of tile u are keys 16 u + 4 (i / 2) + i % 2 and two on, such that transposing a score tile's two 8 x 8 halves
+// gives p in the order in which a word of V holds four keys.
+// The running maximum is only a reference: it moves when a score is 2^8 over it, so that shuffles and the rescaling of the sums
+// are rare; p is at most 2^14 and what f16 loses of it lies below 2^-30 of the largest.
 #pragma once
 
 #include <climits>
@@ -22,7 +29,11 @@
 namespace cck {
 namespace seq {
 
-constexpr int kGranule = 32; // keys of one step of a warp
+// Keys of one step of a warp: 8 KB of codes at 64 and 128 dims. A step has a fixed cost (its pages, its copies, the running maximum) of about
+// what 32 keys cost at 128 dims.
+constexpr int granule_of(int dim) {
+    return dim <= 64 ? 64 : 32;
+}
 
 struct AttentionArgs {
     cck_cache cache;
@@ -33,8 +44,9 @@ struct AttentionArgs {
     float* lse;
     float scale_log2; // softmax_scale * log2(e)
     int q_heads, group, causal, window;
-    int row_tiles, splits, chunk; // splits: chunks of `chunk` keys (a multiple of kGranule) that the launch gives a sequence at most
-    float *part_o, *part_ml;      // [splits][rows * q_heads][dim], [..][2]; null without splits
+    int granule, page_shift; // granule_of(dim); page_tokens = 1 << page_shift
+    int tile_rows, row_tiles; // a sequence's rows times heads of a group, cut into tiles: `tiles` are those of all sequences, row_tiles each
+    float *part_o, *part_ml; // shares of units that several blocks work on: [2 blocks][tile rows][dim], [..][2]; null: a block takes a unit
 };
 
 // keys [lo, hi) that row i (a place in its sequence) sees
@@ -53,17 +65,45 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-    uint32_t v;
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
-    return v;
+__device__ __forceinline__ void mma_e4m3(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// four pieces of 8 rows x 16 bytes; lane l gives the address of row l % 8 of piece l / 8
+__device__ __forceinline__ void ldmatrix4(uint32_t (&w)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ float4 codes_to_f32(uint32_t w) {
+    uint32_t lo, hi;
+    unpack_e4m3(w, lo, hi);
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) { // an 8 x 8 matrix of f16 in the accumulators' layout
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 
 constexpr int kDecodeWarps = 4;
-template <int D>
+// p = 2^(x - base); base = largest x - kHeadroom when it is set, and is set anew when an x is over base + kSlack. It begins below all scores
+constexpr float kHeadroom = 6.f, kSlack = 14.f, kNoBase = -1e30f;
+// NT: tiles of 8 query rows. Blocks of threads an SM: what registers (32 NT of sums, 16 NT of queries at 128 dims) and shared memory hold
+template <class T>
+constexpr bool T_is_f16() {
+    return false;
+}
+template <>
+constexpr bool T_is_f16<__half>() {
+    return true;
+}
+template <int D, int NT>
 struct DecodeShape {
-    static constexpr int kStage = 2 * kGranule * D;                     // keys, then values
-    static constexpr int kStages = 96 * 1024 / (kDecodeWarps * kStage); // two blocks of threads an SM
+    static constexpr int kBlocks = NT == 1 ? 3 : 2;
+    static constexpr int kKeys = granule_of(D), kStage = 2 * kKeys * D; // keys, then values
+    static constexpr int kStages = (NT == 1 ? 64 : 96) * 1024 / (kDecodeWarps * kStage);
     static constexpr int kRing = kDecodeWarps * kStages * kStage;
     static constexpr int kSmem = kRing + kDecodeWarps * kStages * 8 + 16;
 };
@@ -85,74 +125,140 @@ struct TileKeys {
     int g0, g1; // granules of [lo, hi)
 };
 __device__ __forceinline__ TileKeys keys_of_tile(const AttentionArgs& A, const Sequence& s, int r0, int r1) {
+    const int granule = A.granule;
     const int2 first = seen_by(A, s.place0 + r0 / A.group, s.len), last = seen_by(A, s.place0 + (r1 - 1) / A.group, s.len);
     TileKeys t;
     t.lo = first.x, t.hi = last.y, t.all_lo = last.x, t.all_hi = first.y;
-    t.g0 = t.lo / kGranule, t.g1 = max(t.g0, ceil_div(t.hi, kGranule));
+    t.g0 = t.lo / granule, t.g1 = max(t.g0, ceil_div(t.hi, granule));
     return t;
 }
 
-// chunks that have keys; the last one takes what is left where a length is over max_len
-__device__ __forceinline__ int chunks_of(const AttentionArgs& A, const TileKeys& t) {
-    return min(A.splits, ceil_div(t.g1 - t.g0, A.chunk / kGranule));
+// ---- The work, cut into equal shares
+//
+// A unit is a (tile, head); its granules, and all units' one behind the other, are a line that the launch's blocks of threads cut
+// into equal shares, whatever the lengths are. A block's share can begin inside a unit and end inside another: it leaves what it
+// has of the first in slot 0 of its part of the workspace, of the last in slot 1, and merge_kernel puts the shares together.
+struct Tile {
+    Sequence s;
+    int r0, rows; // rows r0 .. r0 + rows - 1 of the sequence's rows times heads of a group
+};
+__device__ __forceinline__ Tile tile_at(const AttentionArgs& A, int i) {
+    Tile t;
+    t.s = sequence_of(A.batch, i / A.row_tiles);
+    t.r0 = i % A.row_tiles * A.tile_rows, t.rows = max(0, min(A.tile_rows, t.s.rows * A.group - t.r0));
+    return t;
+}
+__device__ __forceinline__ int granules_of(const AttentionArgs& A, int i) {
+    const Tile t = tile_at(A, i);
+    if (t.rows == 0) {
+        return 0;
+    }
+    const TileKeys k = keys_of_tile(A, t.s, t.r0, t.r0 + t.rows);
+    return max(1, k.g1 - k.g0); // a tile that sees nothing still has rows to write
+}
+// The tile on the line of one head's granules that `pick` chooses (of start, granules, index), where it starts, and the line's length.
+// Every warp finds out by itself, 32 tiles at a time. `pick` is only asked once the length is known.
+struct Line {
+    int64_t total, start;
+    int tile;
+};
+template <class Pick>
+__device__ __forceinline__ Line line_of(const AttentionArgs& A, Pick pick) {
+    const int n = A.batch.sequences * A.row_tiles, lane = threadIdx.x & 31;
+    Line l{0, 0, 0};
+    int g = lane < n ? granules_of(A, lane) : 0;
+    int64_t sum = g;
+#pragma unroll 1
+    for (int i = 32 + lane; i < n; i += 32) {
+        sum += granules_of(A, i);
+    }
+#pragma unroll
+    for (int o = 16; o; o /= 2) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
+    l.total = sum;
+    int64_t at = 0;
+#pragma unroll 1
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        const int i = i0 + lane;
+        g = i0 == 0 ? g : i < n ? granules_of(A, i) : 0;
+        int64_t upto = g;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+            upto += lane >= o ? x : 0;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, i < n && g > 0 && pick(at + upto - g, g, i, l.total));
+        if (hit) {
+            const int from = __ffs(hit) - 1;
+            l.tile = i0 + from, l.start = __shfl_sync(0xffffffffu, at + upto - g, from);
+            break;
+        }
+        at += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return l;
+}
+// granules of a share: all have as many, the last ones fewer or none
+__device__ __forceinline__ int64_t share_size(int64_t total, int shares) {
+    return (total + shares - 1) / shares;
 }
 
-// A page of the table for 16 or 32 keys, and its scales
+// The keys of a granule that one page holds, and the page's scales
 struct Piece {
-    int page;
-    float a, e, iv; // scale of the scores; log2 and inverse of the values' scale
+    int64_t at; // their first code, in bytes from the cache's
+    float ks, vs;
 };
-__device__ __forceinline__ Piece piece_at(const AttentionArgs& A, int b, int head, int key) {
+__device__ __forceinline__ Piece piece_at(const AttentionArgs& A, int b, int head, int key, bool wanted) {
     const cck_cache& C = A.cache;
-    const int col = key / C.page_tokens;
     Piece r;
-    r.page = 0, r.a = __int_as_float(0x7fffffff), r.e = 0.f, r.iv = 1.f; // not there: scores are NaN, page 0 is read in its place
-    const int p = col < A.batch.table_pages ? A.batch.table[b * A.batch.table_stride + col] : -1;
+    r.at = 0, r.ks = __int_as_float(0x7fffffff), r.vs = 1.f; // not there: scores are NaN, page 0 is read in its place
+    const int col = key >> A.page_shift;
+    const int p = wanted && col < A.batch.table_pages ? A.batch.table[b * A.batch.table_stride + col] : -1;
     if (p >= 0 && p < C.pages) {
-        const int64_t at = int64_t(p) * C.heads + head;
-        const float vs = C.v_scale[at];
-        r.page = p, r.a = C.k_scale[at] * A.scale_log2, r.e = log2f(vs), r.iv = 1.f / vs;
+        const int64_t block = int64_t(p) * C.heads + head;
+        r.at = ((block << A.page_shift) + (key & (C.page_tokens - 1))) * C.dim, r.ks = C.k_scale[block], r.vs = C.v_scale[block];
     }
     return r;
 }
-
-// codes of the 4 keys from `key` on that lie outside [lo, hi) become zero: an unused slot may hold NaN, and 0 * NaN is NaN
-__device__ __forceinline__ uint32_t keep_keys(uint32_t w, int key, int lo, int hi) {
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-        if (key + e < lo || key + e >= hi) {
-            w &= ~(0xFFu << (8 * e));
-        }
-    }
-    return w;
+__device__ __forceinline__ float log2_fast(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float inverse_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
-// MT: tiles of 16 rows a warp keeps
-template <class T, int D, int MT>
-__global__ void __launch_bounds__(kDecodeWarps * 32, 2) decode_kernel(const AttentionArgs A) {
-    using S = DecodeShape<D>;
+// Codes of values outside [lo, hi) in a stage become zero: an unused slot may hold NaN, and 0 * NaN is NaN. Of pages that are not
+// there (`absent`, a bit for each tile of 16 keys) all do.
+template <int D, int kKeys>
+__device__ __noinline__ void clear_values(uint32_t v, int lo, int hi, uint32_t absent) {
+#pragma unroll 1
+    for (int i = threadIdx.x & 31; i < kKeys * D / 4; i += 32) {
+        const int key = i / (4 * D) * 16 + i % 4 * 4;
+        uint32_t w;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(v + 4 * i));
+        for (int e = 0; e < 4; e++) {
+            if (key + e < lo || key + e >= hi || (absent >> (key / 16) & 1)) {
+                w &= ~(0xFFu << (8 * e));
+            }
+        }
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(v + 4 * i), "r"(w) : "memory");
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // the next copy into the stage comes after
+    __syncwarp();
+}
+
+template <class T, int D, int NT>
+__global__ void __launch_bounds__(kDecodeWarps * 32, DecodeShape<D, NT>::kBlocks) decode_kernel(const AttentionArgs A) {
+    using S = DecodeShape<D, NT>;
+    constexpr int kTerms = sizeof(T) == 2 && T_is_f16<T>() ? 3 : 2;
+    constexpr int kRows = 8 * NT, kTiles = S::kKeys / 16, kKeysShift = S::kKeys == 64 ? 6 : 5; // kTiles: of 16 keys
     extern __shared__ __align__(128) unsigned char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n8 = lane >> 2, c4 = lane & 3;
-    const int H = A.cache.heads, P = A.cache.page_tokens, G = A.group;
-    int unit = blockIdx.x;
-    const int split = unit % A.splits;
-    unit /= A.splits;
-    const int head = unit % H;
-    unit /= H;
-    const int tile = unit % A.row_tiles, b = unit / A.row_tiles;
-    if (A.splits > 1) {
-        let_next_start();
-    }
-    const Sequence s = sequence_of(A.batch, b);
-    const int total = s.rows * G, r0 = tile * 16 * MT, r1 = min(r0 + 16 * MT, total);
-    if (r0 >= total) {
-        return;
-    }
-    const TileKeys keys = keys_of_tile(A, s, r0, r1);
-    const int per = A.chunk / kGranule, ga = keys.g0 + split * per, gb = split == A.splits - 1 ? keys.g1 : min(keys.g1, ga + per);
-    if (split > 0 && ga >= gb) {
-        return;
-    }
+    const int H = A.cache.heads, G = A.group;
     const uint32_t ring = shared_u32(smem) + warp * S::kStages * S::kStage;
     const uint32_t bars = shared_u32(smem) + S::kRing + warp * S::kStages * 8;
     if (lane == 0) {
@@ -162,276 +268,395 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 2) decode_kernel(const Atte
         bar_init_done();
     }
     __syncwarp();
+    // what is left of this block's share, and where it is: tile, head, granules done of the unit
+    int64_t left = 1, done = 0;
+    int tile = blockIdx.x / H, head = blockIdx.x % H;
+    if (A.part_o) {
+        let_next_start();
+        int64_t from = 0;
+        const Line line = line_of(A, [&](int64_t start, int g, int, int64_t total) {
+            from = share_size(total * H, gridDim.x) * blockIdx.x;
+            return start * H <= from && from < (start + g) * H;
+        });
+        const int64_t size = share_size(line.total * H, gridDim.x);
+        from = size * blockIdx.x, left = min(size, line.total * H - from);
+        if (left <= 0) {
+            return;
+        }
+        tile = line.tile;
+        const int g = granules_of(A, tile);
+        head = int((from - line.start * H) / g), done = from - line.start * H - int64_t(head) * g;
+    }
+    int slot = 0, phase = 0;
+#pragma unroll 1
+    while (left > 0) {
+    const Tile own = tile_at(A, tile);
+    if (own.rows == 0) {
+        if (!A.part_o) {
+            return;
+        }
+        tile++, head = 0;
+        continue;
+    }
+    const Sequence s = own.s;
+    const int b = tile / A.row_tiles, r0 = own.r0, r1 = r0 + own.rows;
+    const TileKeys keys = keys_of_tile(A, s, r0, r1);
+    const int all = max(1, keys.g1 - keys.g0), ga = keys.g0 + int(done);
+    const int gb = A.part_o ? int(min(int64_t(keys.g0 + all), ga + left)) : keys.g0 + all;
+    const bool alone = ga == keys.g0 && gb == keys.g0 + all; // a unit of this block only
+    const int part = 2 * blockIdx.x + (ga == keys.g0 ? 1 : 0);
 
-    // this warp's granules: ga + warp, + kDecodeWarps, ...; a granule is one piece of a page, or two where pages hold 16 tokens.
-    // A lane looks one piece up, so that 32 are known at a time: `now` for the granule worked on, `next` for copies ahead of it
-    const int mine = gb > ga + warp ? ceil_div(gb - ga - warp, kDecodeWarps) : 0;
-    const int pieces = P < kGranule ? 2 : 1, piece = kGranule / pieces;
+    // this warp's granules: ga + warp, + kDecodeWarps, ...; a granule is one piece of a page, or several of small pages. A lane looks
+    // one piece up, so that 32 are known at a time: `now` for the granule worked on, `next` for copies ahead of it
+    const int mine = max(0, ceil_div(gb - ga - warp, kDecodeWarps));
+    const int piece_shift = min(A.page_shift, kKeysShift), pieces_shift = kKeysShift - piece_shift, pieces = 1 << pieces_shift;
     auto look_up = [&](int first) {
-        const int j = first + lane, key = (ga + warp + j / pieces * kDecodeWarps) * kGranule + j % pieces * piece;
-        return piece_at(A, b, head, j < mine * pieces && key < keys.hi && key + piece > keys.lo ? key : INT_MAX);
+        const int j = first + lane, key = (ga + warp + (j >> pieces_shift) * kDecodeWarps) * S::kKeys + ((j & (pieces - 1)) << piece_shift);
+        return piece_at(A, b, head, key, j < mine << pieces_shift && key < keys.hi && key + (1 << piece_shift) > keys.lo);
     };
     Piece now = look_up(0), next = look_up(32);
     int batch = 0; // `now` holds pieces 32 batch ..
-    auto issue = [&](int i) { // granule i into its stage
-        const uint32_t st = ring + i % S::kStages * S::kStage, bar = bars + i % S::kStages * 8;
-        const int key = (ga + warp + i * kDecodeWarps) * kGranule;
+    auto issue = [&](int i, int slot) { // granule i into its stage
+        const uint32_t st = ring + slot * S::kStage, bar = bars + slot * 8, bytes = D << piece_shift;
         if (lane == 0) {
             bar_expect(bar, S::kStage);
         }
+#pragma unroll 1
         for (int h = 0; h < pieces; h++) {
-            const int j = i * pieces + h;
-            const int page = __shfl_sync(0xffffffffu, j >> 5 == batch ? now.page : next.page, j & 31);
-            const int64_t at = (int64_t(page) * H + head) * P * D + (key + h * piece) % P * D;
+            const int j = (i << pieces_shift) + h;
+            const int64_t at = __shfl_sync(0xffffffffu, j >> 5 == batch ? now.at : next.at, j & 31);
             if (lane == 0) {
-                bulk_load(st + h * piece * D, static_cast<const char*>(A.cache.k) + at, piece * D, bar);
-                bulk_load(st + (kGranule + h * piece) * D, static_cast<const char*>(A.cache.v) + at, piece * D, bar);
+                bulk_load(st + h * bytes, static_cast<const char*>(A.cache.k) + at, bytes, bar);
+                bulk_load(st + S::kKeys * D + h * bytes, static_cast<const char*>(A.cache.v) + at, bytes, bar);
             }
         }
     };
+#pragma unroll 1
     for (int i = 0; i < min(mine, S::kStages); i++) {
-        issue(i);
+        issue(i, (slot + i) % S::kStages);
     }
 
-    // queries: this lane's two rows of each tile, f16 relative to a power of two at the row's largest
-    uint32_t q[MT][D / 16][4];
-    float qs[MT][2];
-    int lo[MT][2], hi[MT][2];
+    // queries: lane n holds its dims of row 8 t + n, in terms; scores of rows 8 t + 2 c and the next come out in the lane
+    uint32_t q[NT][D / 16][kTerms];
+    float qs[NT][2];
+    int lo[NT][2], hi[NT][2];
 #pragma unroll
-    for (int t = 0; t < MT; t++) {
-#pragma unroll
-        for (int half = 0; half < 2; half++) {
-            const int r = r0 + t * 16 + half * 8 + n8;
-            float x[D / 16][4], top = 0.f;
-            lo[t][half] = hi[t][half] = 0;
-#pragma unroll
-            for (int k = 0; k < D / 16; k++) {
-                Vec<T, 4> v{};
-                if (r < r1) {
-                    v = *reinterpret_cast<const Vec<T, 4>*>(static_cast<const T*>(A.q) + (s.row0 + r / G) * A.qr + (head * G + r % G) * A.qh + 16 * k + 4 * c4);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    x[k][e] = to_f32(v.v[e]), top = fmaxf(top, fabsf(x[k][e]));
-                }
-            }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            int ex = 0;
-            if (top > 0.f && top <= 3.402823466e38f) {
-                frexpf(top, &ex);
-            }
-            ex = max(ex, -100);
-            const float down = ldexpf(1.f, -ex);
-            qs[t][half] = ldexpf(1.f, ex);
+    for (int t = 0; t < NT; t++) {
+        const int r = r0 + t * 8 + n8;
+        Vec<T, 4> v[D / 16] = {};
+        float top = 0.f;
+        if (r < r1) {
+            const T* from = static_cast<const T*>(A.q) + (s.row0 + r / G) * A.qr + (head * G + r % G) * A.qh + 4 * c4;
 #pragma unroll
             for (int k = 0; k < D / 16; k++) {
-                q[t][k][half] = pack_f16(x[k][0] * down, x[k][1] * down);
-                q[t][k][2 + half] = pack_f16(x[k][2] * down, x[k][3] * down);
-            }
-            if (r < r1) {
-                const int2 see = seen_by(A, s.place0 + r / G, s.len);
-                lo[t][half] = see.x, hi[t][half] = see.y;
+                v[k] = *reinterpret_cast<const Vec<T, 4>*>(from + 16 * k);
             }
         }
-    }
-
-    float o[MT][D / 8][4] = {}, m[MT][2], l[MT][2] = {};
-#pragma unroll
-    for (int t = 0; t < MT; t++) {
-        m[t][0] = m[t][1] = -INFINITY;
-    }
-    // where this lane's key of score tile 0 and its dim of value tile 0 lie in a stage
-    const int tok = 4 * (n8 >> 1) + (n8 & 1);
-    const uint32_t k_at = (tok >> 3) * 8 * D + (tok & 7) * 16 + 4 * c4, v_at = kGranule * D + n8 * 16 + 4 * c4;
-    for (int i = 0; i < mine; i++) {
-        if ((i * pieces) >> 5 != batch) {
-            now = next, batch++;
-            next = look_up(32 * (batch + 1));
-        }
-        float a[2], e[2], iv[2];
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int from = (i * pieces + (pieces == 2 ? h : 0)) & 31;
-            a[h] = __shfl_sync(0xffffffffu, now.a, from), e[h] = __shfl_sync(0xffffffffu, now.e, from), iv[h] = __shfl_sync(0xffffffffu, now.iv, from);
-        }
-        const uint32_t st = ring + i % S::kStages * S::kStage;
-        const int key0 = (ga + warp + i * kDecodeWarps) * kGranule;
-        if (!bar_wait(bars + i % S::kStages * 8, (i / S::kStages) & 1)) {
-            l[0][0] = l[0][1] = l[MT - 1][0] = l[MT - 1][1] = __int_as_float(0x7fffffff); // never the case; rows come out as NaN
-            break;
-        }
-        float x[MT][4][4] = {};
 #pragma unroll
         for (int k = 0; k < D / 16; k++) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                // tile j: keys 16 (j / 2) + 2 (j % 2) on from tile 0's; 2 (j % 2) stays inside a group of 8
-                uint32_t b0, b1;
-                unpack_e4m3(lds32(st + k_at + (j >> 1) * 16 * D + (j & 1) * 32 + k * 128), b0, b1);
-#pragma unroll
-                for (int t = 0; t < MT; t++) {
-                    mma_f16(x[t][j], q[t][k], b0, b1);
-                }
+            for (int e = 0; e < 4; e++) {
+                top = fmaxf(top, fabsf(to_f32(v[k].v[e])));
             }
         }
-        const bool whole = key0 >= keys.all_lo && key0 + kGranule <= keys.all_hi; // all rows see all keys
-        uint32_t p[MT][4][2];
-        bool grew = false;
-        float corr[MT][2];
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // 2^-ex brings the largest to [128, 256); an infinity makes the row NaN
+        const int ex = min(max((__float_as_int(top) >> 23) - 134, -118), 118);
+        const float down = top <= 3.402823466e38f ? exp2_int(-ex) : __int_as_float(0x7fffffff), up = exp2_int(ex);
 #pragma unroll
-        for (int t = 0; t < MT; t++) {
+        for (int k = 0; k < D / 16; k++) {
+            float4 x = make_float4(to_f32(v[k].v[0]) * down, to_f32(v[k].v[1]) * down, to_f32(v[k].v[2]) * down, to_f32(v[k].v[3]) * down);
 #pragma unroll
-            for (int half = 0; half < 2; half++) {
-                float top = -INFINITY;
+            for (int m = 0; m < kTerms; m++) {
+                q[t][k][m] = pack_e4m3(x.x, x.y, x.z, x.w);
+                const float4 y = codes_to_f32(q[t][k][m]);
+                x = make_float4((x.x - y.x) * 16.f, (x.y - y.y) * 16.f, (x.z - y.z) * 16.f, (x.w - y.w) * 16.f);
+            }
+        }
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
+        for (int h = 0; h < 2; h++) {
+            const int row = r0 + t * 8 + 2 * c4 + h;
+            qs[t][h] = __shfl_sync(0xffffffffu, up, 4 * (2 * c4 + h));
+            lo[t][h] = hi[t][h] = 0;
+            if (row < r1) {
+                const int2 see = seen_by(A, s.place0 + row / G, s.len);
+                lo[t][h] = see.x, hi[t][h] = see.y;
+            }
+        }
+    }
+
+    float o[D / 16][NT][4] = {}, base[NT][2], l[NT][2] = {};
 #pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        float& y = x[t][j][2 * half + c];
-                        y = fmaf(y, a[j >> 1] * qs[t][half], e[j >> 1]);
-                        if (!whole) {
-                            const int key = key0 + 16 * (j >> 1) + 4 * c4 + 2 * (j & 1) + c;
-                            y = key >= lo[t][half] && key < hi[t][half] ? y : -INFINITY;
+    for (int t = 0; t < NT; t++) {
+        base[t][0] = base[t][1] = kNoBase;
+    }
+    const int tok = 4 * (n8 >> 1) + (n8 & 1); // the first key of the lane's score rows
+    // the row of a stage that this lane names to ldmatrix: keys in the order of the score rows; dims
+    const int mk = 4 * ((lane & 7) >> 1) + (lane & 1) + 2 * (lane >> 3 & 1);
+    const uint32_t k_at = (mk >> 3) * 8 * D + (mk & 7) * 16 + (lane >> 4) * 128, v_at = S::kKeys * D + (lane >> 4) * 16 * D + (lane & 15) * 16;
+#pragma unroll 1
+    for (int i = 0; i < mine; i++) {
+        if ((i << pieces_shift) >> 5 != batch) {
+            now = next, batch++;
+            next = look_up(32 * (batch + 1));
+        }
+        float a[kTiles], e[kTiles], iv[kTiles];
+        uint32_t absent = 0;
+        if (pieces == 1) {
+            const float ks = __shfl_sync(0xffffffffu, now.ks, i & 31), vs = __shfl_sync(0xffffffffu, now.vs, i & 31);
+            absent = ks == ks ? 0u : ~0u;
+            a[0] = ks * A.scale_log2, e[0] = log2_fast(vs), iv[0] = inverse_fast(vs);
+#pragma unroll
+            for (int u = 1; u < kTiles; u++) {
+                a[u] = a[0], e[u] = e[0], iv[u] = iv[0];
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < kTiles; u++) {
+                const int from = ((i << pieces_shift) + (u * 16 >> piece_shift)) & 31;
+                const float ks = __shfl_sync(0xffffffffu, now.ks, from), vs = __shfl_sync(0xffffffffu, now.vs, from);
+                absent |= ks == ks ? 0u : 1u << u;
+                a[u] = ks * A.scale_log2, e[u] = log2_fast(vs), iv[u] = inverse_fast(vs);
+            }
+        }
+        const uint32_t st = ring + slot * S::kStage;
+        const int key0 = (ga + warp + i * kDecodeWarps) * S::kKeys;
+        if (!bar_wait(bars + slot * 8, phase)) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                l[t][0] = l[t][1] = __int_as_float(0x7fffffff); // a copy got lost: rows come out as NaN
+            }
+            break;
+        }
+        float x[kTiles][NT][4];
+        {
+            float z[kTerms][kTiles][NT][4] = {};
+#pragma unroll
+            for (int k = 0; k < D / 32; k++) {
+#pragma unroll
+                for (int u = 0; u < kTiles; u++) {
+                    uint32_t w[4];
+                    ldmatrix4(w, st + k_at + u * 16 * D + k * 256);
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+#pragma unroll
+                        for (int m = 0; m < kTerms; m++) {
+                            mma_e4m3(z[m][u][t], w, q[t][2 * k][m], q[t][2 * k + 1][m]);
                         }
-                        top = fmaxf(top, y);
                     }
                 }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float was = m[t][half], is = fmaxf(was, top), base = is == -INFINITY ? 0.f : is;
-                corr[t][half] = exp2_fast(was - base);
-                grew = grew || is > was;
-                m[t][half] = is;
-                float sum = 0.f;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const float p0 = exp2_fast(x[t][j][2 * half] - base), p1 = exp2_fast(x[t][j][2 * half + 1] - base);
-                    sum = fmaf(p0 + p1, iv[j >> 1], sum);
-                    p[t][j][half] = pack_f16(p0, p1);
-                }
-                l[t][half] = fmaf(l[t][half], corr[t][half], sum);
             }
-        }
-        if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-            for (int t = 0; t < MT; t++) {
+            for (int u = 0; u < kTiles; u++) {
 #pragma unroll
-                for (int d = 0; d < D / 8; d++) {
-                    o[t][d][0] *= corr[t][0], o[t][d][1] *= corr[t][0], o[t][d][2] *= corr[t][1], o[t][d][3] *= corr[t][1];
+                for (int t = 0; t < NT; t++) {
+#pragma unroll
+                    for (int v = 0; v < 4; v++) {
+                        float y = z[kTerms - 1][u][t][v];
+#pragma unroll
+                        for (int m = kTerms - 2; m >= 0; m--) {
+                            y = fmaf(y, 1.f / 16.f, z[m][u][t][v]);
+                        }
+                        x[u][t][v] = y * (a[u] * qs[t][v & 1]);
+                    }
                 }
             }
         }
-        const bool ragged = key0 < keys.lo || key0 + kGranule > keys.hi || a[0] != a[0] || a[1] != a[1];
+        // masked scores are -inf
+        if (key0 < keys.all_lo || key0 + S::kKeys > keys.all_hi) {
 #pragma unroll
-        for (int g = 0; g < 2; g++) {
+            for (int u = 0; u < kTiles; u++) {
 #pragma unroll
-            for (int d = 0; d < D / 8; d++) {
-                uint32_t w = lds32(st + v_at + g * 16 * D + d * 128), b0, b1;
-                if (ragged) {
-                    w = a[g] == a[g] ? keep_keys(w, key0 + 16 * g + 4 * c4, keys.lo, keys.hi) : 0u;
+                for (int t = 0; t < NT; t++) {
+#pragma unroll
+                    for (int v = 0; v < 4; v++) {
+                        const int key = key0 + 16 * u + tok + (v & 2);
+                        x[u][t][v] = key >= lo[t][v & 1] && key < hi[t][v & 1] ? x[u][t][v] : -INFINITY;
+                    }
                 }
-                unpack_e4m3(w, b0, b1);
+            }
+        }
+        uint32_t p[kTiles][NT][2];
 #pragma unroll
-                for (int t = 0; t < MT; t++) {
-                    const uint32_t pa[4] = {p[t][2 * g][0], p[t][2 * g][1], p[t][2 * g + 1][0], p[t][2 * g + 1][1]};
-                    mma_f16(o[t][d], pa, b0, b1);
+        for (int t = 0; t < NT; t++) {
+            float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int u = 0; u < kTiles; u++) {
+#pragma unroll
+                for (int v = 0; v < 4; v++) {
+                    x[u][t][v] += e[u];
+                    top[v & 1] = fmaxf(top[v & 1], x[u][t][v]);
+                }
+            }
+            if (__any_sync(0xffffffffu, top[0] > base[t][0] + kSlack || top[1] > base[t][1] + kSlack)) {
+                float corr[2];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const float was = base[t][h];
+#pragma unroll
+                    for (int w = 4; w <= 16; w *= 2) {
+                        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], w));
+                    }
+                    base[t][h] = fmaxf(was, top[h] - kHeadroom);
+                    corr[h] = exp2_fast(was - base[t][h]);
+                    l[t][h] *= corr[h];
+                }
+#pragma unroll
+                for (int d = 0; d < D / 16; d++) {
+                    o[d][t][0] *= corr[0], o[d][t][1] *= corr[1], o[d][t][2] *= corr[0], o[d][t][3] *= corr[1];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kTiles; u++) {
+                const float p0 = exp2_fast(x[u][t][0] - base[t][0]), p1 = exp2_fast(x[u][t][1] - base[t][1]);
+                const float p2 = exp2_fast(x[u][t][2] - base[t][0]), p3 = exp2_fast(x[u][t][3] - base[t][1]);
+                l[t][0] = fmaf(p0 + p2, iv[u], l[t][0]), l[t][1] = fmaf(p1 + p3, iv[u], l[t][1]);
+                p[u][t][0] = transpose8(pack_f16(p0, p1)), p[u][t][1] = transpose8(pack_f16(p2, p3));
+            }
+        }
+        if (key0 < keys.lo || key0 + S::kKeys > keys.hi || absent) {
+            clear_values<D, S::kKeys>(st + S::kKeys * D, keys.lo - key0, keys.hi - key0, absent);
+        }
+#pragma unroll
+        for (int u = 0; u < kTiles; u += 2) {
+#pragma unroll
+            for (int d = 0; d < D / 16; d++) {
+                uint32_t w[4], f[2][4]; // 16 dims of 32 keys; as f16, of 16 keys each
+                ldmatrix4(w, st + v_at + u * 16 * D + d * 256);
+                unpack_e4m3(w[0], f[0][0], f[0][2]), unpack_e4m3(w[1], f[0][1], f[0][3]);
+                unpack_e4m3(w[2], f[1][0], f[1][2]), unpack_e4m3(w[3], f[1][1], f[1][3]);
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    mma_f16(o[d][t], f[0], p[u][t][0], p[u][t][1]);
+                    mma_f16(o[d][t], f[1], p[u + 1][t][0], p[u + 1][t][1]);
                 }
             }
         }
         __syncwarp(); // the stage has been read
         if (i + S::kStages < mine) {
-            issue(i + S::kStages);
+            issue(i + S::kStages, slot);
+        }
+        if (++slot == S::kStages) {
+            slot = 0, phase ^= 1;
         }
     }
 
     // the warps' shares together, through the ring
-    constexpr int kPitch = D + 4, kRows = 16 * MT;
+    constexpr int kPitch = D + 4;
     static_assert(kDecodeWarps * kRows * (kPitch + 2) * 4 <= S::kRing, "the shares fit the ring");
     float* so = reinterpret_cast<float*>(smem);
     float* sm = so + kDecodeWarps * kRows * kPitch;
     __syncthreads();
 #pragma unroll
-    for (int t = 0; t < MT; t++) {
+    for (int t = 0; t < NT; t++) {
 #pragma unroll
-        for (int half = 0; half < 2; half++) {
-            float sum = l[t][half];
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            const int row = warp * kRows + t * 16 + half * 8 + n8;
-            if (c4 == 0) {
-                sm[2 * row] = m[t][half], sm[2 * row + 1] = sum;
+        for (int h = 0; h < 2; h++) {
+            float sum = l[t][h];
+#pragma unroll
+            for (int w = 4; w <= 16; w *= 2) {
+                sum += __shfl_xor_sync(0xffffffffu, sum, w);
+            }
+            const int row = warp * kRows + t * 8 + 2 * c4 + h;
+            if (n8 == 0) {
+                sm[2 * row] = base[t][h], sm[2 * row + 1] = sum;
             }
 #pragma unroll
-            for (int d = 0; d < D / 8; d++) {
-                *reinterpret_cast<float2*>(so + row * kPitch + 8 * d + 2 * c4) = make_float2(o[t][d][2 * half], o[t][d][2 * half + 1]);
+            for (int d = 0; d < D / 16; d++) {
+                so[row * kPitch + 16 * d + n8] = o[d][t][h], so[row * kPitch + 16 * d + 8 + n8] = o[d][t][2 + h];
             }
         }
     }
     __syncthreads();
-    const bool alone = chunks_of(A, keys) <= 1; // what it has is the result
-    constexpr int kLanes = D / 4;                // threads of a row, four dims each
-    for (int i = threadIdx.x; i < (r1 - r0) * kLanes; i += kDecodeWarps * 32) {
-        const int r = i / kLanes, d = i % kLanes * 4, row = r0 + r;
-        float top = -INFINITY, sum = 0.f;
+    constexpr int kLanes = D / 4; // threads of a row, four dims each
+#pragma unroll 1
+    for (int i = threadIdx.x; i < own.rows * kLanes; i += kDecodeWarps * 32) {
+        const int r = i / kLanes, d = i % kLanes * 4;
+        float top = kNoBase, sum = 0.f;
 #pragma unroll
         for (int w = 0; w < kDecodeWarps; w++) {
             top = fmaxf(top, sm[2 * (w * kRows + r)]);
         }
-        const float base = top == -INFINITY ? 0.f : top;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < kDecodeWarps; w++) {
-            const float f = exp2_fast(sm[2 * (w * kRows + r)] - base);
+            const float f = exp2_fast(sm[2 * (w * kRows + r)] - top);
             const float4 z = *reinterpret_cast<const float4*>(so + (w * kRows + r) * kPitch + d);
             sum = fmaf(sm[2 * (w * kRows + r) + 1], f, sum);
             y.x = fmaf(z.x, f, y.x), y.y = fmaf(z.y, f, y.y), y.z = fmaf(z.z, f, y.z), y.w = fmaf(z.w, f, y.w);
         }
-        const int64_t at = int64_t(s.row0 + row / G) * A.q_heads + head * G + row % G;
         if (alone) {
-            store_out<T>(A, s.row0 + row / G, head * G + row % G, d, y, top, sum);
+            store_out<T>(A, s.row0 + (r0 + r) / G, head * G + (r0 + r) % G, d, y, top, sum);
         } else {
-            const int64_t part = int64_t(split) * A.batch.rows * A.q_heads + at;
-            *reinterpret_cast<float4*>(A.part_o + part * D + d) = y;
+            *reinterpret_cast<float4*>(A.part_o + (int64_t(part) * kRows + r) * D + d) = y;
             if (d == 0) {
-                *reinterpret_cast<float2*>(A.part_ml + 2 * part) = make_float2(top, sum);
+                *reinterpret_cast<float2*>(A.part_ml + 2 * (int64_t(part) * kRows + r)) = make_float2(top, sum);
             }
         }
     }
+    if (!A.part_o) {
+        return;
+    }
+    __syncthreads(); // the ring is free again
+    left -= gb - ga, done = 0;
+    if (++head == H) {
+        head = 0, tile++;
+    }
+    }
 }
 
-// The chunks of a row together. A warp takes a (row, query head); tile_rows is the first kernel's.
+// The shares of a unit together: a block takes (unit, row), its warps every eighth share
+constexpr int kMergeWarps = 8;
 template <class T>
-__global__ void __launch_bounds__(128) merge_kernel(const AttentionArgs A, int tile_rows) {
+__global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const AttentionArgs A, int shares) {
+    __shared__ float4 so[kMergeWarps][32];
+    __shared__ float2 sm[kMergeWarps];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = A.cache.dim, H = A.cache.heads;
+    const int tile = blockIdx.x / H, head = blockIdx.x % H, r = blockIdx.y;
+    const Tile own = tile_at(A, tile);
+    int64_t c0 = 0, c1 = 0;
+    if (r < own.rows) { // from the call's inputs alone, while the shares are still being worked on
+        const Line line = line_of(A, [&](int64_t, int, int i, int64_t) { return i == tile; });
+        const int g = granules_of(A, tile);
+        const int64_t size = share_size(line.total * H, shares), start = line.start * H + int64_t(head) * g;
+        c0 = start / size, c1 = (start + g - 1) / size;
+    }
     wait_for_previous();
-    const int lane = threadIdx.x & 31, D = A.cache.dim, G = A.group;
-    const int64_t item = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    const int j = int(item % A.q_heads), b = int(item / A.q_heads / A.batch.max_new), i = int(item / A.q_heads % A.batch.max_new);
-    if (b >= A.batch.sequences) {
+    if (c0 == c1) {
         return;
     }
-    const Sequence s = sequence_of(A.batch, b);
-    if (i >= s.rows) {
-        return;
-    }
-    const int r = i * G + j % G, r0 = r / tile_rows * tile_rows;
-    const TileKeys keys = keys_of_tile(A, s, r0, min(r0 + tile_rows, s.rows * G));
-    const int n = chunks_of(A, keys);
-    if (n <= 1 || 4 * lane >= D) {
-        return;
-    }
-    const int64_t at = int64_t(s.row0 + i) * A.q_heads + j, step = int64_t(A.batch.rows) * A.q_heads;
-    float top = -INFINITY, sum = 0.f;
+    float top = kNoBase, sum = 0.f;
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = 0; c < n; c++) {
-        const float2 ml = *reinterpret_cast<const float2*>(A.part_ml + 2 * (at + c * step));
-        const float4 z = *reinterpret_cast<const float4*>(A.part_o + (at + c * step) * D + 4 * lane);
-        const float is = fmaxf(top, ml.x), base = is == -INFINITY ? 0.f : is;
-        const float f = exp2_fast(top - base), g = exp2_fast(ml.x - base);
-        top = is, sum = sum * f + ml.y * g;
-        y.x = y.x * f + z.x * g, y.y = y.y * f + z.y * g, y.z = y.z * f + z.z * g, y.w = y.w * f + z.w * g;
+#pragma unroll 4
+    for (int64_t c = c0 + warp; c <= c1; c += kMergeWarps) {
+        const int64_t at = (2 * c + (c == c0 ? 1 : 0)) * A.tile_rows + r;
+        const float2 ml = *reinterpret_cast<const float2*>(A.part_ml + 2 * at);
+        const float4 z = 4 * lane < D ? *reinterpret_cast<const float4*>(A.part_o + at * D + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float is = fmaxf(top, ml.x), f = exp2_fast(top - is), w = exp2_fast(ml.x - is);
+        top = is, sum = sum * f + ml.y * w;
+        y.x = y.x * f + z.x * w, y.y = y.y * f + z.y * w, y.z = y.z * f + z.z * w, y.w = y.w * f + z.w * w;
     }
-    store_out<T>(A, s.row0 + i, j, 4 * lane, y, top, sum);
+    so[warp][lane] = y;
+    if (lane == 0) {
+        sm[warp] = make_float2(top, sum);
+    }
+    __syncthreads();
+    if (warp != 0 || 4 * lane >= D) {
+        return;
+    }
+    top = kNoBase, sum = 0.f, y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kMergeWarps; w++) {
+        top = fmaxf(top, sm[w].x);
+    }
+#pragma unroll
+    for (int w = 0; w < kMergeWarps; w++) {
+        const float f = exp2_fast(sm[w].x - top);
+        const float4 z = so[w][lane];
+        sum = fmaf(sm[w].y, f, sum);
+        y.x = fmaf(z.x, f, y.x), y.y = fmaf(z.y, f, y.y), y.z = fmaf(z.z, f, y.z), y.w = fmaf(z.w, f, y.w);
+    }
+    store_out<T>(A, own.s.row0 + (own.r0 + r) / A.group, head * A.group + (own.r0 + r) % A.group, 4 * lane, y, top, sum);
 }
 
 } // namespace seq

@@ -209,69 +209,70 @@ cudaError_t launch_append(cudaStream_t st, const AppendArgs& a, int v, unsigned 
     }
 }
 
-// How an attention call is cut up
+// How an attention call is cut up: whole units, a block each, or equal shares of the line of all units
 struct Plan {
-    int mt;        // tiles of 16 rows a warp keeps
-    int row_tiles; // of 16 mt rows
-    int splits, chunk;
+    int nt;        // tiles of 8 rows a warp keeps
+    int row_tiles; // of 8 nt rows
+    int64_t blocks;
+    bool shares;
     size_t part_bytes, bytes; // of the workspace
 };
 Plan make_plan(const cck_cache& c, const cck_batch& b, int q_heads, int sms) {
     Plan p{};
     const int64_t rows = int64_t(b.max_new) * (q_heads / c.heads);
-    p.mt = rows > 16 ? 2 : 1;
-    p.row_tiles = int((rows + 16 * p.mt - 1) / (16 * p.mt));
-    const int64_t units = int64_t(b.sequences) * c.heads * p.row_tiles, slots = 2 * sms;
-    int64_t splits = units ? (2 * slots + units - 1) / units : 1;
-    const int64_t most = (int64_t(b.max_len) + 255) / 256;
-    splits = splits < most ? splits : most;
-    p.splits = int(splits < 1 ? 1 : splits);
-    p.chunk = int((int64_t(b.max_len) + p.splits - 1) / p.splits + kGranule - 1) / kGranule * kGranule + kGranule;
-    if (p.splits > 1) {
-        p.part_bytes = size_t(p.splits) * b.rows * q_heads * c.dim * 4;
-        p.bytes = p.part_bytes + size_t(p.splits) * b.rows * q_heads * 8;
+    p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+    p.row_tiles = int((rows + 8 * p.nt - 1) / (8 * p.nt));
+    const int64_t units = int64_t(b.sequences) * c.heads * p.row_tiles, slots = (p.nt == 1 ? 3 : 2) * sms;
+    const int64_t granules = int64_t(b.max_len) / granule_of(c.dim) + 2;
+    p.shares = granules > 4 * kDecodeWarps; // a share has two granules a warp at least
+    const int64_t most = (units * granules + 2 * kDecodeWarps - 1) / (2 * kDecodeWarps);
+    p.blocks = !p.shares ? units : most < slots ? most : slots;
+    if (p.shares) {
+        p.part_bytes = size_t(2 * p.blocks) * 8 * p.nt * c.dim * 4;
+        p.bytes = p.part_bytes + size_t(2 * p.blocks) * 8 * p.nt * 8;
     }
     return p;
 }
-template <class T, int D, int MT>
+template <class T, int D, int NT>
 cudaError_t launch_decode(cudaStream_t st, const AttentionArgs& a, unsigned blocks) {
     static std::atomic<bool> ready[kMaxDevices];
     int dev = 0;
     cudaGetDevice(&dev);
     if (!ready[dev].load(std::memory_order_relaxed)) {
-        if (cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(decode_kernel<T, D, MT>), cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeShape<D>::kSmem)) {
+        if (cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(decode_kernel<T, D, NT>), cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeShape<D, NT>::kSmem)) {
             return e;
         }
         ready[dev].store(true, std::memory_order_relaxed);
     }
-    decode_kernel<T, D, MT><<<blocks, kDecodeWarps * 32, DecodeShape<D>::kSmem, st>>>(a);
+    decode_kernel<T, D, NT><<<blocks, kDecodeWarps * 32, DecodeShape<D, NT>::kSmem, st>>>(a);
     return cudaGetLastError();
 }
-template <class T, int MT>
+template <class T, int NT>
 cudaError_t launch_decode(cudaStream_t st, const AttentionArgs& a, unsigned blocks) {
     switch (a.cache.dim) {
-    case 32: return launch_decode<T, 32, MT>(st, a, blocks);
-    case 64: return launch_decode<T, 64, MT>(st, a, blocks);
-    case 96: return launch_decode<T, 96, MT>(st, a, blocks);
-    default: return launch_decode<T, 128, MT>(st, a, blocks);
+    case 32: return launch_decode<T, 32, NT>(st, a, blocks);
+    case 64: return launch_decode<T, 64, NT>(st, a, blocks);
+    case 96: return launch_decode<T, 96, NT>(st, a, blocks);
+    default: return launch_decode<T, 128, NT>(st, a, blocks);
     }
 }
 template <class T>
 cudaError_t launch_attention(cudaStream_t st, const AttentionArgs& a, const Plan& p) {
-    const unsigned blocks = unsigned(int64_t(a.batch.sequences) * a.cache.heads * p.row_tiles * p.splits);
-    if (cudaError_t e = p.mt == 1 ? launch_decode<T, 1>(st, a, blocks) : launch_decode<T, 2>(st, a, blocks)) {
+    const unsigned blocks = unsigned(p.blocks);
+    if (cudaError_t e = p.nt == 1 ? launch_decode<T, 1>(st, a, blocks) : p.nt == 2 ? launch_decode<T, 2>(st, a, blocks) : launch_decode<T, 4>(st, a, blocks)) {
         return e;
     }
-    if (p.splits == 1) {
+    if (!p.shares) {
         return cudaSuccess;
     }
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute dependent;
     dependent.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     dependent.val.programmaticStreamSerializationAllowed = 1;
-    const int64_t items = int64_t(a.batch.sequences) * a.batch.max_new * a.q_heads;
-    cfg.gridDim = dim3(unsigned((items + 3) / 4)), cfg.blockDim = dim3(128), cfg.stream = st, cfg.attrs = &dependent, cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, merge_kernel<T>, a, 16 * p.mt);
+    const int64_t rows = int64_t(a.batch.max_new) * a.group;
+    cfg.gridDim = dim3(unsigned(int64_t(a.batch.sequences) * a.row_tiles * a.cache.heads), unsigned(rows < a.tile_rows ? rows : a.tile_rows));
+    cfg.blockDim = dim3(kMergeWarps * 32), cfg.stream = st, cfg.attrs = &dependent, cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, merge_kernel<T>, a, int(blocks));
 }
 
 } // namespace
@@ -412,7 +413,7 @@ int cck_cache_attention(void* stream, const cck_cache* cache, const cck_batch* b
     if (ws_bytes < p.bytes || (p.bytes && (!ws || !aligned(ws, 16)))) {
         return refuse(CCK_E_WORKSPACE, op, "the workspace is too small, null or not aligned");
     }
-    if (int64_t(batch->sequences) * cache->heads * p.row_tiles * p.splits > 0x7fffffff) {
+    if (int64_t(batch->sequences) * cache->heads * p.row_tiles > 0x7fffffff) {
         return refuse(CCK_E_SHAPE, op, "too many rows for one launch");
     }
     AttentionArgs a{};
@@ -420,8 +421,9 @@ int cck_cache_attention(void* stream, const cck_cache* cache, const cck_batch* b
     a.qr = q->row_stride, a.qh = q->head_stride, a.or_ = out->row_stride, a.oh = out->head_stride;
     a.scale_log2 = softmax_scale * 1.4426950408889634f;
     a.q_heads = q->heads, a.group = q->heads / cache->heads, a.causal = causal != 0, a.window = window;
-    a.row_tiles = p.row_tiles, a.splits = p.splits, a.chunk = p.chunk;
-    if (p.splits > 1) {
+    a.granule = granule_of(cache->dim), a.page_shift = __builtin_ctz(cache->page_tokens);
+    a.tile_rows = 8 * p.nt, a.row_tiles = p.row_tiles;
+    if (p.shares) {
         a.part_o = static_cast<float*>(ws), a.part_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + p.part_bytes);
     }
     const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -130,6 +130,7 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 }
 // Waits for the phase with this parity; gives up (false) after about a second, which nothing but a lost copy can cause.
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+#pragma unroll 1
     for (int i = 0; i < 1 << 18; i++) {
         uint32_t ok;
         asm volatile(
