@@ -605,58 +605,71 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DecodeShape<D, NT>::kBlocks
     }
 }
 
-// The shares of a unit together: a block takes (unit, row), its warps every eighth share
+// The shares of a unit together. Blocks x are the shares: the unit that begins in the share and goes on in the next. Its rows are dealt
+// out to the blocks y and to the warps, or, where there are many shares, the shares of a row to the warps.
 constexpr int kMergeWarps = 8;
 template <class T>
-__global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const AttentionArgs A, int shares) {
+__global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const AttentionArgs A) {
     __shared__ float4 so[kMergeWarps][32];
     __shared__ float2 sm[kMergeWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = A.cache.dim, H = A.cache.heads;
-    const int tile = blockIdx.x / H, head = blockIdx.x % H, r = blockIdx.y;
-    const Tile own = tile_at(A, tile);
-    int64_t c0 = 0, c1 = 0;
-    if (r < own.rows) { // from the call's inputs alone, while the shares are still being worked on
-        const Line line = line_of(A, [&](int64_t, int, int i, int64_t) { return i == tile; });
-        const int g = granules_of(A, tile);
-        const int64_t size = share_size(line.total * H, shares), start = line.start * H + int64_t(head) * g;
-        c0 = start / size, c1 = (start + g - 1) / size;
+    // from the call's inputs alone, while the shares are still being worked on
+    int64_t size = 0, last = 0; // granules of a share; this one's last
+    const Line line = line_of(A, [&](int64_t start, int g, int, int64_t total) {
+        size = share_size(total * H, gridDim.x), last = size * (blockIdx.x + 1) - 1;
+        return start * H <= last && last < (start + g) * H;
+    });
+    size = share_size(line.total * H, gridDim.x), last = size * (blockIdx.x + 1) - 1;
+    int rows = 0, head = 0;
+    int64_t c1 = 0;
+    Tile own{};
+    if (last < line.total * H) {
+        const int g = granules_of(A, line.tile);
+        head = int((last - line.start * H) / g);
+        const int64_t start = line.start * H + int64_t(head) * g, end = start + g;
+        if (start > last - size && end > last + 1) {
+            own = tile_at(A, line.tile), rows = own.rows, c1 = (end - 1) / size;
+        }
     }
     wait_for_previous();
-    if (c0 == c1) {
-        return;
-    }
-    float top = kNoBase, sum = 0.f;
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int64_t c0 = blockIdx.x;
+    const bool together = c1 - c0 >= 2 * kMergeWarps; // a row by all warps
+    const int stride = together ? gridDim.y : gridDim.y * kMergeWarps;
+#pragma unroll 1
+    for (int r = together ? blockIdx.y : blockIdx.y * kMergeWarps + warp; r < rows; r += stride) {
+        float top = kNoBase, sum = 0.f;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int64_t c = c0 + warp; c <= c1; c += kMergeWarps) {
-        const int64_t at = (2 * c + (c == c0 ? 1 : 0)) * A.tile_rows + r;
-        const float2 ml = *reinterpret_cast<const float2*>(A.part_ml + 2 * at);
-        const float4 z = 4 * lane < D ? *reinterpret_cast<const float4*>(A.part_o + at * D + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
-        const float is = fmaxf(top, ml.x), f = exp2_fast(top - is), w = exp2_fast(ml.x - is);
-        top = is, sum = sum * f + ml.y * w;
-        y.x = y.x * f + z.x * w, y.y = y.y * f + z.y * w, y.z = y.z * f + z.z * w, y.w = y.w * f + z.w * w;
+        for (int64_t c = together ? c0 + warp : c0; c <= c1; c += together ? kMergeWarps : 1) {
+            const int64_t at = (2 * c + (c == c0 ? 1 : 0)) * A.tile_rows + r;
+            const float2 ml = *reinterpret_cast<const float2*>(A.part_ml + 2 * at);
+            const float4 z = 4 * lane < D ? *reinterpret_cast<const float4*>(A.part_o + at * D + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float is = fmaxf(top, ml.x), f = exp2_fast(top - is), w = exp2_fast(ml.x - is);
+            top = is, sum = sum * f + ml.y * w;
+            y.x = y.x * f + z.x * w, y.y = y.y * f + z.y * w, y.z = y.z * f + z.z * w, y.w = y.w * f + z.w * w;
+        }
+        if (together) {
+            so[warp][lane] = y;
+            if (lane == 0) {
+                sm[warp] = make_float2(top, sum);
+            }
+            __syncthreads();
+            top = kNoBase, sum = 0.f, y = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int w = 0; w < kMergeWarps; w++) {
+                top = fmaxf(top, sm[w].x);
+            }
+            for (int w = 0; w < kMergeWarps; w++) {
+                const float f = exp2_fast(sm[w].x - top);
+                const float4 z = so[w][lane];
+                sum = fmaf(sm[w].y, f, sum);
+                y.x = fmaf(z.x, f, y.x), y.y = fmaf(z.y, f, y.y), y.z = fmaf(z.z, f, y.z), y.w = fmaf(z.w, f, y.w);
+            }
+            __syncthreads();
+        }
+        if (4 * lane < D && (!together || warp == 0)) {
+            store_out<T>(A, own.s.row0 + (own.r0 + r) / A.group, head * A.group + (own.r0 + r) % A.group, 4 * lane, y, top, sum);
+        }
     }
-    so[warp][lane] = y;
-    if (lane == 0) {
-        sm[warp] = make_float2(top, sum);
-    }
-    __syncthreads();
-    if (warp != 0 || 4 * lane >= D) {
-        return;
-    }
-    top = kNoBase, sum = 0.f, y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < kMergeWarps; w++) {
-        top = fmaxf(top, sm[w].x);
-    }
-#pragma unroll
-    for (int w = 0; w < kMergeWarps; w++) {
-        const float f = exp2_fast(sm[w].x - top);
-        const float4 z = so[w][lane];
-        sum = fmaf(sm[w].y, f, sum);
-        y.x = fmaf(z.x, f, y.x), y.y = fmaf(z.y, f, y.y), y.z = fmaf(z.z, f, y.z), y.w = fmaf(z.w, f, y.w);
-    }
-    store_out<T>(A, own.s.row0 + (own.r0 + r) / A.group, head * A.group + (own.r0 + r) % A.group, 4 * lane, y, top, sum);
 }
 
 } // namespace seq

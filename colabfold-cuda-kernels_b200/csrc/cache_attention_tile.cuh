@@ -1,0 +1,655 @@
+// Attention over the paged 8-bit cache for many rows: prompts and pieces of them. The mathematics are cache_attention.cuh's.
+//
+// Bound by the tensor cores and by the exponentials, which take as long: for 256 rows and 128 keys of 128 dims 2048 cycles of
+// tcgen05.mma and 2048 of the special function units. A block of threads keeps two tiles of 128 rows, so that one's products run
+// beside the other's exponentials:
+//   warps 0-3, 4-7   softmax of tile 0, 1: a thread owns a row, S comes from and p goes to tensor memory
+//   warp 8           loads: pages as they lie into the rings (one bulk copy a page: the cache's layout is the operand's), their scales
+//   warp 9           issues the products
+//   warps 12-15      V to f16
+// S = q K^T is kind::f8f6f4 on the codes, q in terms of 4 bits, two of a bf16 and three of an f16 (as in cache_attention.cuh, but into
+// one accumulator: a term's last bit is 2^-17 of the row's largest): no work for K at all, in the time that f16 would take.
+// O += p V is kind::f16 for the sake of p's range, p read from tensor memory, where it takes S's place. Tensor memory: S 2 x 128
+// columns, O 2 x dim.
+#pragma once
+
+#include "cache_attention.cuh"
+
+namespace cck {
+namespace seq {
+
+constexpr int kTileKeys = 128, kTileRows = 128, kUnitRows = 2 * kTileRows, kTileThreads = 512;
+
+template <class T, int D>
+struct TileShape {
+    static constexpr int kTerms = T_is_f16<T>() ? 3 : 2;
+    static constexpr int kQ = kTileRows * D;          // bytes of a term of a tile
+    static constexpr int kCodes = kTileKeys * D;      // bytes of the codes of K or V
+    static constexpr int kKStages = kTerms == 3 ? 2 : 3, kVStages = 2, kHStages = 2; // K; V; V in f16
+    static constexpr int kOffK = 2 * kTerms * kQ, kOffV = kOffK + kKStages * kCodes, kOffH = kOffV + kVStages * kCodes;
+    static constexpr int kOffCtl = kOffH + kHStages * 2 * kCodes;
+    static constexpr int kSmem = kOffCtl + 2048;
+    static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+// A tile's scales are read until its softmax is done. The loads of tile j wait for V of j - 3 to be converted, that for p V of j - 5: they are at
+// most 5 tiles ahead, and a slot's next phase cannot end before its last one has been waited for.
+constexpr int kScaleSlots = 8;
+struct TileScale {
+    float a, e, iv, none;
+};
+struct TileCtl {
+    uint64_t q_full[2], k_full[3], k_empty[3], v_full[2], v_empty[2], h_full[2], h_empty[2], s_full[2], p_full[2], o_done[2];
+    uint64_t scale_full[kScaleSlots];
+    TileScale scale[kScaleSlots][kTileKeys / 16];
+    uint32_t absent[kScaleSlots]; // a bit for each 16 keys whose page is not there, or that nobody sees
+    uint32_t tmem;
+    int abort;
+};
+static_assert(sizeof(TileCtl) <= 2048, "control block");
+
+// A wait that gives up after about a second, which nothing but a lost copy can cause; then every later one returns at once
+__device__ __forceinline__ void tile_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+    const uint32_t b = shared_u32(bar);
+#pragma unroll 1
+    for (int i = 0; i < 1 << 18; i++) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(b), "r"(parity), "r"(4000)
+            : "memory");
+        if (ok) {
+            return;
+        }
+        if (*abort) {
+            return;
+        }
+    }
+    *abort = 1;
+}
+// position in a ring
+template <int N>
+struct Ring {
+    int i = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void next() {
+        if (++i == N) {
+            i = 0, phase ^= 1;
+        }
+    }
+};
+
+// ---- tensor memory and tcgen05
+__device__ __forceinline__ void tm_ld32(uint32_t at, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(at)
+        : "memory");
+}
+// waits for the thread's loads; the registers pass through so that no use of them moves before it
+__device__ __forceinline__ void tm_ld_wait(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tm_st32(uint32_t at, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+        "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void tm_st_wait() {
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tm_fence_before() {
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tm_fence_after() {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+// Shared-memory descriptor of a K-major operand in core matrices of 8 rows x 16 bytes without a swizzle: `lead` bytes to the next 16
+// bytes along k, `stride` to the next 8 rows. Start address >> 4 in bits [0,14), lead >> 4 in [16,30), stride >> 4 in [32,46), version 1
+// in [46,48), no swizzle: 0 in [61,64).
+__device__ __forceinline__ uint64_t tile_desc(uint32_t at, uint32_t lead, uint32_t stride) {
+    return uint64_t((at & 0x3FFFFu) >> 4) | uint64_t(lead >> 4) << 16 | uint64_t(stride >> 4) << 32 | uint64_t(1) << 46;
+}
+// f32 accumulator (bits [4,6) = 1), M >> 4 in [24,29), N >> 3 in [17,23), both operands K-major; the types' fields are 0: e4m3 of
+// kind::f8f6f4, f16 of kind::f16
+__device__ __forceinline__ uint32_t tile_idesc(int m, int n) {
+    return 1u << 4 | uint32_t(n >> 3) << 17 | uint32_t(m >> 4) << 24;
+}
+__device__ __forceinline__ uint32_t elected() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e;
+}
+__device__ __forceinline__ void mma_codes(uint32_t el, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(el)
+        : "memory");
+}
+__device__ __forceinline__ void mma_halves(uint32_t el, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(el)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t el, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(shared_u32(bar)),
+        "r"(el)
+        : "memory");
+}
+
+// What a block works on, unit after unit; every role goes through the same ones
+struct Segment {
+    int b, head, r0, rows; // sequence; rows of the unit
+    Sequence s;
+    TileKeys keys;
+    int ga, gb;     // tiles of keys
+    bool alone;     // the whole unit
+    int part;       // slot of the workspace, where it is not
+};
+struct Worker {
+    int64_t left = 1, done = 0;
+    int tile, head;
+    __device__ __forceinline__ Worker(const AttentionArgs& A) {
+        const int H = A.cache.heads;
+        // units of long sequences' last rows first: they see the most keys
+        tile = A.batch.sequences * A.row_tiles - 1 - blockIdx.x / H, head = blockIdx.x % H;
+        if (A.part_o) {
+            int64_t from = 0;
+            const Line line = line_of(A, [&](int64_t start, int g, int, int64_t total) {
+                from = share_size(total * H, gridDim.x) * blockIdx.x;
+                return start * H <= from && from < (start + g) * H;
+            });
+            const int64_t size = share_size(line.total * H, gridDim.x);
+            from = size * blockIdx.x, left = min(size, line.total * H - from);
+            if (left > 0) {
+                tile = line.tile;
+                const int g = granules_of(A, tile);
+                head = int((from - line.start * H) / g), done = from - line.start * H - int64_t(head) * g;
+            }
+        }
+    }
+    __device__ __forceinline__ bool next(const AttentionArgs& A, Segment& g) {
+        const int H = A.cache.heads;
+        Tile own;
+        while (left > 0) {
+            own = tile_at(A, tile);
+            if (own.rows > 0) {
+                break;
+            }
+            if (!A.part_o) {
+                left = 0;
+            }
+            tile++, head = 0;
+        }
+        if (left <= 0) {
+            return false;
+        }
+        g.s = own.s, g.b = tile / A.row_tiles, g.head = head, g.r0 = own.r0, g.rows = own.rows;
+        g.keys = keys_of_tile(A, own.s, own.r0, own.r0 + own.rows);
+        const int all = max(1, g.keys.g1 - g.keys.g0);
+        g.ga = g.keys.g0 + int(done), g.gb = A.part_o ? int(min(int64_t(g.keys.g0 + all), g.ga + left)) : g.keys.g0 + all;
+        g.alone = g.ga == g.keys.g0 && g.gb == g.keys.g0 + all, g.part = 2 * blockIdx.x + (g.ga == g.keys.g0 ? 1 : 0);
+        if (A.part_o) {
+            left -= g.gb - g.ga, done = 0;
+            if (++head == H) {
+                head = 0, tile++;
+            }
+        } else {
+            left = 0;
+        }
+        return true;
+    }
+};
+
+template <class T, int D>
+__device__ __forceinline__ void tile_softmax(const AttentionArgs& A, unsigned char* smem, TileCtl* ctl) {
+    using S = TileShape<T, D>;
+    const int t = threadIdx.x >> 7, row = threadIdx.x & 127;
+    const uint32_t lanes = uint32_t(row & ~31) << 16, ts = ctl->tmem + lanes + t * 128, to = ctl->tmem + lanes + 256 + t * 128;
+    Worker work(A);
+    Segment g;
+    uint32_t step = 0; // tiles of keys so far
+    uint32_t s_phase = 0, o_phase = 0;
+#pragma unroll 1
+    while (work.next(A, g)) {
+        const int n = g.gb - g.ga;
+        if (t * kTileRows >= g.rows) { // the unit has no second tile
+            step += n;
+            continue;
+        }
+        const int r = g.r0 + t * kTileRows + row, r1 = g.r0 + g.rows, rt = g.r0 + t * kTileRows;
+        // queries in terms; a row that is not there is zero
+        float up = 0.f;
+        {
+            Vec<T, 8> v[D / 8] = {};
+            float top = 0.f;
+            if (r < r1) {
+                const T* from = static_cast<const T*>(A.q) + (g.s.row0 + r / A.group) * A.qr + (g.head * A.group + r % A.group) * A.qh;
+#pragma unroll
+                for (int k = 0; k < D / 8; k++) {
+                    v[k] = *reinterpret_cast<const Vec<T, 8>*>(from + 8 * k);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < D / 8; k++) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    top = fmaxf(top, fabsf(to_f32(v[k].v[e])));
+                }
+            }
+            const int ex = min(max((__float_as_int(top) >> 23) - 134, -118), 118);
+            const float down = top <= 3.402823466e38f ? exp2_int(-ex) : __int_as_float(0x7fffffff);
+            up = exp2_int(ex);
+            unsigned char* q = smem + t * S::kTerms * S::kQ + (row >> 3) * 8 * D + (row & 7) * 16;
+#pragma unroll
+            for (int k = 0; k < D / 16; k++) {
+                uint32_t w[S::kTerms][4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const auto& c = v[2 * k + j / 2].v;
+                    float4 x = make_float4(to_f32(c[4 * (j % 2)]) * down, to_f32(c[4 * (j % 2) + 1]) * down, to_f32(c[4 * (j % 2) + 2]) * down, to_f32(c[4 * (j % 2) + 3]) * down);
+#pragma unroll
+                    for (int m = 0; m < S::kTerms; m++) {
+                        w[m][j] = pack_e4m3(x.x, x.y, x.z, x.w);
+                        const float4 y = codes_to_f32(w[m][j]);
+                        x = make_float4(x.x - y.x, x.y - y.y, x.z - y.z, x.w - y.w);
+                    }
+                }
+#pragma unroll
+                for (int m = 0; m < S::kTerms; m++) {
+                    *reinterpret_cast<uint4*>(q + m * S::kQ + k * 128) = make_uint4(w[m][0], w[m][1], w[m][2], w[m][3]);
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            bar_arrive(shared_u32(&ctl->q_full[t]));
+        }
+        int2 see = make_int2(0, 0);
+        if (r < r1) {
+            see = seen_by(A, g.s.place0 + r / A.group, g.s.len);
+        }
+        const TileKeys mine = keys_of_tile(A, g.s, rt, min(rt + kTileRows, r1));
+        float base = kNoBase, l = 0.f;
+#pragma unroll 1
+        for (int i = 0; i < n; i++) {
+            const uint32_t slot = (step + i) % kScaleSlots;
+            const TileScale* sc = ctl->scale[slot];
+            tile_wait(&ctl->scale_full[slot], (step + i) / kScaleSlots & 1, &ctl->abort);
+            tile_wait(&ctl->s_full[t], s_phase, &ctl->abort);
+            s_phase ^= 1;
+            tm_fence_after();
+            uint32_t x[128];
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                tm_ld32(ts + 32 * c, x + 32 * c);
+            }
+            const int key0 = (g.ga + i) * kTileKeys;
+            const bool whole = key0 >= mine.all_lo && key0 + kTileKeys <= mine.all_hi;
+            float top = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                tm_ld_wait(x + 32 * c);
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const float f = sc[2 * c + u].a * up, e = sc[2 * c + u].e;
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        uint32_t& y = x[32 * c + 16 * u + j];
+                        y = __float_as_uint(fmaf(__uint_as_float(y), f, e));
+                    }
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int j = 0; j < 32; j++) {
+                        const int key = key0 + 32 * c + j;
+                        x[32 * c + j] = key >= see.x && key < see.y ? x[32 * c + j] : 0xff800000u;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 32; j++) {
+                    top = fmaxf(top, __uint_as_float(x[32 * c + j]));
+                }
+            }
+            if (__any_sync(0xffffffffu, top > base + kSlack)) {
+                const float was = base;
+                base = top > base + kSlack ? top - kHeadroom : base;
+                const float corr = exp2_fast(was - base);
+                l *= corr;
+                if (i > 0) { // S of this step was issued after the last step's p V was done, and this step's waits for p
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t o[32];
+                        tm_ld32(to + c, o);
+                        tm_ld_wait(o);
+#pragma unroll
+                        for (int j = 0; j < 32; j++) {
+                            o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+                        }
+                        tm_st32(to + c, o);
+                    }
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                uint32_t p[32];
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    float sum = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const float p0 = exp2_fast(__uint_as_float(x[64 * c + 16 * u + 2 * j]) - base), p1 = exp2_fast(__uint_as_float(x[64 * c + 16 * u + 2 * j + 1]) - base);
+                        sum += p0 + p1;
+                        p[8 * u + j] = pack_f16(p0, p1);
+                    }
+                    l = fmaf(sum, sc[4 * c + u].iv, l);
+                }
+                tm_st32(ts + 32 * c, p);
+            }
+            tm_st_wait();
+            tm_fence_before();
+            bar_arrive(shared_u32(&ctl->p_full[t]));
+            if (i < n - 1) {
+                o_phase ^= 1; // the commit of this step's p V, which nobody here waits for
+            }
+        }
+        step += n;
+        tile_wait(&ctl->o_done[t], o_phase, &ctl->abort);
+        o_phase ^= 1;
+        tm_fence_after();
+        if (ctl->abort) {
+            l = __int_as_float(0x7fffffff);
+        }
+        const int64_t part = int64_t(g.part) * kUnitRows + t * kTileRows + row;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tm_ld32(to + c, o);
+            tm_ld_wait(o);
+            if (r < r1) {
+                if (g.alone) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8) {
+                        const float inv = l == 0.f ? 0.f : 1.f / l;
+                        Vec<T, 8> v;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            v.v[e] = from_f32<T>(__uint_as_float(o[j + e]) * inv);
+                        }
+                        *reinterpret_cast<Vec<T, 8>*>(static_cast<T*>(A.out) + (g.s.row0 + r / A.group) * A.or_ + (g.head * A.group + r % A.group) * A.oh + c + j) = v;
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        *reinterpret_cast<uint4*>(A.part_o + part * D + c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                    }
+                }
+            }
+        }
+        if (r < r1) {
+            if (!g.alone) {
+                *reinterpret_cast<float2*>(A.part_ml + 2 * part) = make_float2(base, l);
+            } else if (A.lse) {
+                A.lse[int64_t(g.s.row0 + r / A.group) * A.q_heads + g.head * A.group + r % A.group] = l == 0.f ? -INFINITY : 0.69314718055994531f * (base + log2f(l));
+            }
+        }
+        tm_fence_before();
+    }
+}
+
+template <class T, int D>
+__device__ __forceinline__ void tile_load(const AttentionArgs& A, unsigned char* smem, TileCtl* ctl) {
+    using S = TileShape<T, D>;
+    const int lane = threadIdx.x & 31;
+    const int shift = min(A.page_shift, 7); // a copy's tokens
+    Worker work(A);
+    Segment g;
+    uint32_t step = 0;
+    Ring<S::kKStages> kr;
+    Ring<S::kVStages> vr;
+#pragma unroll 1
+    while (work.next(A, g)) {
+        const int n = g.gb - g.ga;
+        // a lane looks 16 keys up, 8 lanes a tile, four tiles at a time
+        auto look_up = [&](int first) {
+            const int i = first + (lane >> 3), key = (g.ga + i) * kTileKeys + (lane & 7) * 16;
+            return piece_at(A, g.b, g.head, key, i < n && key < g.keys.hi && key + 16 > g.keys.lo);
+        };
+        Piece now = look_up(0), next = look_up(4);
+#pragma unroll 1
+        for (int i = 0; i < n; i++) {
+            if (i && (i & 3) == 0) {
+                now = next, next = look_up(i + 4);
+            }
+            const int from = (i & 3) * 8;
+            const uint32_t there = __ballot_sync(0xffffffffu, now.ks == now.ks) >> from & 0xFFu;
+            // a copy for each page: the first of its 16-key pieces that is there; where a window begins inside a page, from there on
+            const int mine = lane & 7, per = 1 << (shift - 4), group = mine & ~(per - 1);
+            const uint32_t in_page = there >> group & ((1u << per) - 1);
+            const bool leads = in_page && mine == group + __ffs(in_page) - 1 && lane >> 3 == (i & 3);
+            const uint32_t bytes = uint32_t(__popc(in_page)) * 16 * D;
+            tile_wait(&ctl->k_empty[kr.i], kr.phase ^ 1, &ctl->abort);
+            if (lane >> 3 == (i & 3)) {
+                TileScale sc;
+                sc.a = now.ks * A.scale_log2, sc.e = log2_fast(now.vs), sc.iv = inverse_fast(now.vs), sc.none = 0.f;
+                ctl->scale[(step + i) % kScaleSlots][mine] = sc;
+            }
+            if (lane == 0) {
+                ctl->absent[(step + i) % kScaleSlots] = ~there & 0xFFu;
+            }
+            __syncwarp();
+            const uint32_t kb = shared_u32(&ctl->k_full[kr.i]), vb = shared_u32(&ctl->v_full[vr.i]);
+            if (lane == 0) {
+                bar_arrive(shared_u32(&ctl->scale_full[(step + i) % kScaleSlots]));
+                bar_expect(kb, __popc(there) * 16 * D);
+            }
+            __syncwarp();
+            if (leads) {
+                bulk_load(shared_u32(smem + S::kOffK + kr.i * S::kCodes + mine * 16 * D), static_cast<const char*>(A.cache.k) + now.at, bytes, kb);
+            }
+            tile_wait(&ctl->v_empty[vr.i], vr.phase ^ 1, &ctl->abort);
+            if (lane == 0) {
+                bar_expect(vb, __popc(there) * 16 * D);
+            }
+            __syncwarp();
+            if (leads) {
+                bulk_load(shared_u32(smem + S::kOffV + vr.i * S::kCodes + mine * 16 * D), static_cast<const char*>(A.cache.v) + now.at, bytes, vb);
+            }
+            kr.next(), vr.next();
+        }
+        step += n;
+    }
+}
+
+template <class T, int D>
+__device__ __forceinline__ void tile_convert(const AttentionArgs& A, unsigned char* smem, TileCtl* ctl) {
+    using S = TileShape<T, D>;
+    const int tid = threadIdx.x & 127;
+    Worker work(A);
+    Segment g;
+    uint32_t step = 0;
+    Ring<S::kVStages> vr;
+    Ring<S::kHStages> hr;
+#pragma unroll 1
+    while (work.next(A, g)) {
+        const int n = g.gb - g.ga;
+#pragma unroll 1
+        for (int i = 0; i < n; i++) {
+            tile_wait(&ctl->v_full[vr.i], vr.phase, &ctl->abort);
+            tile_wait(&ctl->h_empty[hr.i], hr.phase ^ 1, &ctl->abort);
+            const uint32_t absent = ctl->absent[(step + i) % kScaleSlots];
+            const int key0 = (g.ga + i) * kTileKeys;
+            const bool edge = absent || key0 < g.keys.lo || key0 + kTileKeys > g.keys.hi;
+            const uint4* from = reinterpret_cast<const uint4*>(smem + S::kOffV + vr.i * S::kCodes);
+            uint4* to = reinterpret_cast<uint4*>(smem + S::kOffH + hr.i * 2 * S::kCodes);
+#pragma unroll 4
+            for (int c = tid; c < 8 * D; c += 128) { // 16 keys of a dim
+                uint4 w = from[c];
+                const int k16 = c / D, d = c % D;
+                if (edge) { // an unused slot may hold NaN, and 0 * NaN is NaN
+                    const bool gone = absent >> k16 & 1;
+                    auto keep = [&](uint32_t x, int key) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            if (gone || key + e < g.keys.lo || key + e >= g.keys.hi) {
+                                x &= ~(0xFFu << (8 * e));
+                            }
+                        }
+                        return x;
+                    };
+                    const int key = key0 + 16 * k16;
+                    w = make_uint4(keep(w.x, key), keep(w.y, key + 4), keep(w.z, key + 8), keep(w.w, key + 12));
+                }
+                uint4 lo, hi;
+                unpack_e4m3(w.x, lo.x, lo.y), unpack_e4m3(w.y, lo.z, lo.w), unpack_e4m3(w.z, hi.x, hi.y), unpack_e4m3(w.w, hi.z, hi.w);
+                to[2 * k16 * D + d] = lo, to[(2 * k16 + 1) * D + d] = hi;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if ((threadIdx.x & 31) == 0) {
+                bar_arrive(shared_u32(&ctl->v_empty[vr.i]));
+                bar_arrive(shared_u32(&ctl->h_full[hr.i]));
+            }
+            vr.next(), hr.next();
+        }
+        step += n;
+    }
+}
+
+template <class T, int D>
+__device__ __forceinline__ void tile_products(const AttentionArgs& A, unsigned char* smem, TileCtl* ctl) {
+    using S = TileShape<T, D>;
+    const uint32_t el = elected(), tm = ctl->tmem, sm = shared_u32(smem);
+    const uint32_t is = tile_idesc(kTileRows, kTileKeys), io = tile_idesc(kTileRows, D);
+    Worker work(A);
+    Segment g;
+    Ring<S::kKStages> kr;
+    Ring<S::kHStages> hr;
+    uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0}, o_phase[2] = {0, 0};
+#pragma unroll 1
+    while (work.next(A, g)) {
+        const int n = g.gb - g.ga, tiles = g.rows > kTileRows ? 2 : 1;
+#pragma unroll 1
+        for (int i = 0; i < n; i++) {
+            tile_wait(&ctl->k_full[kr.i], kr.phase, &ctl->abort);
+#pragma unroll 1
+            for (int t = 0; t < tiles; t++) {
+                if (i == 0) {
+                    tile_wait(&ctl->q_full[t], q_phase[t], &ctl->abort);
+                    q_phase[t] ^= 1;
+                } else { // p of the last step, where S goes, has been read
+                    tile_wait(&ctl->o_done[t], o_phase[t], &ctl->abort);
+                    o_phase[t] ^= 1;
+                }
+                tm_fence_after();
+                const uint32_t q = sm + t * S::kTerms * S::kQ, k = sm + S::kOffK + kr.i * S::kCodes;
+#pragma unroll
+                for (int m = 0; m < S::kTerms; m++) {
+#pragma unroll
+                    for (int c = 0; c < D / 32; c++) {
+                        mma_codes(el, tm + t * 128, tile_desc(q + m * S::kQ + c * 256, 128, 8 * D), tile_desc(k + c * 256, 128, 8 * D), is, m + c > 0);
+                    }
+                }
+                mma_commit(el, &ctl->s_full[t]);
+            }
+            mma_commit(el, &ctl->k_empty[kr.i]);
+            kr.next();
+            tile_wait(&ctl->h_full[hr.i], hr.phase, &ctl->abort);
+#pragma unroll 1
+            for (int t = 0; t < tiles; t++) {
+                tile_wait(&ctl->p_full[t], p_phase[t], &ctl->abort);
+                p_phase[t] ^= 1;
+                tm_fence_after();
+                const uint32_t v = sm + S::kOffH + hr.i * 2 * S::kCodes;
+#pragma unroll
+                for (int c = 0; c < kTileKeys / 16; c++) {
+                    mma_halves(el, tm + 256 + t * 128, tm + t * 128 + 8 * c, tile_desc(v + c * 32 * D, 16 * D, 128), io, i + c > 0);
+                }
+                mma_commit(el, &ctl->o_done[t]);
+            }
+            mma_commit(el, &ctl->h_empty[hr.i]);
+            hr.next();
+        }
+        // the segment's last o_done is the softmax warps' own; here its phase only passes
+#pragma unroll 1
+        for (int t = 0; t < tiles; t++) {
+            o_phase[t] ^= 1;
+        }
+    }
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const AttentionArgs A) {
+    using S = TileShape<T, D>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    TileCtl* ctl = reinterpret_cast<TileCtl*>(smem + S::kOffCtl);
+    const int warp = threadIdx.x >> 5;
+    if (A.part_o) {
+        let_next_start();
+    }
+    if (threadIdx.x == 0) {
+        auto init = [](uint64_t& b, int n) { bar_init(shared_u32(&b), n); };
+        for (int t = 0; t < 2; t++) {
+            init(ctl->q_full[t], kTileRows), init(ctl->s_full[t], 1), init(ctl->p_full[t], kTileRows), init(ctl->o_done[t], 1);
+            init(ctl->v_full[t], 1), init(ctl->v_empty[t], 4), init(ctl->h_full[t], 4), init(ctl->h_empty[t], 1);
+        }
+        for (int i = 0; i < 3; i++) {
+            init(ctl->k_full[i], 1), init(ctl->k_empty[i], 1);
+        }
+        for (int i = 0; i < kScaleSlots; i++) {
+            init(ctl->scale_full[i], 1);
+        }
+        bar_init_done();
+        ctl->abort = 0;
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_u32(&ctl->tmem)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tm_fence_before();
+    }
+    __syncthreads();
+    tm_fence_after();
+    // 512 threads of 128 registers: 256 of 200 and 256 of 56
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        tile_softmax<T, D>(A, smem, ctl);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 8) {
+            tile_load<T, D>(A, smem, ctl);
+        } else if (warp == 9) {
+            tile_products<T, D>(A, smem, ctl);
+        } else if (warp >= 12) {
+            tile_convert<T, D>(A, smem, ctl);
+        }
+    }
+    tm_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tm_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(ctl->tmem), "r"(512) : "memory");
+    }
+}
+
+} // namespace seq
+} // namespace cck

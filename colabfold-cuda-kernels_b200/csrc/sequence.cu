@@ -4,7 +4,7 @@
 #include <cstdio>
 
 #include "cache_append.cuh"
-#include "cache_attention.cuh"
+#include "cache_attention_tile.cuh"
 #include "report.h"
 
 using namespace cck;
@@ -211,68 +211,86 @@ cudaError_t launch_append(cudaStream_t st, const AppendArgs& a, int v, unsigned 
 
 // How an attention call is cut up: whole units, a block each, or equal shares of the line of all units
 struct Plan {
-    int nt;        // tiles of 8 rows a warp keeps
-    int row_tiles; // of 8 nt rows
+    int nt;                 // tiles of 8 rows of a warp of decode_kernel; 0: tile_kernel
+    int granule, tile_rows; // keys and rows of a step
+    int row_tiles;          // of a sequence
     int64_t blocks;
     bool shares;
+    int merge_y;
     size_t part_bytes, bytes; // of the workspace
 };
 Plan make_plan(const cck_cache& c, const cck_batch& b, int q_heads, int sms) {
     Plan p{};
     const int64_t rows = int64_t(b.max_new) * (q_heads / c.heads);
-    p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
-    p.row_tiles = int((rows + 8 * p.nt - 1) / (8 * p.nt));
-    const int64_t units = int64_t(b.sequences) * c.heads * p.row_tiles, slots = (p.nt == 1 ? 3 : 2) * sms;
-    const int64_t granules = int64_t(b.max_len) / granule_of(c.dim) + 2;
-    p.shares = granules > 4 * kDecodeWarps; // a share has two granules a warp at least
-    const int64_t most = (units * granules + 2 * kDecodeWarps - 1) / (2 * kDecodeWarps);
+    p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 0;
+    p.granule = p.nt ? granule_of(c.dim) : kTileKeys, p.tile_rows = p.nt ? 8 * p.nt : kUnitRows;
+    p.row_tiles = int((rows + p.tile_rows - 1) / p.tile_rows);
+    const int64_t units = int64_t(b.sequences) * c.heads * p.row_tiles, slots = (p.nt == 0 ? 1 : p.nt == 1 ? 3 : 2) * sms;
+    const int64_t granules = int64_t(b.max_len) / p.granule + 2;
+    const int least = p.nt ? 2 * kDecodeWarps : 2; // granules of a share
+    p.shares = granules > 2 * least && units < 8 * slots;
+    const int64_t most = (units * granules + least - 1) / least;
     p.blocks = !p.shares ? units : most < slots ? most : slots;
     if (p.shares) {
-        p.part_bytes = size_t(2 * p.blocks) * 8 * p.nt * c.dim * 4;
-        p.bytes = p.part_bytes + size_t(2 * p.blocks) * 8 * p.nt * 8;
+        p.merge_y = p.nt == 0 ? 16 : units < 64 ? p.tile_rows : 1;
+        p.part_bytes = size_t(2 * p.blocks) * p.tile_rows * c.dim * 4;
+        p.bytes = p.part_bytes + size_t(2 * p.blocks) * p.tile_rows * 8;
     }
     return p;
 }
-template <class T, int D, int NT>
-cudaError_t launch_decode(cudaStream_t st, const AttentionArgs& a, unsigned blocks) {
-    static std::atomic<bool> ready[kMaxDevices];
+// the attribute that a kernel of more than 48 KB needs, once a device
+template <class K>
+cudaError_t allow_shared(K kernel, int bytes, std::atomic<bool>* ready) {
     int dev = 0;
-    cudaGetDevice(&dev);
+    if (cudaError_t e = cudaGetDevice(&dev)) {
+        return e;
+    }
     if (!ready[dev].load(std::memory_order_relaxed)) {
-        if (cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(decode_kernel<T, D, NT>), cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeShape<D, NT>::kSmem)) {
+        if (cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) {
             return e;
         }
         ready[dev].store(true, std::memory_order_relaxed);
     }
+    return cudaSuccess;
+}
+template <class T, int D, int NT>
+cudaError_t launch_decode(cudaStream_t st, const AttentionArgs& a, unsigned blocks) {
+    static std::atomic<bool> ready[kMaxDevices];
+    if (cudaError_t e = allow_shared(decode_kernel<T, D, NT>, DecodeShape<D, NT>::kSmem, ready)) {
+        return e;
+    }
     decode_kernel<T, D, NT><<<blocks, kDecodeWarps * 32, DecodeShape<D, NT>::kSmem, st>>>(a);
     return cudaGetLastError();
 }
-template <class T, int NT>
-cudaError_t launch_decode(cudaStream_t st, const AttentionArgs& a, unsigned blocks) {
-    switch (a.cache.dim) {
-    case 32: return launch_decode<T, 32, NT>(st, a, blocks);
-    case 64: return launch_decode<T, 64, NT>(st, a, blocks);
-    case 96: return launch_decode<T, 96, NT>(st, a, blocks);
-    default: return launch_decode<T, 128, NT>(st, a, blocks);
+template <class T, int D>
+cudaError_t launch_tile(cudaStream_t st, const AttentionArgs& a, unsigned blocks) {
+    static std::atomic<bool> ready[kMaxDevices];
+    if (cudaError_t e = allow_shared(tile_kernel<T, D>, TileShape<T, D>::kSmem, ready)) {
+        return e;
     }
+    tile_kernel<T, D><<<blocks, kTileThreads, TileShape<T, D>::kSmem, st>>>(a);
+    return cudaGetLastError();
+}
+template <class T, int D>
+cudaError_t launch_attention(cudaStream_t st, const AttentionArgs& a, const Plan& p) {
+    const unsigned blocks = unsigned(p.blocks);
+    return p.nt == 0 ? launch_tile<T, D>(st, a, blocks) : p.nt == 1 ? launch_decode<T, D, 1>(st, a, blocks) : launch_decode<T, D, 2>(st, a, blocks);
 }
 template <class T>
 cudaError_t launch_attention(cudaStream_t st, const AttentionArgs& a, const Plan& p) {
-    const unsigned blocks = unsigned(p.blocks);
-    if (cudaError_t e = p.nt == 1 ? launch_decode<T, 1>(st, a, blocks) : p.nt == 2 ? launch_decode<T, 2>(st, a, blocks) : launch_decode<T, 4>(st, a, blocks)) {
+    const cudaError_t e = a.cache.dim == 32   ? launch_attention<T, 32>(st, a, p)
+                          : a.cache.dim == 64 ? launch_attention<T, 64>(st, a, p)
+                          : a.cache.dim == 96 ? launch_attention<T, 96>(st, a, p)
+                                              : launch_attention<T, 128>(st, a, p);
+    if (e || !p.shares) {
         return e;
-    }
-    if (!p.shares) {
-        return cudaSuccess;
     }
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute dependent;
     dependent.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     dependent.val.programmaticStreamSerializationAllowed = 1;
-    const int64_t rows = int64_t(a.batch.max_new) * a.group;
-    cfg.gridDim = dim3(unsigned(int64_t(a.batch.sequences) * a.row_tiles * a.cache.heads), unsigned(rows < a.tile_rows ? rows : a.tile_rows));
-    cfg.blockDim = dim3(kMergeWarps * 32), cfg.stream = st, cfg.attrs = &dependent, cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, merge_kernel<T>, a, int(blocks));
+    cfg.gridDim = dim3(unsigned(p.blocks), unsigned(p.merge_y)), cfg.blockDim = dim3(kMergeWarps * 32), cfg.stream = st, cfg.attrs = &dependent, cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, merge_kernel<T>, a);
 }
 
 } // namespace
@@ -413,7 +431,7 @@ int cck_cache_attention(void* stream, const cck_cache* cache, const cck_batch* b
     if (ws_bytes < p.bytes || (p.bytes && (!ws || !aligned(ws, 16)))) {
         return refuse(CCK_E_WORKSPACE, op, "the workspace is too small, null or not aligned");
     }
-    if (int64_t(batch->sequences) * cache->heads * p.row_tiles > 0x7fffffff) {
+    if (p.blocks > 0x7fffffff) {
         return refuse(CCK_E_SHAPE, op, "too many rows for one launch");
     }
     AttentionArgs a{};
@@ -421,8 +439,8 @@ int cck_cache_attention(void* stream, const cck_cache* cache, const cck_batch* b
     a.qr = q->row_stride, a.qh = q->head_stride, a.or_ = out->row_stride, a.oh = out->head_stride;
     a.scale_log2 = softmax_scale * 1.4426950408889634f;
     a.q_heads = q->heads, a.group = q->heads / cache->heads, a.causal = causal != 0, a.window = window;
-    a.granule = granule_of(cache->dim), a.page_shift = __builtin_ctz(cache->page_tokens);
-    a.tile_rows = 8 * p.nt, a.row_tiles = p.row_tiles;
+    a.granule = p.granule, a.page_shift = __builtin_ctz(cache->page_tokens);
+    a.tile_rows = p.tile_rows, a.row_tiles = p.row_tiles;
     if (p.shares) {
         a.part_o = static_cast<float*>(ws), a.part_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + p.part_bytes);
     }
