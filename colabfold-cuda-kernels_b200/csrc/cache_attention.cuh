@@ -252,7 +252,7 @@ __device__ __noinline__ void clear_values(uint32_t v, int lo, int hi, uint32_t a
 }
 
 template <class T, int D, int NT>
-__global__ void __launch_bounds__(kDecodeWarps * 32, DecodeShape<D, NT>::kBlocks) decode_kernel(const AttentionArgs A) {
+__global__ void __launch_bounds__(kDecodeWarps * 32, DecodeShape<D, NT>::kBlocks) decode_kernel(const __grid_constant__ AttentionArgs A) {
     using S = DecodeShape<D, NT>;
     constexpr int kTerms = sizeof(T) == 2 && T_is_f16<T>() ? 3 : 2;
     constexpr int kRows = 8 * NT, kTiles = S::kKeys / 16, kKeysShift = S::kKeys == 64 ? 6 : 5; // kTiles: of 16 keys
@@ -609,7 +609,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DecodeShape<D, NT>::kBlocks
 // out to the blocks y and to the warps, or, where there are many shares, the shares of a row to the warps.
 constexpr int kMergeWarps = 8;
 template <class T>
-__global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const AttentionArgs A) {
+__global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_constant__ AttentionArgs A) {
     __shared__ float4 so[kMergeWarps][32];
     __shared__ float2 sm[kMergeWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = A.cache.dim, H = A.cache.heads;

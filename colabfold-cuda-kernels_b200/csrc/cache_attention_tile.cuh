@@ -5,20 +5,24 @@
 // beside the other's exponentials:
 //   warps 0-3, 4-7   softmax of tile 0, 1: a thread owns a row, S comes from and p goes to tensor memory
 //   warp 8           loads: pages as they lie into the rings (one bulk copy a page: the cache's layout is the operand's), their scales
-//   warp 9           issues the products
+//   warps 9, 10      issue the products of tile 0, 1
 //   warps 12-15      V to f16
 // S = q K^T is kind::f8f6f4 on the codes, q in terms of 4 bits, two of a bf16 and three of an f16 (as in cache_attention.cuh, but into
 // one accumulator: a term's last bit is 2^-17 of the row's largest): no work for K at all, in the time that f16 would take.
-// O += p V is kind::f16 for the sake of p's range, p read from tensor memory, where it takes S's place. Tensor memory: S 2 x 128
-// columns, O 2 x dim.
+// O += p V is kind::f16 for the sake of p's range, p read from tensor memory. Tensor memory (512 columns): O 2 x 128, S 2 x 2 x 64. S is
+// computed for 64 keys at a time into two buffers, p takes its place: a batch of eight tcgen05.mma needs some 530 cycles more than its
+// products from the issue to the waiting thread, so that a tile whose S, softmax and p V follow one another takes 4800 cycles for 128 keys
+// whatever the rates are. With a buffer ahead, the softmax is the chain.
 #pragma once
+
+#include <cstddef>
 
 #include "cache_attention.cuh"
 
 namespace cck {
 namespace seq {
 
-constexpr int kTileKeys = 128, kTileRows = 128, kUnitRows = 2 * kTileRows, kTileThreads = 512;
+constexpr int kTileKeys = 128, kHalfKeys = 64, kTileRows = 128, kUnitRows = 2 * kTileRows, kTileThreads = 512;
 
 template <class T, int D>
 struct TileShape {
@@ -29,17 +33,15 @@ struct TileShape {
     static constexpr int kOffK = 2 * kTerms * kQ, kOffV = kOffK + kKStages * kCodes, kOffH = kOffV + kVStages * kCodes;
     static constexpr int kOffCtl = kOffH + kHStages * 2 * kCodes;
     static constexpr int kSmem = kOffCtl + 2048;
-    static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 // A tile's scales are read until its softmax is done. The loads of tile j wait for V of j - 3 to be converted, that for p V of j - 5: they are at
-// most 5 tiles ahead, and a slot's next phase cannot end before its last one has been waited for.
+// most 5 tiles ahead. The scales are written before K's barrier is armed, which the products wait for, and these arrive at S's barrier.
 constexpr int kScaleSlots = 8;
 struct TileScale {
     float a, e, iv, none;
 };
 struct TileCtl {
-    uint64_t q_full[2], k_full[3], k_empty[3], v_full[2], v_empty[2], h_full[2], h_empty[2], s_full[2], p_full[2], o_done[2];
-    uint64_t scale_full[kScaleSlots];
+    uint64_t q_full[2], k_full[3], k_empty[3], v_full[2], v_empty[2], h_full[2], h_empty[2], s_full[2][2], p_full[2][2], o_done[2][2]; // [tile][buffer of S]
     TileScale scale[kScaleSlots][kTileKeys / 16];
     uint32_t absent[kScaleSlots]; // a bit for each 16 keys whose page is not there, or that nobody sees
     uint32_t tmem;
@@ -48,8 +50,7 @@ struct TileCtl {
 static_assert(sizeof(TileCtl) <= 2048, "control block");
 
 // A wait that gives up after about a second, which nothing but a lost copy can cause; then every later one returns at once
-__device__ __forceinline__ void tile_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
-    const uint32_t b = shared_u32(bar);
+__device__ __forceinline__ void tile_wait(uint32_t b, uint32_t parity, volatile int* abort) {
 #pragma unroll 1
     for (int i = 0; i < 1 << 18; i++) {
         uint32_t ok;
@@ -66,6 +67,9 @@ __device__ __forceinline__ void tile_wait(uint64_t* bar, uint32_t parity, volati
         }
     }
     *abort = 1;
+}
+__device__ __forceinline__ void tile_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+    tile_wait(shared_u32(bar), parity, abort);
 }
 // position in a ring
 template <int N>
@@ -112,6 +116,17 @@ __device__ __forceinline__ void tm_st32(uint32_t at, const uint32_t* r) {
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(at)
         : "memory");
 }
+__device__ __forceinline__ void tm_st16(uint32_t at, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
+        "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ void tm_st_wait() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -123,9 +138,12 @@ __device__ __forceinline__ void tm_fence_after() {
 }
 // Shared-memory descriptor of a K-major operand in core matrices of 8 rows x 16 bytes without a swizzle: `lead` bytes to the next 16
 // bytes along k, `stride` to the next 8 rows. Start address >> 4 in bits [0,14), lead >> 4 in [16,30), stride >> 4 in [32,46), version 1
-// in [46,48), no swizzle: 0 in [61,64).
-__device__ __forceinline__ uint64_t tile_desc(uint32_t at, uint32_t lead, uint32_t stride) {
-    return uint64_t((at & 0x3FFFFu) >> 4) | uint64_t(lead >> 4) << 16 | uint64_t(stride >> 4) << 32 | uint64_t(1) << 46;
+// in [46,48), no swizzle: 0 in [61,64). The high word is a constant; n bytes on are n >> 4 in the low one.
+__device__ __forceinline__ uint32_t desc_low(uint32_t at, uint32_t lead) {
+    return (at & 0x3FFFFu) >> 4 | (lead >> 4) << 16;
+}
+constexpr uint32_t desc_high(uint32_t stride) {
+    return stride >> 4 | 1u << 14;
 }
 // f32 accumulator (bits [4,6) = 1), M >> 4 in [24,29), N >> 3 in [17,23), both operands K-major; the types' fields are 0: e4m3 of
 // kind::f8f6f4, f16 of kind::f16
@@ -137,24 +155,29 @@ __device__ __forceinline__ uint32_t elected() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
     return e;
 }
-__device__ __forceinline__ void mma_codes(uint32_t el, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// The operands of tcgen05.mma live in uniform registers: everything here is a value that the compiler knows to be the same in all
+// lanes (uniform()), and the whole warp issues, predicated on one lane
+__device__ __forceinline__ uint32_t uniform(uint32_t v) {
+    return __shfl_sync(0xffffffffu, v, 0);
+}
+__device__ __forceinline__ void mma_codes(uint32_t el, uint32_t d, uint32_t a, uint32_t a_high, uint32_t b, uint32_t b_high, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(el)
+        "{\n\t.reg .pred p, e;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %6, 0;\n\tsetp.ne.b32 e, %7, 0;\n\tmov.b64 x, {%1, %2};\n\tmov.b64 y, {%3, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], x, y, %5, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(a_high), "r"(b), "r"(b_high), "r"(idesc), "r"(acc), "r"(el)
         : "memory");
 }
-__device__ __forceinline__ void mma_halves(uint32_t el, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_halves(uint32_t el, uint32_t d, uint32_t a, uint32_t b, uint32_t b_high, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(el)
+        "{\n\t.reg .pred p, e;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 e, %6, 0;\n\tmov.b64 y, {%2, %3};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(b_high), "r"(idesc), "r"(acc), "r"(el)
         : "memory");
 }
-__device__ __forceinline__ void mma_commit(uint32_t el, uint64_t* bar) {
+__device__ __forceinline__ void mma_commit(uint32_t el, uint32_t bar) {
     asm volatile(
         "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
-        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(shared_u32(bar)),
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
         "r"(el)
         : "memory");
 }
@@ -171,7 +194,7 @@ struct Segment {
 struct Worker {
     int64_t left = 1, done = 0;
     int tile, head;
-    __device__ __forceinline__ Worker(const AttentionArgs& A) {
+    __device__ __noinline__ Worker(const AttentionArgs& A) { // out of line, as next(): four roles run them, a few times each
         const int H = A.cache.heads;
         // units of long sequences' last rows first: they see the most keys
         tile = A.batch.sequences * A.row_tiles - 1 - blockIdx.x / H, head = blockIdx.x % H;
@@ -190,7 +213,7 @@ struct Worker {
             }
         }
     }
-    __device__ __forceinline__ bool next(const AttentionArgs& A, Segment& g) {
+    __device__ __noinline__ bool next(const AttentionArgs& A, Segment& g) {
         const int H = A.cache.heads;
         Tile own;
         while (left > 0) {
@@ -228,10 +251,11 @@ __device__ __forceinline__ void tile_softmax(const AttentionArgs& A, unsigned ch
     using S = TileShape<T, D>;
     const int t = threadIdx.x >> 7, row = threadIdx.x & 127;
     const uint32_t lanes = uint32_t(row & ~31) << 16, ts = ctl->tmem + lanes + t * 128, to = ctl->tmem + lanes + 256 + t * 128;
+    // the scale's sign goes to the queries, so that the largest score of 16 keys is that of the largest product
+    const float sign = A.scale_log2 < 0.f ? -1.f : 1.f;
     Worker work(A);
     Segment g;
-    uint32_t step = 0; // tiles of keys so far
-    uint32_t s_phase = 0, o_phase = 0;
+    uint32_t step = 0, own = 0; // tiles of keys so far: of the block, of this tile of rows
 #pragma unroll 1
     while (work.next(A, g)) {
         const int n = g.gb - g.ga;
@@ -260,8 +284,8 @@ __device__ __forceinline__ void tile_softmax(const AttentionArgs& A, unsigned ch
                 }
             }
             const int ex = min(max((__float_as_int(top) >> 23) - 134, -118), 118);
-            const float down = top <= 3.402823466e38f ? exp2_int(-ex) : __int_as_float(0x7fffffff);
-            up = exp2_int(ex);
+            const float down = top <= 3.402823466e38f ? sign * exp2_int(-ex) : __int_as_float(0x7fffffff);
+            up = sign * exp2_int(ex);
             unsigned char* q = smem + t * S::kTerms * S::kQ + (row >> 3) * 8 * D + (row & 7) * 16;
 #pragma unroll
             for (int k = 0; k < D / 16; k++) {
@@ -292,90 +316,82 @@ __device__ __forceinline__ void tile_softmax(const AttentionArgs& A, unsigned ch
         const TileKeys mine = keys_of_tile(A, g.s, rt, min(rt + kTileRows, r1));
         float base = kNoBase, l = 0.f;
 #pragma unroll 1
-        for (int i = 0; i < n; i++) {
-            const uint32_t slot = (step + i) % kScaleSlots;
-            const TileScale* sc = ctl->scale[slot];
-            tile_wait(&ctl->scale_full[slot], (step + i) / kScaleSlots & 1, &ctl->abort);
-            tile_wait(&ctl->s_full[t], s_phase, &ctl->abort);
-            s_phase ^= 1;
+        for (int j = 0; j < 2 * n; j++) { // 64 keys at a time
+            const int i = j >> 1, h = j & 1;
+            const uint32_t slot = (step + i) % kScaleSlots, td = ts + h * kHalfKeys;
+            const TileScale* sc = ctl->scale[slot] + 4 * h;
+            tile_wait(&ctl->s_full[t][h], (own + i) & 1, &ctl->abort);
             tm_fence_after();
-            uint32_t x[128];
+            uint32_t x[64];
+            tm_ld32(td, x), tm_ld32(td + 32, x + 32);
+            const int key0 = (g.ga + i) * kTileKeys + h * kHalfKeys;
+            const bool whole = key0 >= mine.all_lo && key0 + kHalfKeys <= mine.all_hi;
+            tm_ld_wait(x), tm_ld_wait(x + 32);
+            float f[4], e[4], top = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                tm_ld32(ts + 32 * c, x + 32 * c);
+            for (int u = 0; u < 4; u++) {
+                f[u] = sc[u].a * up, e[u] = sc[u].e;
             }
-            const int key0 = (g.ga + i) * kTileKeys;
-            const bool whole = key0 >= mine.all_lo && key0 + kTileKeys <= mine.all_hi;
-            float top = -INFINITY;
+            if (!whole) { // scaled first: a page that is not there has a NaN scale, which a masked score must not take
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                tm_ld_wait(x + 32 * c);
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const float f = sc[2 * c + u].a * up, e = sc[2 * c + u].e;
-#pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        uint32_t& y = x[32 * c + 16 * u + j];
-                        y = __float_as_uint(fmaf(__uint_as_float(y), f, e));
-                    }
-                }
-                if (!whole) {
-#pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        const int key = key0 + 32 * c + j;
-                        x[32 * c + j] = key >= see.x && key < see.y ? x[32 * c + j] : 0xff800000u;
-                    }
+                for (int c = 0; c < 64; c++) {
+                    const float y = fmaf(__uint_as_float(x[c]), f[c / 16], e[c / 16]);
+                    x[c] = __float_as_uint(key0 + c >= see.x && key0 + c < see.y ? y : -INFINITY);
                 }
 #pragma unroll
-                for (int j = 0; j < 32; j++) {
-                    top = fmaxf(top, __uint_as_float(x[32 * c + j]));
+                for (int u = 0; u < 4; u++) {
+                    f[u] = 1.f, e[u] = 0.f;
                 }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const float* y = reinterpret_cast<const float*>(x + 16 * u);
+                const float m0 = max3(max3(y[0], y[1], y[2]), max3(y[3], y[4], y[5]), max3(y[6], y[7], y[8]));
+                const float m1 = max3(max3(y[9], y[10], y[11]), max3(y[12], y[13], y[14]), y[15]);
+                top = fmaxf(top, fmaf(fmaxf(m0, m1), f[u], e[u]));
             }
             if (__any_sync(0xffffffffu, top > base + kSlack)) {
                 const float was = base;
                 base = top > base + kSlack ? top - kHeadroom : base;
                 const float corr = exp2_fast(was - base);
                 l *= corr;
-                if (i > 0) { // S of this step was issued after the last step's p V was done, and this step's waits for p
+                if (j > 0) { // O is whole when the last p V is done; the next one waits for this p
+                    tile_wait(&ctl->o_done[t][h ^ 1], (own + ((j - 1) >> 1)) & 1, &ctl->abort);
+                    tm_fence_after();
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
                         uint32_t o[32];
                         tm_ld32(to + c, o);
                         tm_ld_wait(o);
 #pragma unroll
-                        for (int j = 0; j < 32; j++) {
-                            o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+                        for (int k = 0; k < 32; k++) {
+                            o[k] = __float_as_uint(__uint_as_float(o[k]) * corr);
                         }
                         tm_st32(to + c, o);
                     }
                 }
             }
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
-                uint32_t p[32];
+            for (int u = 0; u < 4; u++) {
+                const float eb = e[u] - base;
+                float sum[2] = {0.f, 0.f};
 #pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    float sum = 0.f;
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const float p0 = exp2_fast(__uint_as_float(x[64 * c + 16 * u + 2 * j]) - base), p1 = exp2_fast(__uint_as_float(x[64 * c + 16 * u + 2 * j + 1]) - base);
-                        sum += p0 + p1;
-                        p[8 * u + j] = pack_f16(p0, p1);
-                    }
-                    l = fmaf(sum, sc[4 * c + u].iv, l);
+                for (int k = 0; k < 8; k++) {
+                    const float p0 = exp2_fast(fmaf(__uint_as_float(x[16 * u + 2 * k]), f[u], eb)), p1 = exp2_fast(fmaf(__uint_as_float(x[16 * u + 2 * k + 1]), f[u], eb));
+                    sum[0] += p0, sum[1] += p1;
+                    x[8 * u + k] = pack_f16(p0, p1);
                 }
-                tm_st32(ts + 32 * c, p);
+                l = fmaf(sum[0] + sum[1], sc[u].iv, l);
             }
+            tm_st32(td, x);
             tm_st_wait();
             tm_fence_before();
-            bar_arrive(shared_u32(&ctl->p_full[t]));
-            if (i < n - 1) {
-                o_phase ^= 1; // the commit of this step's p V, which nobody here waits for
-            }
+            bar_arrive(shared_u32(&ctl->p_full[t][h]));
         }
         step += n;
-        tile_wait(&ctl->o_done[t], o_phase, &ctl->abort);
-        o_phase ^= 1;
+        tile_wait(&ctl->o_done[t][0], (own + n - 1) & 1, &ctl->abort);
+        tile_wait(&ctl->o_done[t][1], (own + n - 1) & 1, &ctl->abort);
+        own += n;
         tm_fence_after();
         if (ctl->abort) {
             l = __int_as_float(0x7fffffff);
@@ -460,7 +476,6 @@ __device__ __forceinline__ void tile_load(const AttentionArgs& A, unsigned char*
             __syncwarp();
             const uint32_t kb = shared_u32(&ctl->k_full[kr.i]), vb = shared_u32(&ctl->v_full[vr.i]);
             if (lane == 0) {
-                bar_arrive(shared_u32(&ctl->scale_full[(step + i) % kScaleSlots]));
                 bar_expect(kb, __popc(there) * 16 * D);
             }
             __syncwarp();
@@ -536,70 +551,95 @@ __device__ __forceinline__ void tile_convert(const AttentionArgs& A, unsigned ch
     }
 }
 
+// The products of tile t: p V of 64 keys, then the S that takes p's place. A warp for each tile: what it runs between two batches is fetched
+// anew each time, some 5 cycles an instruction, and one warp for both, whatever the order, held the tiles up to 5000 cycles a step.
 template <class T, int D>
-__device__ __forceinline__ void tile_products(const AttentionArgs& A, unsigned char* smem, TileCtl* ctl) {
+__device__ __forceinline__ void tile_products(const AttentionArgs& A, unsigned char* smem, TileCtl* ctl, uint32_t t) {
     using S = TileShape<T, D>;
-    const uint32_t el = elected(), tm = ctl->tmem, sm = shared_u32(smem);
-    const uint32_t is = tile_idesc(kTileRows, kTileKeys), io = tile_idesc(kTileRows, D);
-    Worker work(A);
-    Segment g;
+    const uint32_t el = elected(), sm = uniform(shared_u32(smem)), bars = uniform(shared_u32(ctl));
+    const uint32_t is = tile_idesc(kTileRows, kHalfKeys), io = tile_idesc(kTileRows, D);
+    const uint32_t ts = uniform(ctl->tmem + t * 128), to = ts - t * 128 + 256 + t * 128, q = uniform(desc_low(sm + t * S::kTerms * S::kQ, 128));
+    const uint32_t q_full = bars + offsetof(TileCtl, q_full) + 8 * t, s_full = bars + offsetof(TileCtl, s_full) + 16 * t;
+    const uint32_t p_full = bars + offsetof(TileCtl, p_full) + 16 * t, o_done = bars + offsetof(TileCtl, o_done) + 16 * t;
+    volatile int* abort = &ctl->abort;
     Ring<S::kKStages> kr;
     Ring<S::kHStages> hr;
-    uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0}, o_phase[2] = {0, 0};
+    uint32_t turn = 0, units = 0; // parities: of the tile's steps, of its units
+    Worker work(A);
+    Segment g;
 #pragma unroll 1
     while (work.next(A, g)) {
-        const int n = g.gb - g.ga, tiles = g.rows > kTileRows ? 2 : 1;
+        const int n = uniform(g.gb - g.ga);
+        if (uniform(g.rows) <= kTileRows * t) { // no second tile: its share of the stages is given back
+#pragma unroll 1
+            for (int i = 0; i < n; i++) {
+                tile_wait(bars + offsetof(TileCtl, k_full) + 8 * kr.i, kr.phase, abort);
+                tile_wait(bars + offsetof(TileCtl, h_full) + 8 * hr.i, hr.phase, abort);
+                if (el) {
+                    bar_arrive(bars + offsetof(TileCtl, k_empty) + 8 * kr.i), bar_arrive(bars + offsetof(TileCtl, h_empty) + 8 * hr.i);
+                }
+                kr.next(), hr.next();
+            }
+            continue;
+        }
+        auto scores = [&](uint32_t k, int h) {
+            tm_fence_after();
+#pragma unroll
+            for (int m = 0; m < S::kTerms; m++) {
+#pragma unroll
+                for (int c = 0; c < D / 32; c++) {
+                    mma_codes(el, ts + h * kHalfKeys, q + m * (S::kQ >> 4) + c * 16, desc_high(8 * D), k + h * (kHalfKeys * D >> 4) + c * 16, desc_high(8 * D), is, m + c > 0);
+                }
+            }
+            mma_commit(el, s_full + 8 * h);
+            if (el) { // the scales, which came with K, are the softmax's to read
+                bar_arrive(s_full + 8 * h);
+            }
+        };
+        const uint32_t k0 = desc_low(sm + S::kOffK, 128), v0 = desc_low(sm + S::kOffH, 16 * D);
+        tile_wait(q_full, units, abort);
+        tile_wait(bars + offsetof(TileCtl, k_full) + 8 * kr.i, kr.phase, abort);
+        uint32_t k = uniform(k0 + kr.i * (S::kCodes >> 4));
+        scores(k, 0), scores(k, 1);
+        mma_commit(el, bars + offsetof(TileCtl, k_empty) + 8 * kr.i);
+        kr.next();
 #pragma unroll 1
         for (int i = 0; i < n; i++) {
-            tile_wait(&ctl->k_full[kr.i], kr.phase, &ctl->abort);
-#pragma unroll 1
-            for (int t = 0; t < tiles; t++) {
-                if (i == 0) {
-                    tile_wait(&ctl->q_full[t], q_phase[t], &ctl->abort);
-                    q_phase[t] ^= 1;
-                } else { // p of the last step, where S goes, has been read
-                    tile_wait(&ctl->o_done[t], o_phase[t], &ctl->abort);
-                    o_phase[t] ^= 1;
-                }
+            const uint32_t v = uniform(v0 + hr.i * (2 * S::kCodes >> 4));
+            k = uniform(k0 + kr.i * (S::kCodes >> 4));
+            tile_wait(bars + offsetof(TileCtl, h_full) + 8 * hr.i, hr.phase, abort);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                tile_wait(p_full + 8 * h, turn, abort);
                 tm_fence_after();
-                const uint32_t q = sm + t * S::kTerms * S::kQ, k = sm + S::kOffK + kr.i * S::kCodes;
 #pragma unroll
-                for (int m = 0; m < S::kTerms; m++) {
-#pragma unroll
-                    for (int c = 0; c < D / 32; c++) {
-                        mma_codes(el, tm + t * 128, tile_desc(q + m * S::kQ + c * 256, 128, 8 * D), tile_desc(k + c * 256, 128, 8 * D), is, m + c > 0);
+                for (int c = 0; c < kHalfKeys / 16; c++) {
+                    mma_halves(el, to, ts + h * kHalfKeys + 8 * c, v + (h * kHalfKeys / 16 + c) * 2 * D, desc_high(128), io, h + c > 0 ? 1 : i);
+                }
+                mma_commit(el, o_done + 8 * h);
+                if (h == 1) {
+                    mma_commit(el, bars + offsetof(TileCtl, h_empty) + 8 * hr.i);
+                }
+                if (i + 1 < n) {
+                    if (h == 0) {
+                        tile_wait(bars + offsetof(TileCtl, k_full) + 8 * kr.i, kr.phase, abort);
                     }
+                    tile_wait(o_done + 8 * h, turn, abort);
+                    scores(k, h);
                 }
-                mma_commit(el, &ctl->s_full[t]);
             }
-            mma_commit(el, &ctl->k_empty[kr.i]);
-            kr.next();
-            tile_wait(&ctl->h_full[hr.i], hr.phase, &ctl->abort);
-#pragma unroll 1
-            for (int t = 0; t < tiles; t++) {
-                tile_wait(&ctl->p_full[t], p_phase[t], &ctl->abort);
-                p_phase[t] ^= 1;
-                tm_fence_after();
-                const uint32_t v = sm + S::kOffH + hr.i * 2 * S::kCodes;
-#pragma unroll
-                for (int c = 0; c < kTileKeys / 16; c++) {
-                    mma_halves(el, tm + 256 + t * 128, tm + t * 128 + 8 * c, tile_desc(v + c * 32 * D, 16 * D, 128), io, i + c > 0);
-                }
-                mma_commit(el, &ctl->o_done[t]);
+            if (i + 1 < n) {
+                mma_commit(el, bars + offsetof(TileCtl, k_empty) + 8 * kr.i);
+                kr.next();
             }
-            mma_commit(el, &ctl->h_empty[hr.i]);
-            hr.next();
+            hr.next(), turn ^= 1;
         }
-        // the segment's last o_done is the softmax warps' own; here its phase only passes
-#pragma unroll 1
-        for (int t = 0; t < tiles; t++) {
-            o_phase[t] ^= 1;
-        }
+        units ^= 1;
     }
 }
 
 template <class T, int D>
-__global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const AttentionArgs A) {
+__global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_constant__ AttentionArgs A) {
     using S = TileShape<T, D>;
     extern __shared__ __align__(128) unsigned char smem[];
     TileCtl* ctl = reinterpret_cast<TileCtl*>(smem + S::kOffCtl);
@@ -610,14 +650,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const AttentionAr
     if (threadIdx.x == 0) {
         auto init = [](uint64_t& b, int n) { bar_init(shared_u32(&b), n); };
         for (int t = 0; t < 2; t++) {
-            init(ctl->q_full[t], kTileRows), init(ctl->s_full[t], 1), init(ctl->p_full[t], kTileRows), init(ctl->o_done[t], 1);
-            init(ctl->v_full[t], 1), init(ctl->v_empty[t], 4), init(ctl->h_full[t], 4), init(ctl->h_empty[t], 1);
+            init(ctl->q_full[t], kTileRows);
+            for (int h = 0; h < 2; h++) {
+                init(ctl->s_full[t][h], 2), init(ctl->p_full[t][h], kTileRows), init(ctl->o_done[t][h], 1);
+            }
+            init(ctl->v_full[t], 1), init(ctl->v_empty[t], 4), init(ctl->h_full[t], 4), init(ctl->h_empty[t], 2);
         }
         for (int i = 0; i < 3; i++) {
-            init(ctl->k_full[i], 1), init(ctl->k_empty[i], 1);
-        }
-        for (int i = 0; i < kScaleSlots; i++) {
-            init(ctl->scale_full[i], 1);
+            init(ctl->k_full[i], 1), init(ctl->k_empty[i], 2);
         }
         bar_init_done();
         ctl->abort = 0;
@@ -629,19 +669,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const AttentionAr
     }
     __syncthreads();
     tm_fence_after();
-    // 512 threads of 128 registers: 256 of 200 and 256 of 56
     if (warp < 8) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         tile_softmax<T, D>(A, smem, ctl);
-    } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == 8) {
-            tile_load<T, D>(A, smem, ctl);
-        } else if (warp == 9) {
-            tile_products<T, D>(A, smem, ctl);
-        } else if (warp >= 12) {
-            tile_convert<T, D>(A, smem, ctl);
-        }
+    } else if (warp == 8) {
+        tile_load<T, D>(A, smem, ctl);
+    } else if (warp == 9 || warp == 10) {
+        tile_products<T, D>(A, smem, ctl, warp - 9);
+    } else if (warp >= 12) {
+        tile_convert<T, D>(A, smem, ctl);
     }
     tm_fence_before();
     __syncthreads();
