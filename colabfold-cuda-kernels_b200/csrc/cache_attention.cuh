@@ -44,9 +44,12 @@ struct AttentionArgs {
     float* lse;
     float scale_log2; // softmax_scale * log2(e)
     int q_heads, group, causal, window;
-    int granule, page_shift; // granule_of(dim); page_tokens = 1 << page_shift
+    int granule_shift, page_shift; // keys of a step and tokens of a page are powers of two
+    int unit_cost;
     int tile_rows, row_tiles; // a sequence's rows times heads of a group, cut into tiles: `tiles` are those of all sequences, row_tiles each
-    float *part_o, *part_ml; // shares of units that several blocks work on: [2 blocks][tile rows][dim], [..][2]; null: a block takes a unit
+    // shares of units that several blocks work on: sums [2 blocks][tile rows][dim], reference and sum [..][2]; null: a block takes a unit
+    float *part_o, *part_ml;
+    struct Split* splits;
 };
 
 // keys [lo, hi) that row i (a place in its sequence) sees
@@ -125,11 +128,10 @@ struct TileKeys {
     int g0, g1; // granules of [lo, hi)
 };
 __device__ __forceinline__ TileKeys keys_of_tile(const AttentionArgs& A, const Sequence& s, int r0, int r1) {
-    const int granule = A.granule;
     const int2 first = seen_by(A, s.place0 + r0 / A.group, s.len), last = seen_by(A, s.place0 + (r1 - 1) / A.group, s.len);
     TileKeys t;
     t.lo = first.x, t.hi = last.y, t.all_lo = last.x, t.all_hi = first.y;
-    t.g0 = t.lo / granule, t.g1 = max(t.g0, ceil_div(t.hi, granule));
+    t.g0 = t.lo >> A.granule_shift, t.g1 = max(t.g0, (t.hi + (1 << A.granule_shift) - 1) >> A.granule_shift);
     return t;
 }
 
@@ -144,64 +146,71 @@ struct Tile {
 };
 __device__ __forceinline__ Tile tile_at(const AttentionArgs& A, int i) {
     Tile t;
-    t.s = sequence_of(A.batch, i / A.row_tiles);
-    t.r0 = i % A.row_tiles * A.tile_rows, t.rows = max(0, min(A.tile_rows, t.s.rows * A.group - t.r0));
+    const int b = A.row_tiles == 1 ? i : i / A.row_tiles;
+    t.s = sequence_of(A.batch, b);
+    t.r0 = (i - b * A.row_tiles) * A.tile_rows, t.rows = max(0, min(A.tile_rows, t.s.rows * A.group - t.r0));
     return t;
 }
-__device__ __forceinline__ int granules_of(const AttentionArgs& A, int i) {
+// a unit's stretch of the line: its cost beside the granules (queries, the way out, an empty pipeline) in granules, then these
+__device__ __forceinline__ int weight_of(const AttentionArgs& A, int i) {
     const Tile t = tile_at(A, i);
     if (t.rows == 0) {
         return 0;
     }
     const TileKeys k = keys_of_tile(A, t.s, t.r0, t.r0 + t.rows);
-    return max(1, k.g1 - k.g0); // a tile that sees nothing still has rows to write
+    return A.unit_cost + max(1, k.g1 - k.g0); // a tile that sees nothing still has rows to write
 }
-// The tile on the line of one head's granules that `pick` chooses (of start, granules, index), where it starts, and the line's length.
-// Every warp finds out by itself, 32 tiles at a time. `pick` is only asked once the length is known.
+// Where a share begins: the tile, its start on the line of one head's granules, and the granules of a share (all have as many, the last
+// ones fewer or none). A warp finds out together, 32 tiles at a time.
 struct Line {
-    int64_t total, start;
+    int64_t size, left, start; // granules of all heads: of a share, left in this one, before the tile
     int tile;
 };
-template <class Pick>
-__device__ __forceinline__ Line line_of(const AttentionArgs& A, Pick pick) {
-    const int n = A.batch.sequences * A.row_tiles, lane = threadIdx.x & 31;
-    Line l{0, 0, 0};
-    int g = lane < n ? granules_of(A, lane) : 0;
-    int64_t sum = g;
+__device__ __forceinline__ Line line_of(const AttentionArgs& A, int share, int shares) {
+    const int n = A.batch.sequences * A.row_tiles, lane = threadIdx.x & 31, H = A.cache.heads;
+    const int first = lane < n ? weight_of(A, lane) : 0;
+    int64_t sum = first;
 #pragma unroll 1
     for (int i = 32 + lane; i < n; i += 32) {
-        sum += granules_of(A, i);
+        sum += weight_of(A, i);
     }
 #pragma unroll
     for (int o = 16; o; o /= 2) {
         sum += __shfl_xor_sync(0xffffffffu, sum, o);
     }
-    l.total = sum;
+    Line l;
+    l.size = (sum * H + shares - 1) / shares, l.start = 0, l.tile = 0;
+    const int64_t from = l.size * share;
+    l.left = min(l.size, sum * H - from);
+    if (l.left <= 0) {
+        return l;
+    }
     int64_t at = 0;
 #pragma unroll 1
     for (int i0 = 0; i0 < n; i0 += 32) {
-        const int i = i0 + lane;
-        g = i0 == 0 ? g : i < n ? granules_of(A, i) : 0;
-        int64_t upto = g;
+        const int i = i0 + lane, g = i0 == 0 ? first : i < n ? weight_of(A, i) : 0;
+        int upto = g;
 #pragma unroll
         for (int o = 1; o < 32; o *= 2) {
-            const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+            const int x = __shfl_up_sync(0xffffffffu, upto, o);
             upto += lane >= o ? x : 0;
         }
-        const unsigned hit = __ballot_sync(0xffffffffu, i < n && g > 0 && pick(at + upto - g, g, i, l.total));
+        const int64_t start = (at + upto - g) * H;
+        const unsigned hit = __ballot_sync(0xffffffffu, g > 0 && start <= from && from < start + int64_t(g) * H);
         if (hit) {
-            const int from = __ffs(hit) - 1;
-            l.tile = i0 + from, l.start = __shfl_sync(0xffffffffu, at + upto - g, from);
+            const int who = __ffs(hit) - 1;
+            l.tile = i0 + who, l.start = __shfl_sync(0xffffffffu, start, who);
             break;
         }
         at += __shfl_sync(0xffffffffu, upto, 31);
     }
     return l;
 }
-// granules of a share: all have as many, the last ones fewer or none
-__device__ __forceinline__ int64_t share_size(int64_t total, int shares) {
-    return (total + shares - 1) / shares;
-}
+// A unit that begins in a share and goes on in the next: what merge_kernel needs of it, a word of four for each share. last: the last
+// share that has a part of it; the share itself if there is no such unit.
+struct Split {
+    int tile, head, last, none;
+};
 
 // The keys of a granule that one page holds, and the page's scales
 struct Piece {
@@ -269,23 +278,17 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DecodeShape<D, NT>::kBlocks
     }
     __syncwarp();
     // what is left of this block's share, and where it is: tile, head, granules done of the unit
-    int64_t left = 1, done = 0;
+    int64_t left = 1, done = 0, size = 0, at = 0; // at: on the line
     int tile = blockIdx.x / H, head = blockIdx.x % H;
+    Split split{0, 0, int(blockIdx.x), 0};
     if (A.part_o) {
         let_next_start();
-        int64_t from = 0;
-        const Line line = line_of(A, [&](int64_t start, int g, int, int64_t total) {
-            from = share_size(total * H, gridDim.x) * blockIdx.x;
-            return start * H <= from && from < (start + g) * H;
-        });
-        const int64_t size = share_size(line.total * H, gridDim.x);
-        from = size * blockIdx.x, left = min(size, line.total * H - from);
-        if (left <= 0) {
-            return;
+        const Line line = line_of(A, blockIdx.x, gridDim.x);
+        left = line.left, size = line.size, at = size * blockIdx.x, tile = line.tile;
+        if (left > 0) {
+            const int w = weight_of(A, tile);
+            head = int((at - line.start) / w), done = at - line.start - int64_t(head) * w;
         }
-        tile = line.tile;
-        const int g = granules_of(A, tile);
-        head = int((from - line.start * H) / g), done = from - line.start * H - int64_t(head) * g;
     }
     int slot = 0, phase = 0;
 #pragma unroll 1
@@ -301,9 +304,18 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DecodeShape<D, NT>::kBlocks
     const Sequence s = own.s;
     const int b = tile / A.row_tiles, r0 = own.r0, r1 = r0 + own.rows;
     const TileKeys keys = keys_of_tile(A, s, r0, r1);
-    const int all = max(1, keys.g1 - keys.g0), ga = keys.g0 + int(done);
-    const int gb = A.part_o ? int(min(int64_t(keys.g0 + all), ga + left)) : keys.g0 + all;
-    const bool alone = ga == keys.g0 && gb == keys.g0 + all; // a unit of this block only
+    const int all = max(1, keys.g1 - keys.g0);
+    // what of the unit's stretch of the line is the share's, without the cost at its head
+    const int64_t to = A.part_o ? min(int64_t(all + A.unit_cost), done + left) : all + A.unit_cost, unit_at = at - done;
+    const int ga = keys.g0 + max(0, int(done) - A.unit_cost), gb = keys.g0 + max(0, int(to) - A.unit_cost);
+    left -= to - done, at = unit_at + to, done = 0;
+    if (gb == ga) { // the cost alone: the next share begins with the unit
+        break;
+    }
+    const bool alone = gb - ga == all; // a unit of this block only
+    if (ga == keys.g0 && !alone) {
+        split.tile = tile, split.head = head, split.last = int((unit_at + all + A.unit_cost - 1) / size);
+    }
     const int part = 2 * blockIdx.x + (ga == keys.g0 ? 1 : 0);
 
     // this warp's granules: ga + warp, + kDecodeWarps, ...; a granule is one piece of a page, or several of small pages. A lane looks
@@ -598,10 +610,12 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DecodeShape<D, NT>::kBlocks
         return;
     }
     __syncthreads(); // the ring is free again
-    left -= gb - ga, done = 0;
     if (++head == H) {
         head = 0, tile++;
     }
+    }
+    if (A.part_o && threadIdx.x == 0) {
+        A.splits[blockIdx.x] = split;
     }
 }
 
@@ -612,36 +626,22 @@ template <class T>
 __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_constant__ AttentionArgs A) {
     __shared__ float4 so[kMergeWarps][32];
     __shared__ float2 sm[kMergeWarps];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = A.cache.dim, H = A.cache.heads;
-    // from the call's inputs alone, while the shares are still being worked on
-    int64_t size = 0, last = 0; // granules of a share; this one's last
-    const Line line = line_of(A, [&](int64_t start, int g, int, int64_t total) {
-        size = share_size(total * H, gridDim.x), last = size * (blockIdx.x + 1) - 1;
-        return start * H <= last && last < (start + g) * H;
-    });
-    size = share_size(line.total * H, gridDim.x), last = size * (blockIdx.x + 1) - 1;
-    int rows = 0, head = 0;
-    int64_t c1 = 0;
-    Tile own{};
-    if (last < line.total * H) {
-        const int g = granules_of(A, line.tile);
-        head = int((last - line.start * H) / g);
-        const int64_t start = line.start * H + int64_t(head) * g, end = start + g;
-        if (start > last - size && end > last + 1) {
-            own = tile_at(A, line.tile), rows = own.rows, c1 = (end - 1) / size;
-        }
-    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = A.cache.dim, c0 = blockIdx.x;
     wait_for_previous();
-    const int64_t c0 = blockIdx.x;
-    const bool together = c1 - c0 >= 2 * kMergeWarps; // a row by all warps
+    const Split split = A.splits[c0];
+    if (split.last == c0) {
+        return;
+    }
+    const Tile own = tile_at(A, split.tile);
+    const bool together = split.last - c0 >= 2 * kMergeWarps; // a row by all warps
     const int stride = together ? gridDim.y : gridDim.y * kMergeWarps;
 #pragma unroll 1
-    for (int r = together ? blockIdx.y : blockIdx.y * kMergeWarps + warp; r < rows; r += stride) {
+    for (int r = together ? blockIdx.y : blockIdx.y * kMergeWarps + warp; r < own.rows; r += stride) {
         float top = kNoBase, sum = 0.f;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-        for (int64_t c = together ? c0 + warp : c0; c <= c1; c += together ? kMergeWarps : 1) {
-            const int64_t at = (2 * c + (c == c0 ? 1 : 0)) * A.tile_rows + r;
+        for (int c = together ? c0 + warp : c0; c <= split.last; c += together ? kMergeWarps : 1) {
+            const int64_t at = (2 * int64_t(c) + (c == c0 ? 1 : 0)) * A.tile_rows + r;
             const float2 ml = *reinterpret_cast<const float2*>(A.part_ml + 2 * at);
             const float4 z = 4 * lane < D ? *reinterpret_cast<const float4*>(A.part_o + at * D + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
             const float is = fmaxf(top, ml.x), f = exp2_fast(top - is), w = exp2_fast(ml.x - is);
@@ -667,7 +667,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_co
             __syncthreads();
         }
         if (4 * lane < D && (!together || warp == 0)) {
-            store_out<T>(A, own.s.row0 + (own.r0 + r) / A.group, head * A.group + (own.r0 + r) % A.group, 4 * lane, y, top, sum);
+            store_out<T>(A, own.s.row0 + (own.r0 + r) / A.group, split.head * A.group + (own.r0 + r) % A.group, 4 * lane, y, top, sum);
         }
     }
 }

@@ -4,9 +4,9 @@
 // tcgen05.mma and 2048 of the special function units. A block of threads keeps two tiles of 128 rows, so that one's products run
 // beside the other's exponentials:
 //   warps 0-3, 4-7   softmax of tile 0, 1: a thread owns a row, S comes from and p goes to tensor memory
-//   warp 8           loads: pages as they lie into the rings (one bulk copy a page: the cache's layout is the operand's), their scales
-//   warps 9, 10      issue the products of tile 0, 1
-//   warps 12-15      V to f16
+//   warp 8           what to work on; loads: pages as they lie into the rings (one bulk copy a page: the cache's layout is the operand's)
+//   warps 9 - 12     issue S of tile 0 and 1, p V of tile 0 and 1
+//   warps 13-15      V to f16
 // S = q K^T is kind::f8f6f4 on the codes, q in terms of 4 bits, two of a bf16 and three of an f16 (as in cache_attention.cuh, but into
 // one accumulator: a term's last bit is 2^-17 of the row's largest): no work for K at all, in the time that f16 would take.
 // O += p V is kind::f16 for the sake of p's range, p read from tensor memory. Tensor memory (512 columns): O 2 x 128, S 2 x 2 x 64. S is
@@ -23,16 +23,19 @@ namespace cck {
 namespace seq {
 
 constexpr int kTileKeys = 128, kHalfKeys = 64, kTileRows = 128, kUnitRows = 2 * kTileRows, kTileThreads = 512;
+constexpr int kConvertWarps = 3;
 
+constexpr int kCtlBytes = 2048;
 template <class T, int D>
 struct TileShape {
     static constexpr int kTerms = T_is_f16<T>() ? 3 : 2;
     static constexpr int kQ = kTileRows * D;          // bytes of a term of a tile
     static constexpr int kCodes = kTileKeys * D;      // bytes of the codes of K or V
-    static constexpr int kKStages = kTerms == 3 ? 2 : 3, kVStages = 2, kHStages = 2; // K; V; V in f16
+    static constexpr int kKStages = kTerms == 3 ? 2 : 3, kVStages = kTerms == 3 && D == 128 ? 1 : 2, kHStages = 2; // K; V; V in f16
     static constexpr int kOffK = 2 * kTerms * kQ, kOffV = kOffK + kKStages * kCodes, kOffH = kOffV + kVStages * kCodes;
     static constexpr int kOffCtl = kOffH + kHStages * 2 * kCodes;
-    static constexpr int kSmem = kOffCtl + 2048;
+    static constexpr int kSmem = kOffCtl + kCtlBytes;
+    static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 // A tile's scales are read until its softmax is done. The loads of tile j wait for V of j - 3 to be converted, that for p V of j - 5: they are at
 // most 5 tiles ahead. The scales are written before K's barrier is armed, which the products wait for, and these arrive at S's barrier.
@@ -40,14 +43,25 @@ constexpr int kScaleSlots = 8;
 struct TileScale {
     float a, e, iv, none;
 };
+// What a block works on, unit after unit: found out by the loading warp, read by all others
+struct Segment {
+    int head, r0, rows, row0, place0, len; // rows r0 .. of the sequence that begins at row0
+    int lo, hi;                             // keys that the unit's rows see
+    int ga, gb;                             // tiles of keys; none: the end
+    int part;                               // slot of the workspace; -1: the unit is the block's alone
+};
+constexpr int kSegments = 3, kReaders = 8 + 4 + kConvertWarps; // warps that read a segment
 struct TileCtl {
-    uint64_t q_full[2], k_full[3], k_empty[3], v_full[2], v_empty[2], h_full[2], h_empty[2], s_full[2][2], p_full[2][2], o_done[2][2]; // [tile][buffer of S]
+    uint64_t q_full[2], k_full[3], k_empty[3], v_full[2], v_empty[2], h_full[2], h_empty[2];
+    uint64_t s_full[2][2], p_full[2][2], o_done[2][2]; // [tile][buffer of S]
+    uint64_t seg_full[kSegments], seg_empty[kSegments];
+    Segment seg[kSegments];
     TileScale scale[kScaleSlots][kTileKeys / 16];
     uint32_t absent[kScaleSlots]; // a bit for each 16 keys whose page is not there, or that nobody sees
     uint32_t tmem;
     int abort;
 };
-static_assert(sizeof(TileCtl) <= 2048, "control block");
+static_assert(sizeof(TileCtl) <= kCtlBytes, "control block");
 
 // A wait that gives up after about a second, which nothing but a lost copy can cause; then every later one returns at once
 __device__ __forceinline__ void tile_wait(uint32_t b, uint32_t parity, volatile int* abort) {
@@ -93,6 +107,15 @@ __device__ __forceinline__ void tm_ld32(uint32_t at, uint32_t* r) {
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
           "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
           "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void tm_ld16(uint32_t at, uint32_t* r) { // with the wait
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(at)
         : "memory");
 }
@@ -182,128 +205,93 @@ __device__ __forceinline__ void mma_commit(uint32_t el, uint32_t bar) {
         : "memory");
 }
 
-// What a block works on, unit after unit; every role goes through the same ones
-struct Segment {
-    int b, head, r0, rows; // sequence; rows of the unit
-    Sequence s;
-    TileKeys keys;
-    int ga, gb;     // tiles of keys
-    bool alone;     // the whole unit
-    int part;       // slot of the workspace, where it is not
-};
-struct Worker {
-    int64_t left = 1, done = 0;
-    int tile, head;
-    __device__ __noinline__ Worker(const AttentionArgs& A) { // out of line, as next(): four roles run them, a few times each
-        const int H = A.cache.heads;
-        // units of long sequences' last rows first: they see the most keys
-        tile = A.batch.sequences * A.row_tiles - 1 - blockIdx.x / H, head = blockIdx.x % H;
-        if (A.part_o) {
-            int64_t from = 0;
-            const Line line = line_of(A, [&](int64_t start, int g, int, int64_t total) {
-                from = share_size(total * H, gridDim.x) * blockIdx.x;
-                return start * H <= from && from < (start + g) * H;
-            });
-            const int64_t size = share_size(line.total * H, gridDim.x);
-            from = size * blockIdx.x, left = min(size, line.total * H - from);
-            if (left > 0) {
-                tile = line.tile;
-                const int g = granules_of(A, tile);
-                head = int((from - line.start * H) / g), done = from - line.start * H - int64_t(head) * g;
-            }
-        }
+// pairs of f16 to codes and back
+__device__ __forceinline__ uint32_t halves_to_codes(__half2 a, __half2 b) {
+    uint32_t w;
+    asm("{\n\t.reg .b16 x, y;\n\tcvt.rn.satfinite.e4m3x2.f16x2 x, %1;\n\tcvt.rn.satfinite.e4m3x2.f16x2 y, %2;\n\tmov.b32 %0, {x, y};\n\t}"
+        : "=r"(w)
+        : "r"(*reinterpret_cast<const uint32_t*>(&a)), "r"(*reinterpret_cast<const uint32_t*>(&b)));
+    return w;
+}
+// the next segment; false at the end. A whole warp calls
+__device__ __forceinline__ bool next_segment(TileCtl* ctl, Ring<kSegments>& r, Segment& g) {
+    tile_wait(&ctl->seg_full[r.i], r.phase, &ctl->abort);
+    g = ctl->seg[r.i];
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) {
+        bar_arrive(shared_u32(&ctl->seg_empty[r.i]));
     }
-    __device__ __noinline__ bool next(const AttentionArgs& A, Segment& g) {
-        const int H = A.cache.heads;
-        Tile own;
-        while (left > 0) {
-            own = tile_at(A, tile);
-            if (own.rows > 0) {
-                break;
-            }
-            if (!A.part_o) {
-                left = 0;
-            }
-            tile++, head = 0;
-        }
-        if (left <= 0) {
-            return false;
-        }
-        g.s = own.s, g.b = tile / A.row_tiles, g.head = head, g.r0 = own.r0, g.rows = own.rows;
-        g.keys = keys_of_tile(A, own.s, own.r0, own.r0 + own.rows);
-        const int all = max(1, g.keys.g1 - g.keys.g0);
-        g.ga = g.keys.g0 + int(done), g.gb = A.part_o ? int(min(int64_t(g.keys.g0 + all), g.ga + left)) : g.keys.g0 + all;
-        g.alone = g.ga == g.keys.g0 && g.gb == g.keys.g0 + all, g.part = 2 * blockIdx.x + (g.ga == g.keys.g0 ? 1 : 0);
-        if (A.part_o) {
-            left -= g.gb - g.ga, done = 0;
-            if (++head == H) {
-                head = 0, tile++;
-            }
-        } else {
-            left = 0;
-        }
-        return true;
-    }
-};
+    r.next();
+    return g.gb > g.ga && !*static_cast<volatile int*>(&ctl->abort);
+}
 
 template <class T, int D>
 __device__ __forceinline__ void tile_softmax(const AttentionArgs& A, unsigned char* smem, TileCtl* ctl) {
     using S = TileShape<T, D>;
-    const int t = threadIdx.x >> 7, row = threadIdx.x & 127;
+    const int t = threadIdx.x >> 7, row = threadIdx.x & 127, lane = threadIdx.x & 31;
     const uint32_t lanes = uint32_t(row & ~31) << 16, ts = ctl->tmem + lanes + t * 128, to = ctl->tmem + lanes + 256 + t * 128;
     // the scale's sign goes to the queries, so that the largest score of 16 keys is that of the largest product
     const float sign = A.scale_log2 < 0.f ? -1.f : 1.f;
-    Worker work(A);
+    Ring<kSegments> segments;
     Segment g;
     uint32_t step = 0, own = 0; // tiles of keys so far: of the block, of this tile of rows
 #pragma unroll 1
-    while (work.next(A, g)) {
+    while (next_segment(ctl, segments, g)) {
         const int n = g.gb - g.ga;
         if (t * kTileRows >= g.rows) { // the unit has no second tile
             step += n;
             continue;
         }
-        const int r = g.r0 + t * kTileRows + row, r1 = g.r0 + g.rows, rt = g.r0 + t * kTileRows;
-        // queries in terms; a row that is not there is zero
+        const int rt = g.r0 + t * kTileRows, r = rt + row, r1 = g.r0 + g.rows;
+        // Queries in terms, two rows at a time: 16 lanes hold eight dims of a row each; a row that is not there is zero. Scaled to 256 at its
+        // row's largest, a bf16 is an f16 too (down to 2^-32 of that), in which the terms are split off, two at a time.
         float up = 0.f;
         {
-            Vec<T, 8> v[D / 8] = {};
-            float top = 0.f;
-            if (r < r1) {
-                const T* from = static_cast<const T*>(A.q) + (g.s.row0 + r / A.group) * A.qr + (g.head * A.group + r % A.group) * A.qh;
+            const int c = lane & 15, at0 = (row & ~31) + (lane >> 4);
+            unsigned char* to_q = smem + t * S::kTerms * S::kQ + (c >> 1) * 128 + (c & 1) * 8;
+#pragma unroll 1
+            for (int k0 = 0; k0 < 16; k0 += 8) {
+                Vec<T, 8> v[8] = {};
 #pragma unroll
-                for (int k = 0; k < D / 8; k++) {
-                    v[k] = *reinterpret_cast<const Vec<T, 8>*>(from + 8 * k);
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < D / 8; k++) {
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    top = fmaxf(top, fabsf(to_f32(v[k].v[e])));
-                }
-            }
-            const int ex = min(max((__float_as_int(top) >> 23) - 134, -118), 118);
-            const float down = top <= 3.402823466e38f ? sign * exp2_int(-ex) : __int_as_float(0x7fffffff);
-            up = sign * exp2_int(ex);
-            unsigned char* q = smem + t * S::kTerms * S::kQ + (row >> 3) * 8 * D + (row & 7) * 16;
-#pragma unroll
-            for (int k = 0; k < D / 16; k++) {
-                uint32_t w[S::kTerms][4];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const auto& c = v[2 * k + j / 2].v;
-                    float4 x = make_float4(to_f32(c[4 * (j % 2)]) * down, to_f32(c[4 * (j % 2) + 1]) * down, to_f32(c[4 * (j % 2) + 2]) * down, to_f32(c[4 * (j % 2) + 3]) * down);
-#pragma unroll
-                    for (int m = 0; m < S::kTerms; m++) {
-                        w[m][j] = pack_e4m3(x.x, x.y, x.z, x.w);
-                        const float4 y = codes_to_f32(w[m][j]);
-                        x = make_float4(x.x - y.x, x.y - y.y, x.z - y.z, x.w - y.w);
+                for (int k = 0; k < 8; k++) { // all loads on their way before the first store
+                    if (const int rr = rt + at0 + 2 * (k0 + k); rr < r1 && 8 * c < D) {
+                        v[k] = *reinterpret_cast<const Vec<T, 8>*>(static_cast<const T*>(A.q) + (g.row0 + rr / A.group) * A.qr + (g.head * A.group + rr % A.group) * A.qh + 8 * c);
                     }
                 }
 #pragma unroll
-                for (int m = 0; m < S::kTerms; m++) {
-                    *reinterpret_cast<uint4*>(q + m * S::kQ + k * 128) = make_uint4(w[m][0], w[m][1], w[m][2], w[m][3]);
+                for (int k = 0; k < 8; k++) {
+                    const int at = at0 + 2 * (k0 + k);
+                    float x[8], top = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        x[e] = to_f32(v[k].v[e]), top = fmaxf(top, fabsf(x[e]));
+                    }
+#pragma unroll
+                    for (int w = 1; w < 16; w *= 2) {
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+                    }
+                    const int ex = min(max((__float_as_int(top) >> 23) - 134, -118), 118);
+                    const float down = top <= 3.402823466e38f ? sign * exp2_int(-ex) : __int_as_float(0x7fffffff);
+                    const float its = __shfl_sync(0xffffffffu, sign * exp2_int(ex), (lane & 1) * 16);
+                    up = lane >> 1 == k0 + k ? its : up;
+                    __half2 z[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        z[e] = __floats2half2_rn(x[2 * e] * down, x[2 * e + 1] * down);
+                    }
+#pragma unroll
+                    for (int m = 0; m < S::kTerms; m++) {
+                        const uint32_t w0 = halves_to_codes(z[0], z[1]), w1 = halves_to_codes(z[2], z[3]);
+                        if (8 * c < D) {
+                            *reinterpret_cast<uint2*>(to_q + m * S::kQ + (at >> 3) * 8 * D + (at & 7) * 16) = make_uint2(w0, w1);
+                        }
+                        uint32_t y[4];
+                        unpack_e4m3(w0, y[0], y[1]), unpack_e4m3(w1, y[2], y[3]);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            z[e] = __hsub2(z[e], *reinterpret_cast<const __half2*>(&y[e]));
+                        }
+                    }
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -311,28 +299,27 @@ __device__ __forceinline__ void tile_softmax(const AttentionArgs& A, unsigned ch
         }
         int2 see = make_int2(0, 0);
         if (r < r1) {
-            see = seen_by(A, g.s.place0 + r / A.group, g.s.len);
+            see = seen_by(A, g.place0 + r / A.group, g.len);
         }
-        const TileKeys mine = keys_of_tile(A, g.s, rt, min(rt + kTileRows, r1));
+        // keys that all rows of the tile see
+        const int all_lo = seen_by(A, g.place0 + (min(rt + kTileRows, r1) - 1) / A.group, g.len).x, all_hi = seen_by(A, g.place0 + rt / A.group, g.len).y;
         float base = kNoBase, l = 0.f;
 #pragma unroll 1
         for (int j = 0; j < 2 * n; j++) { // 64 keys at a time
-            const int i = j >> 1, h = j & 1;
-            const uint32_t slot = (step + i) % kScaleSlots, td = ts + h * kHalfKeys;
-            const TileScale* sc = ctl->scale[slot] + 4 * h;
+            const int i = j >> 1, h = j & 1, key0 = (g.ga + i) * kTileKeys + h * kHalfKeys;
+            const uint32_t td = ts + h * kHalfKeys;
+            const TileScale* sc = ctl->scale[(step + i) % kScaleSlots] + 4 * h;
             tile_wait(&ctl->s_full[t][h], (own + i) & 1, &ctl->abort);
             tm_fence_after();
             uint32_t x[64];
             tm_ld32(td, x), tm_ld32(td + 32, x + 32);
-            const int key0 = (g.ga + i) * kTileKeys + h * kHalfKeys;
-            const bool whole = key0 >= mine.all_lo && key0 + kHalfKeys <= mine.all_hi;
-            tm_ld_wait(x), tm_ld_wait(x + 32);
             float f[4], e[4], top = -INFINITY;
 #pragma unroll
             for (int u = 0; u < 4; u++) {
                 f[u] = sc[u].a * up, e[u] = sc[u].e;
             }
-            if (!whole) { // scaled first: a page that is not there has a NaN scale, which a masked score must not take
+            tm_ld_wait(x), tm_ld_wait(x + 32);
+            if (key0 < all_lo || key0 + kHalfKeys > all_hi) { // masked scores are -inf; scaled first: a page that is not there has a NaN scale, which they must not take
 #pragma unroll
                 for (int c = 0; c < 64; c++) {
                     const float y = fmaf(__uint_as_float(x[c]), f[c / 16], e[c / 16]);
@@ -359,29 +346,29 @@ __device__ __forceinline__ void tile_softmax(const AttentionArgs& A, unsigned ch
                     tile_wait(&ctl->o_done[t][h ^ 1], (own + ((j - 1) >> 1)) & 1, &ctl->abort);
                     tm_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
-                        uint32_t o[32];
-                        tm_ld32(to + c, o);
-                        tm_ld_wait(o);
+                    for (int c = 0; c < D; c += 16) {
+                        uint32_t o[16];
+                        tm_ld16(to + c, o);
 #pragma unroll
-                        for (int k = 0; k < 32; k++) {
+                        for (int k = 0; k < 16; k++) {
                             o[k] = __float_as_uint(__uint_as_float(o[k]) * corr);
                         }
-                        tm_st32(to + c, o);
+                        tm_st16(to + c, o);
                     }
                 }
             }
 #pragma unroll
             for (int u = 0; u < 4; u++) {
                 const float eb = e[u] - base;
-                float sum[2] = {0.f, 0.f};
+                float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const float p0 = exp2_fast(fmaf(__uint_as_float(x[16 * u + 2 * k]), f[u], eb)), p1 = exp2_fast(fmaf(__uint_as_float(x[16 * u + 2 * k + 1]), f[u], eb));
-                    sum[0] += p0, sum[1] += p1;
-                    x[8 * u + k] = pack_f16(p0, p1);
+                for (int k = 0; k < 8; k++) { // packed: half the instructions
+                    const float2 y = __ffma2_rn(make_float2(__uint_as_float(x[16 * u + 2 * k]), __uint_as_float(x[16 * u + 2 * k + 1])), make_float2(f[u], f[u]), make_float2(eb, eb));
+                    const float2 p = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+                    sum = __fadd2_rn(sum, p);
+                    x[8 * u + k] = pack_f16(p.x, p.y);
                 }
-                l = fmaf(sum[0] + sum[1], sc[u].iv, l);
+                l = fmaf(sum.x + sum.y, sc[u].iv, l);
             }
             tm_st32(td, x);
             tm_st_wait();
@@ -397,36 +384,38 @@ __device__ __forceinline__ void tile_softmax(const AttentionArgs& A, unsigned ch
             l = __int_as_float(0x7fffffff);
         }
         const int64_t part = int64_t(g.part) * kUnitRows + t * kTileRows + row;
+        const int64_t out_row = g.row0 + r / A.group;
+        const int out_head = g.head * A.group + r % A.group;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
             uint32_t o[32];
             tm_ld32(to + c, o);
             tm_ld_wait(o);
-            if (r < r1) {
-                if (g.alone) {
+            if (r >= r1) {
+            } else if (g.part < 0) {
+                T* y = static_cast<T*>(A.out) + out_row * A.or_ + out_head * A.oh + c;
 #pragma unroll
-                    for (int j = 0; j < 32; j += 8) {
-                        const float inv = l == 0.f ? 0.f : 1.f / l;
-                        Vec<T, 8> v;
+                for (int j = 0; j < 32; j += 8) {
+                    Vec<T, 8> v;
 #pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            v.v[e] = from_f32<T>(__uint_as_float(o[j + e]) * inv);
-                        }
-                        *reinterpret_cast<Vec<T, 8>*>(static_cast<T*>(A.out) + (g.s.row0 + r / A.group) * A.or_ + (g.head * A.group + r % A.group) * A.oh + c + j) = v;
+                    for (int e = 0; e < 8; e++) {
+                        v.v[e] = from_f32<T>(__uint_as_float(o[j + e]) * inv);
                     }
-                } else {
+                    *reinterpret_cast<Vec<T, 8>*>(y + j) = v;
+                }
+            } else {
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        *reinterpret_cast<uint4*>(A.part_o + part * D + c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-                    }
+                for (int j = 0; j < 32; j += 4) {
+                    *reinterpret_cast<uint4*>(A.part_o + part * D + c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
                 }
             }
         }
         if (r < r1) {
-            if (!g.alone) {
+            if (g.part >= 0) {
                 *reinterpret_cast<float2*>(A.part_ml + 2 * part) = make_float2(base, l);
             } else if (A.lse) {
-                A.lse[int64_t(g.s.row0 + r / A.group) * A.q_heads + g.head * A.group + r % A.group] = l == 0.f ? -INFINITY : 0.69314718055994531f * (base + log2f(l));
+                A.lse[out_row * A.q_heads + out_head] = l == 0.f ? -INFINITY : 0.69314718055994531f * (base + log2f(l));
             }
         }
         tm_fence_before();
@@ -436,20 +425,67 @@ __device__ __forceinline__ void tile_softmax(const AttentionArgs& A, unsigned ch
 template <class T, int D>
 __device__ __forceinline__ void tile_load(const AttentionArgs& A, unsigned char* smem, TileCtl* ctl) {
     using S = TileShape<T, D>;
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, H = A.cache.heads;
     const int shift = min(A.page_shift, 7); // a copy's tokens
-    Worker work(A);
-    Segment g;
     uint32_t step = 0;
     Ring<S::kKStages> kr;
     Ring<S::kVStages> vr;
+    Ring<kSegments> segments;
+    // the block's share, or its unit: those of the last rows, which see the most keys, come first
+    int64_t left = 1, done = 0, size = 0, at = 0; // at: on the line
+    int tile = A.batch.sequences * A.row_tiles - 1 - blockIdx.x / H, head = blockIdx.x % H;
+    Split split{0, 0, int(blockIdx.x), 0};
+    if (A.part_o) {
+        const Line line = line_of(A, blockIdx.x, gridDim.x);
+        left = line.left, size = line.size, at = size * blockIdx.x, tile = line.tile;
+        if (left > 0) {
+            const int g = weight_of(A, tile);
+            head = int((at - line.start) / g), done = at - line.start - int64_t(head) * g;
+        }
+    }
 #pragma unroll 1
-    while (work.next(A, g)) {
+    while (true) {
+        Segment g{};
+        int b = 0;
+        while (left > 0) {
+            const Tile own = tile_at(A, tile);
+            if (own.rows == 0) {
+                left = A.part_o ? left : 0;
+                tile++, head = 0;
+                continue;
+            }
+            const TileKeys keys = keys_of_tile(A, own.s, own.r0, own.r0 + own.rows);
+            const int all = max(1, keys.g1 - keys.g0);
+            // what of the unit's stretch of the line is the share's, without the cost at its head
+            const int64_t to = A.part_o ? min(int64_t(all + A.unit_cost), done + left) : all + A.unit_cost, unit_at = at - done;
+            const int ga = max(0, int(done) - A.unit_cost), gb = max(0, int(to) - A.unit_cost);
+            left = A.part_o ? left - (to - done) : 0, at = unit_at + to, done = 0;
+            b = A.row_tiles == 1 ? tile : tile / A.row_tiles;
+            g.head = head, g.r0 = own.r0, g.rows = own.rows, g.row0 = own.s.row0, g.place0 = own.s.place0, g.len = own.s.len, g.lo = keys.lo, g.hi = keys.hi;
+            g.ga = keys.g0 + ga, g.gb = keys.g0 + gb;
+            g.part = gb - ga == all ? -1 : 2 * int(blockIdx.x) + (ga == 0 ? 1 : 0);
+            if (A.part_o && ga == 0 && gb > 0 && gb < all) {
+                split.tile = tile, split.head = head, split.last = int((unit_at + all + A.unit_cost - 1) / size);
+            }
+            if (++head == H) {
+                head = 0, tile++;
+            }
+            break;
+        }
+        tile_wait(&ctl->seg_empty[segments.i], segments.phase ^ 1, &ctl->abort);
+        if (lane == 0) {
+            ctl->seg[segments.i] = g;
+            bar_arrive(shared_u32(&ctl->seg_full[segments.i]));
+        }
+        segments.next();
         const int n = g.gb - g.ga;
+        if (n == 0 || *static_cast<volatile int*>(&ctl->abort)) {
+            break;
+        }
         // a lane looks 16 keys up, 8 lanes a tile, four tiles at a time
         auto look_up = [&](int first) {
             const int i = first + (lane >> 3), key = (g.ga + i) * kTileKeys + (lane & 7) * 16;
-            return piece_at(A, g.b, g.head, key, i < n && key < g.keys.hi && key + 16 > g.keys.lo);
+            return piece_at(A, b, g.head, key, i < n && key < g.hi && key + 16 > g.lo);
         };
         Piece now = look_up(0), next = look_up(4);
 #pragma unroll 1
@@ -494,19 +530,22 @@ __device__ __forceinline__ void tile_load(const AttentionArgs& A, unsigned char*
         }
         step += n;
     }
+    if (A.part_o && lane == 0) {
+        A.splits[blockIdx.x] = split;
+    }
 }
 
 template <class T, int D>
-__device__ __forceinline__ void tile_convert(const AttentionArgs& A, unsigned char* smem, TileCtl* ctl) {
+__device__ __forceinline__ void tile_convert(unsigned char* smem, TileCtl* ctl) {
     using S = TileShape<T, D>;
-    const int tid = threadIdx.x & 127;
-    Worker work(A);
+    const int tid = threadIdx.x - (kTileThreads - 32 * kConvertWarps);
+    Ring<kSegments> segments;
     Segment g;
     uint32_t step = 0;
     Ring<S::kVStages> vr;
     Ring<S::kHStages> hr;
 #pragma unroll 1
-    while (work.next(A, g)) {
+    while (next_segment(ctl, segments, g)) {
         const int n = g.gb - g.ga;
 #pragma unroll 1
         for (int i = 0; i < n; i++) {
@@ -514,11 +553,11 @@ __device__ __forceinline__ void tile_convert(const AttentionArgs& A, unsigned ch
             tile_wait(&ctl->h_empty[hr.i], hr.phase ^ 1, &ctl->abort);
             const uint32_t absent = ctl->absent[(step + i) % kScaleSlots];
             const int key0 = (g.ga + i) * kTileKeys;
-            const bool edge = absent || key0 < g.keys.lo || key0 + kTileKeys > g.keys.hi;
+            const bool edge = absent || key0 < g.lo || key0 + kTileKeys > g.hi;
             const uint4* from = reinterpret_cast<const uint4*>(smem + S::kOffV + vr.i * S::kCodes);
             uint4* to = reinterpret_cast<uint4*>(smem + S::kOffH + hr.i * 2 * S::kCodes);
 #pragma unroll 4
-            for (int c = tid; c < 8 * D; c += 128) { // 16 keys of a dim
+            for (int c = tid; c < 8 * D; c += 32 * kConvertWarps) { // 16 keys of a dim
                 uint4 w = from[c];
                 const int k16 = c / D, d = c % D;
                 if (edge) { // an unused slot may hold NaN, and 0 * NaN is NaN
@@ -526,7 +565,7 @@ __device__ __forceinline__ void tile_convert(const AttentionArgs& A, unsigned ch
                     auto keep = [&](uint32_t x, int key) {
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            if (gone || key + e < g.keys.lo || key + e >= g.keys.hi) {
+                            if (gone || key + e < g.lo || key + e >= g.hi) {
                                 x &= ~(0xFFu << (8 * e));
                             }
                         }
@@ -551,90 +590,93 @@ __device__ __forceinline__ void tile_convert(const AttentionArgs& A, unsigned ch
     }
 }
 
-// The products of tile t: p V of 64 keys, then the S that takes p's place. A warp for each tile: what it runs between two batches is fetched
-// anew each time, some 5 cycles an instruction, and one warp for both, whatever the order, held the tiles up to 5000 cycles a step.
+// The products, a warp for each kind and tile: S as soon as p V has read p from its buffer, p V as soon as p is there. What a warp runs
+// between two batches is fetched anew each time, some 5 cycles an instruction: one warp that polled for whatever was ready held the tiles
+// up to 5500 cycles a step, one warp for each tile to 4000.
 template <class T, int D>
-__device__ __forceinline__ void tile_products(const AttentionArgs& A, unsigned char* smem, TileCtl* ctl, uint32_t t) {
+__device__ __forceinline__ void tile_scores(unsigned char* smem, TileCtl* ctl, uint32_t t) {
     using S = TileShape<T, D>;
-    const uint32_t el = elected(), sm = uniform(shared_u32(smem)), bars = uniform(shared_u32(ctl));
-    const uint32_t is = tile_idesc(kTileRows, kHalfKeys), io = tile_idesc(kTileRows, D);
-    const uint32_t ts = uniform(ctl->tmem + t * 128), to = ts - t * 128 + 256 + t * 128, q = uniform(desc_low(sm + t * S::kTerms * S::kQ, 128));
-    const uint32_t q_full = bars + offsetof(TileCtl, q_full) + 8 * t, s_full = bars + offsetof(TileCtl, s_full) + 16 * t;
-    const uint32_t p_full = bars + offsetof(TileCtl, p_full) + 16 * t, o_done = bars + offsetof(TileCtl, o_done) + 16 * t;
+    const uint32_t el = elected(), sm = uniform(shared_u32(smem)), bars = uniform(shared_u32(ctl)), is = tile_idesc(kTileRows, kHalfKeys);
+    const uint32_t ts = uniform(ctl->tmem + t * 128), q = uniform(desc_low(sm + t * S::kTerms * S::kQ, 128)), k0 = desc_low(sm + S::kOffK, 128);
+    const uint32_t s_full = bars + offsetof(TileCtl, s_full) + 16 * t, o_done = bars + offsetof(TileCtl, o_done) + 16 * t;
     volatile int* abort = &ctl->abort;
     Ring<S::kKStages> kr;
-    Ring<S::kHStages> hr;
-    uint32_t turn = 0, units = 0; // parities: of the tile's steps, of its units
-    Worker work(A);
+    Ring<kSegments> segments;
     Segment g;
+    uint32_t turn = 0, units = 0; // parities: of the tile's steps before this one, of its units
 #pragma unroll 1
-    while (work.next(A, g)) {
+    while (next_segment(ctl, segments, g)) {
         const int n = uniform(g.gb - g.ga);
-        if (uniform(g.rows) <= kTileRows * t) { // no second tile: its share of the stages is given back
-#pragma unroll 1
-            for (int i = 0; i < n; i++) {
-                tile_wait(bars + offsetof(TileCtl, k_full) + 8 * kr.i, kr.phase, abort);
-                tile_wait(bars + offsetof(TileCtl, h_full) + 8 * hr.i, hr.phase, abort);
-                if (el) {
-                    bar_arrive(bars + offsetof(TileCtl, k_empty) + 8 * kr.i), bar_arrive(bars + offsetof(TileCtl, h_empty) + 8 * hr.i);
-                }
-                kr.next(), hr.next();
-            }
-            continue;
+        const bool mine = uniform(g.rows) > kTileRows * t; // else no second tile: its share of the stages is given back
+        if (mine) {
+            tile_wait(bars + offsetof(TileCtl, q_full) + 8 * t, units, abort);
+            units ^= 1;
         }
-        auto scores = [&](uint32_t k, int h) {
-            tm_fence_after();
+#pragma unroll 1
+        for (int i = 0; i < n; i++) {
+            const uint32_t k = uniform(k0 + kr.i * (S::kCodes >> 4));
+            tile_wait(bars + offsetof(TileCtl, k_full) + 8 * kr.i, kr.phase, abort);
+            if (mine) {
 #pragma unroll
-            for (int m = 0; m < S::kTerms; m++) {
+                for (int h = 0; h < 2; h++) {
+                    if (i > 0) { // p of the step before, which lies where S goes, has been read
+                        tile_wait(o_done + 8 * h, turn ^ 1, abort);
+                    }
+                    tm_fence_after();
 #pragma unroll
-                for (int c = 0; c < D / 32; c++) {
-                    mma_codes(el, ts + h * kHalfKeys, q + m * (S::kQ >> 4) + c * 16, desc_high(8 * D), k + h * (kHalfKeys * D >> 4) + c * 16, desc_high(8 * D), is, m + c > 0);
+                    for (int m = 0; m < S::kTerms; m++) {
+#pragma unroll
+                        for (int c = 0; c < D / 32; c++) {
+                            mma_codes(el, ts + h * kHalfKeys, q + m * (S::kQ >> 4) + c * 16, desc_high(8 * D), k + h * (kHalfKeys * D >> 4) + c * 16, desc_high(8 * D), is, m + c > 0);
+                        }
+                    }
+                    mma_commit(el, s_full + 8 * h);
+                    if (el) { // the scales, which came with K, are the softmax's to read
+                        bar_arrive(s_full + 8 * h);
+                    }
                 }
+                turn ^= 1;
             }
-            mma_commit(el, s_full + 8 * h);
-            if (el) { // the scales, which came with K, are the softmax's to read
-                bar_arrive(s_full + 8 * h);
-            }
-        };
-        const uint32_t k0 = desc_low(sm + S::kOffK, 128), v0 = desc_low(sm + S::kOffH, 16 * D);
-        tile_wait(q_full, units, abort);
-        tile_wait(bars + offsetof(TileCtl, k_full) + 8 * kr.i, kr.phase, abort);
-        uint32_t k = uniform(k0 + kr.i * (S::kCodes >> 4));
-        scores(k, 0), scores(k, 1);
-        mma_commit(el, bars + offsetof(TileCtl, k_empty) + 8 * kr.i);
-        kr.next();
+            mma_commit(el, bars + offsetof(TileCtl, k_empty) + 8 * kr.i);
+            kr.next();
+        }
+    }
+}
+template <class T, int D>
+__device__ __forceinline__ void tile_sums(unsigned char* smem, TileCtl* ctl, uint32_t t) {
+    using S = TileShape<T, D>;
+    const uint32_t el = elected(), sm = uniform(shared_u32(smem)), bars = uniform(shared_u32(ctl)), io = tile_idesc(kTileRows, D);
+    const uint32_t ts = uniform(ctl->tmem + t * 128), to = uniform(ctl->tmem + 256 + t * 128), v0 = desc_low(sm + S::kOffH, 16 * D);
+    const uint32_t p_full = bars + offsetof(TileCtl, p_full) + 16 * t, o_done = bars + offsetof(TileCtl, o_done) + 16 * t;
+    volatile int* abort = &ctl->abort;
+    Ring<S::kHStages> hr;
+    Ring<kSegments> segments;
+    Segment g;
+    uint32_t turn = 0;
+#pragma unroll 1
+    while (next_segment(ctl, segments, g)) {
+        const int n = uniform(g.gb - g.ga);
+        const bool mine = uniform(g.rows) > kTileRows * t;
 #pragma unroll 1
         for (int i = 0; i < n; i++) {
             const uint32_t v = uniform(v0 + hr.i * (2 * S::kCodes >> 4));
-            k = uniform(k0 + kr.i * (S::kCodes >> 4));
             tile_wait(bars + offsetof(TileCtl, h_full) + 8 * hr.i, hr.phase, abort);
+            if (mine) {
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                tile_wait(p_full + 8 * h, turn, abort);
-                tm_fence_after();
+                for (int h = 0; h < 2; h++) {
+                    tile_wait(p_full + 8 * h, turn, abort);
+                    tm_fence_after();
 #pragma unroll
-                for (int c = 0; c < kHalfKeys / 16; c++) {
-                    mma_halves(el, to, ts + h * kHalfKeys + 8 * c, v + (h * kHalfKeys / 16 + c) * 2 * D, desc_high(128), io, h + c > 0 ? 1 : i);
-                }
-                mma_commit(el, o_done + 8 * h);
-                if (h == 1) {
-                    mma_commit(el, bars + offsetof(TileCtl, h_empty) + 8 * hr.i);
-                }
-                if (i + 1 < n) {
-                    if (h == 0) {
-                        tile_wait(bars + offsetof(TileCtl, k_full) + 8 * kr.i, kr.phase, abort);
+                    for (int c = 0; c < kHalfKeys / 16; c++) {
+                        mma_halves(el, to, ts + h * kHalfKeys + 8 * c, v + (h * kHalfKeys / 16 + c) * 2 * D, desc_high(128), io, h + c > 0 ? 1 : i);
                     }
-                    tile_wait(o_done + 8 * h, turn, abort);
-                    scores(k, h);
+                    mma_commit(el, o_done + 8 * h);
                 }
+                turn ^= 1;
             }
-            if (i + 1 < n) {
-                mma_commit(el, bars + offsetof(TileCtl, k_empty) + 8 * kr.i);
-                kr.next();
-            }
-            hr.next(), turn ^= 1;
+            mma_commit(el, bars + offsetof(TileCtl, h_empty) + 8 * hr.i);
+            hr.next();
         }
-        units ^= 1;
     }
 }
 
@@ -654,10 +696,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
             for (int h = 0; h < 2; h++) {
                 init(ctl->s_full[t][h], 2), init(ctl->p_full[t][h], kTileRows), init(ctl->o_done[t][h], 1);
             }
-            init(ctl->v_full[t], 1), init(ctl->v_empty[t], 4), init(ctl->h_full[t], 4), init(ctl->h_empty[t], 2);
+            init(ctl->v_full[t], 1), init(ctl->v_empty[t], kConvertWarps), init(ctl->h_full[t], kConvertWarps), init(ctl->h_empty[t], 2);
         }
         for (int i = 0; i < 3; i++) {
             init(ctl->k_full[i], 1), init(ctl->k_empty[i], 2);
+        }
+        for (int i = 0; i < kSegments; i++) {
+            init(ctl->seg_full[i], 1), init(ctl->seg_empty[i], kReaders);
         }
         bar_init_done();
         ctl->abort = 0;
@@ -673,10 +718,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
         tile_softmax<T, D>(A, smem, ctl);
     } else if (warp == 8) {
         tile_load<T, D>(A, smem, ctl);
-    } else if (warp == 9 || warp == 10) {
-        tile_products<T, D>(A, smem, ctl, warp - 9);
-    } else if (warp >= 12) {
-        tile_convert<T, D>(A, smem, ctl);
+    } else if (warp < 11) {
+        tile_scores<T, D>(smem, ctl, warp - 9);
+    } else if (warp < 13) {
+        tile_sums<T, D>(smem, ctl, warp - 11);
+    } else {
+        tile_convert<T, D>(smem, ctl);
     }
     tm_fence_before();
     __syncthreads();

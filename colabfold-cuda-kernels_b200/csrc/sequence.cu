@@ -217,7 +217,7 @@ struct Plan {
     int64_t blocks;
     bool shares;
     int merge_y;
-    size_t part_bytes, bytes; // of the workspace
+    size_t part_bytes, ml_bytes, bytes; // of the workspace
 };
 Plan make_plan(const cck_cache& c, const cck_batch& b, int q_heads, int sms) {
     Plan p{};
@@ -234,7 +234,8 @@ Plan make_plan(const cck_cache& c, const cck_batch& b, int q_heads, int sms) {
     if (p.shares) {
         p.merge_y = p.nt == 0 ? 16 : units < 64 ? p.tile_rows : 1;
         p.part_bytes = size_t(2 * p.blocks) * p.tile_rows * c.dim * 4;
-        p.bytes = p.part_bytes + size_t(2 * p.blocks) * p.tile_rows * 8;
+        p.ml_bytes = size_t(2 * p.blocks) * p.tile_rows * 8;
+        p.bytes = p.part_bytes + p.ml_bytes + size_t(p.blocks) * sizeof(Split);
     }
     return p;
 }
@@ -439,10 +440,11 @@ int cck_cache_attention(void* stream, const cck_cache* cache, const cck_batch* b
     a.qr = q->row_stride, a.qh = q->head_stride, a.or_ = out->row_stride, a.oh = out->head_stride;
     a.scale_log2 = softmax_scale * 1.4426950408889634f;
     a.q_heads = q->heads, a.group = q->heads / cache->heads, a.causal = causal != 0, a.window = window;
-    a.granule = p.granule, a.page_shift = __builtin_ctz(cache->page_tokens);
+    a.granule_shift = __builtin_ctz(p.granule), a.unit_cost = p.nt ? 8 : 3, a.page_shift = __builtin_ctz(cache->page_tokens);
     a.tile_rows = p.tile_rows, a.row_tiles = p.row_tiles;
     if (p.shares) {
         a.part_o = static_cast<float*>(ws), a.part_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + p.part_bytes);
+        a.splits = reinterpret_cast<Split*>(static_cast<char*>(ws) + p.part_bytes + p.ml_bytes);
     }
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     return launched(op, q->dtype == CCK_BF16 ? launch_attention<__nv_bfloat16>(st, a, p) : launch_attention<__half>(st, a, p));
