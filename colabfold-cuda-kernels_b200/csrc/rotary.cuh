@@ -2,9 +2,11 @@
 //
 //   pair (a, b) of a head, angle t = pos[axis of the pair][row] * freq[pair]:  (a cos t - b sin t, b cos t + a sin t)
 //
-// Bound by memory: every value is read once and written once. The angles belong to a row and are shared by its heads, so a thread
-// keeps V pairs of one row in registers and goes through the heads with them: the reduction of the argument in 64 bits costs what a
-// few heads' rotation does. V pairs are one or two vectors of up to 16 bytes on each side.
+// Bound by memory: every value is read once and written once. The angles belong to a row and are shared by its heads: a warp takes a row,
+// or a part of a row's heads where rows are few, computes the row's cosines and sines once, into its own shared memory, while the first
+// vectors are on their way; a lane then keeps V pairs and goes through heads with them. V pairs are one or two vectors of up to 16 bytes on
+// each side. Warps wait for nobody and go from row to row: blocks that shared a table of several rows spent 3.5 us each, mostly waiting,
+// and 8192 rows of 40 heads took 55 us.
 #pragma once
 
 #include "sequence.cuh"
@@ -14,94 +16,180 @@ namespace seq {
 
 // the axis that pair p turns with
 __device__ __forceinline__ int axis_of(const cck_rotation& r, int p) {
-    int a = 0, edge = r.section[0];
-    while (a < r.axes - 1 && p >= edge) {
-        edge += r.section[++a];
+    int edge = r.section[0];
+    if (r.axes == 1 || p < edge) {
+        return 0;
     }
-    return a;
+    edge += r.section[1];
+    if (r.axes == 2 || p < edge) {
+        return 1;
+    }
+    return r.axes == 3 || p < edge + r.section[2] ? 2 : 3;
 }
-// Turns of pair p at position pos, reduced to [-1/2, 1/2] in 64 bits: of a position of a million and a frequency of 1 an f32 product
-// would leave 0.03 radians open. What is left fits f32 to 2^-25 of a turn.
-__device__ __forceinline__ float2 cos_sin(int pos, float freq) {
-    const double turns = double(pos) * double(freq) * 0.15915494309189533577;
-    const float t = float(turns - rint(turns));
-    float2 cs;
-    sincospif(2.f * t, &cs.y, &cs.x);
-    return cs;
+// A frequency as turns per position modulo one, in units of 2^-64: position times this, modulo 2^64, is the angle reduced without an error but
+// the frequency's (the product in 64 bits and this rounding: 2^-25 of a turn at a position times frequency of 2^31). An f32 product
+// would leave 0.03 radians open at a position of a million.
+struct Turns {
+    uint64_t per;
+    bool finite;
+};
+__device__ __forceinline__ Turns turns_of(float freq) {
+    const double x = double(freq) * 0.15915494309189533577, f = x - floor(x);
+    return {f < 1.0 ? __double2ull_rn(f * 18446744073709551616.0) : 0, freq - freq == 0.f};
+}
+// The nearest quarter turn is taken off in integers; what is left, at most pi / 4, goes through the Taylor series of sine and cosine about
+// zero to the ninth and tenth power (the terms after them are below 2e-9 of the result), half of what sincospif() takes.
+__device__ __forceinline__ float2 cos_sin(int pos, Turns t) {
+    const int32_t angle = int32_t((t.per * uint64_t(int64_t(pos))) >> 32);     // of a turn, in 2^-32
+    const int32_t quarter = int32_t(uint32_t(angle) + 0x20000000u) >> 30;       // -2 .. 1
+    const float x = __int2float_rn(int32_t(uint32_t(angle) - (uint32_t(quarter) << 30))) * 1.46291807926715968e-9f, y = x * x; // 2 pi / 2^32
+    float s = fmaf(y, 1.f / 362880.f, -1.f / 5040.f), c = fmaf(y, -1.f / 3628800.f, 1.f / 40320.f);
+    s = fmaf(y, s, 1.f / 120.f), c = fmaf(y, c, -1.f / 720.f);
+    s = fmaf(y, s, -1.f / 6.f), c = fmaf(y, c, 1.f / 24.f);
+    s = fmaf(x * y, s, x), c = fmaf(y, c, -0.5f);
+    c = fmaf(y, c, 1.f);
+    // a quarter turn on: (c, s) -> (-s, c)
+    const bool odd = quarter & 1;
+    const float u = odd ? s : c, v = odd ? c : s;
+    const uint32_t flip_c = uint32_t(quarter + 1) & 2u, flip_s = uint32_t(quarter) & 2u;
+    const float2 cs = make_float2(__uint_as_float(__float_as_uint(u) ^ flip_c << 30), __uint_as_float(__float_as_uint(v) ^ flip_s << 30));
+    return t.finite ? cs : make_float2(__int_as_float(0x7fffffff), __int_as_float(0x7fffffff));
 }
 __device__ __forceinline__ float2 rotate(float a, float b, float2 cs) {
     return make_float2(fmaf(a, cs.x, -b * cs.y), fmaf(b, cs.x, a * cs.y));
 }
 
-// Rows of `x` rotated into `y` by the threads t of a block of nt, which is the g-th of a set. A row has `items` items a head: pairs
-// [V p, V p + V) for p < rot_items, then 2V copied dimensions each. hs threads share a row's heads.
+// Cosines and sines of `rows` rows from row0 on, all pairs: table[row][pair]. The block's threads t of nt
+__device__ __forceinline__ void fill_table(const cck_rotation& R, float2* table, int64_t row0, int rows, int t, int nt) {
+    const int pairs = R.dims / 2;
+    const int step = nt > pairs ? nt / pairs : 1; // rows at once
+    // a thread stays with a pair where it can: its frequency is converted once
+    for (int p = t % pairs; p < pairs; p += nt) {
+        const Turns f = turns_of(R.freq[p]);
+        const int* pos = R.pos + axis_of(R, p) * R.pos_stride + row0;
+        if (nt > pairs && t >= step * pairs) {
+            return;
+        }
+#pragma unroll 4
+        for (int r = nt > pairs ? t / pairs : 0; r < rows; r += step) {
+            table[r * pairs + p] = cos_sin(pos[r], f);
+        }
+    }
+}
+
+// x rotated into y, a unit (one of `splits` parts of a row's heads) after the other: those of warp `unit`, + step, ... A head of a row has `items`
+// items: pairs [V p, V p + V) for p < rot_items, then 2V copied dimensions each. table: the warp's own, dims / 2 entries.
 struct RotaryShape {
-    int rows, dim, heads, rot_items, items, hs, sign;
+    int rows, dim, heads, rot_items, items, splits, part_heads, sign;
+    int64_t units;
     int64_t xr, xh, yr, yh;
     const void* x;
     void* y;
 };
-template <class T, int V>
-__device__ __forceinline__ void rotary_block(const cck_rotation& R, const RotaryShape& s, int g, int t, int nt) {
-    using Vt = Vec<T, V>;
-    const int slots = nt / s.items, item = t % s.items;
-    const int64_t slot = int64_t(g) * slots + t / s.items;
-    const int64_t row = slot / s.hs;
-    const int h0 = int(slot % s.hs);
-    if (t >= slots * s.items || row >= s.rows) {
-        return;
+template <class T, int V, bool kAdjacent>
+__device__ __forceinline__ void rotary_warp(const cck_rotation& R, const RotaryShape& s, float2* table, int64_t unit, int64_t step) {
+    using Vt = Words<V * sizeof(T)>;
+    const int lane = threadIdx.x & 31, pairs = R.dims / 2;
+    // the frequencies of this lane's first pairs, and their axes, stay
+    constexpr int kKept = 2;
+    Turns kept[kKept];
+    const int* pos[kKept];
+#pragma unroll
+    for (int k = 0; k < kKept; k++) {
+        if (const int p = lane + 32 * k; p < pairs) {
+            kept[k] = turns_of(R.freq[p]), pos[k] = R.pos + axis_of(R, p) * R.pos_stride;
+        }
     }
-    const bool turn = item < s.rot_items;
-    const int p0 = item * V;
-    // where the item's two vectors lie inside a head
-    const int i0 = turn ? (R.adjacent ? 2 * p0 : p0) : R.dims + (item - s.rot_items) * 2 * V;
-    const int i1 = turn && !R.adjacent ? p0 + R.dims / 2 : i0 + V;
-    const bool both = turn || i1 < s.dim;
-    const T* x = static_cast<const T*>(s.x) + row * s.xr;
-    T* y = static_cast<T*>(s.y) + row * s.yr;
-    constexpr int kAhead = 4; // heads whose loads are on their way together
-    float2 cs[V];
-    for (int h = h0; h < s.heads; h += kAhead * s.hs) {
-        Vt a[kAhead], b[kAhead];
+    const int stride = s.items < 32 ? 32 / s.items : 1, first = s.items < 32 ? lane / s.items : 0; // heads at once; this lane's
+    const int64_t xs = stride * s.xh, ys = stride * s.yh;
+#pragma unroll 1
+    for (; unit < s.units; unit += step) {
+        const int64_t row = s.splits == 1 ? unit : unit / s.splits;
+        const int h_begin = s.splits == 1 ? 0 : int(unit - row * s.splits) * s.part_heads;
+        const int heads = first < stride ? max(0, ceil_div(min(s.part_heads, s.heads - h_begin) - first, stride)) : 0; // of this lane
+#pragma unroll 1
+        for (int item0 = 0; item0 < s.items; item0 += 32) {
+            const int item = s.items < 32 ? lane - first * s.items : item0 + lane;
+            const bool turn = item < s.rot_items;
+            const int p0 = item * V;
+            // where the item's two vectors lie inside a head
+            const int i0 = turn ? (kAdjacent ? 2 * p0 : p0) : R.dims + (item - s.rot_items) * 2 * V;
+            const int i1 = turn && !kAdjacent ? p0 + pairs : i0 + V;
+            const bool both = turn || i1 < s.dim;
+            const T* x = static_cast<const T*>(s.x) + row * s.xr + (h_begin + first) * s.xh + i0;
+            T* y = static_cast<T*>(s.y) + row * s.yr + (h_begin + first) * s.yh + i0;
+            const int over = i1 - i0, mine = item < s.items ? heads : 0;
+            constexpr int kAhead = 4; // heads whose loads are on their way together
+            Vt a[kAhead], b[kAhead];
+            auto load = [&](int left) {
 #pragma unroll
-        for (int u = 0; u < kAhead; u++) {
-            if (const int hh = h + u * s.hs; hh < s.heads) {
-                a[u] = *reinterpret_cast<const Vt*>(x + hh * s.xh + i0);
-                b[u] = both ? *reinterpret_cast<const Vt*>(x + hh * s.xh + i1) : a[u];
-            }
-        }
-        if (h == h0 && turn) { // behind the first loads
-#pragma unroll
-            for (int v = 0; v < V; v++) {
-                const int p = p0 + v;
-                cs[v] = cos_sin(R.pos[axis_of(R, p) * R.pos_stride + row], R.freq[p]);
-                cs[v].y = s.sign < 0 ? -cs[v].y : cs[v].y;
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < kAhead; u++) {
-            if (const int hh = h + u * s.hs; hh < s.heads) {
-                if (turn) {
-#pragma unroll
-                    for (int v = 0; v < V; v++) {
-                        T &pa = R.adjacent ? (2 * v < V ? a[u].v[(2 * v) % V] : b[u].v[(2 * v) % V]) : a[u].v[v];
-                        T &pb = R.adjacent ? (2 * v + 1 < V ? a[u].v[(2 * v + 1) % V] : b[u].v[(2 * v + 1) % V]) : b[u].v[v];
-                        const float2 z = rotate(to_f32(pa), to_f32(pb), cs[v]);
-                        pa = from_f32<T>(z.x), pb = from_f32<T>(z.y);
+                for (int u = 0; u < kAhead; u++, x += xs) {
+                    if (u < left) {
+                        a[u] = *reinterpret_cast<const Vt*>(x);
+                        b[u] = both ? *reinterpret_cast<const Vt*>(x + over) : a[u];
                     }
                 }
-                *reinterpret_cast<Vt*>(y + hh * s.yh + i0) = a[u];
-                if (both) {
-                    *reinterpret_cast<Vt*>(y + hh * s.yh + i1) = b[u];
+            };
+            load(mine);
+            if (item0 == 0) {
+                __syncwarp(); // the last row's table has been read
+#pragma unroll
+                for (int k = 0; k < kKept; k++) {
+                    if (lane + 32 * k < pairs) {
+                        table[lane + 32 * k] = cos_sin(pos[k][row], kept[k]);
+                    }
                 }
+#pragma unroll 1
+                for (int p = lane + 32 * kKept; p < pairs; p += 32) {
+                    table[p] = cos_sin(R.pos[axis_of(R, p) * R.pos_stride + row], turns_of(R.freq[p]));
+                }
+                __syncwarp();
+            }
+            float2 cs[V];
+            if (turn) {
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    cs[v] = table[p0 + v];
+                    cs[v].y = s.sign < 0 ? -cs[v].y : cs[v].y;
+                }
+            }
+#pragma unroll 1
+            for (int left = mine; left > 0; left -= kAhead) {
+#pragma unroll
+                for (int u = 0; u < kAhead; u++, y += ys) {
+                    if (u >= left) {
+                        break;
+                    }
+                    if (turn) {
+                        float p[V], q[V];
+                        to_floats<T, V>(a[u], p), to_floats<T, V>(b[u], q);
+#pragma unroll
+                        for (int v = 0; v < V; v++) {
+                            // pair v: of the two vectors, or neighbours in their 2 V values
+                            float &pa = !kAdjacent || 2 * v < V ? p[kAdjacent ? 2 * v % V : v] : q[2 * v % V];
+                            float &pb = kAdjacent && 2 * v + 1 < V ? p[(2 * v + 1) % V] : q[kAdjacent ? (2 * v + 1) % V : v];
+                            const float2 z = rotate(pa, pb, cs[v]);
+                            pa = z.x, pb = z.y;
+                        }
+                        a[u] = from_floats<T, V>(p), b[u] = from_floats<T, V>(q);
+                    }
+                    *reinterpret_cast<Vt*>(y) = a[u];
+                    if (both) {
+                        *reinterpret_cast<Vt*>(y + over) = b[u];
+                    }
+                }
+                load(left - kAhead);
             }
         }
     }
 }
 
-template <class T, int V>
-__global__ void __launch_bounds__(512) rotary_kernel(const cck_rotation R, const RotaryShape s) {
-    rotary_block<T, V>(R, s, blockIdx.x, threadIdx.x, blockDim.x);
+constexpr int kRotaryThreads = 256;
+template <class T, int V, bool kAdjacent>
+__global__ void __launch_bounds__(kRotaryThreads, 3) rotary_kernel(const __grid_constant__ cck_rotation R, const __grid_constant__ RotaryShape s) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    const int warp = threadIdx.x >> 5, warps = kRotaryThreads / 32;
+    rotary_warp<T, V, kAdjacent>(R, s, reinterpret_cast<float2*>(smem) + warp * (R.dims / 2), int64_t(blockIdx.x) * warps + warp, int64_t(gridDim.x) * warps);
 }
 
 } // namespace seq

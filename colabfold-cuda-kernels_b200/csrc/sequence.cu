@@ -2,6 +2,7 @@
 // Declarations: include/cck_b200.h.
 #include <atomic>
 #include <cstdio>
+#include <type_traits>
 
 #include "cache_append.cuh"
 #include "cache_attention_tile.cuh"
@@ -157,55 +158,102 @@ int rotary_vector(const cck_rotation& r, int dim, const cck_rows& x, const cck_r
     }
     return 1;
 }
+// How rows and heads are dealt out to warps, of which a multiprocessor holds 24: whole rows, or parts of a row's heads where rows are few, down to
+// one head a lane
 RotaryShape rotary_shape(const cck_rotation& r, int rows, int dim, const cck_rows& x, const cck_rows& y, bool inverse, int v, int sms) {
     RotaryShape s{};
     s.rows = rows, s.dim = dim, s.heads = x.heads, s.sign = inverse ? -1 : 1;
     s.x = x.data, s.y = y.data, s.xr = x.row_stride, s.xh = x.head_stride, s.yr = y.row_stride, s.yh = y.head_stride;
     s.rot_items = r.dims / 2 / v;
     s.items = s.rot_items + (x.data == y.data ? 0 : ceil_div(dim - r.dims, 2 * v));
-    // threads that share a row's heads: few, since each computes the row's angles anew, but enough to fill the GPU
-    const int64_t want = int64_t(sms) * 2048, one = int64_t(rows) * (s.items ? s.items : 1);
-    s.hs = int(one >= want ? 1 : (want + one - 1) / one);
-    s.hs = s.hs < x.heads ? s.hs : x.heads;
+    if (s.items == 0) { // in place, and nothing turns
+        return s;
+    }
+    const int warps = 24 * sms, at_once = s.items < 32 ? 32 / s.items : 1, most = ceil_div(x.heads, at_once);
+    int splits = 1;
+    if (rows < warps) {
+        splits = ceil_div(warps, rows) < most ? ceil_div(warps, rows) : most;
+    } else { // a few rounds of rows: parts of a row where they fill the last round by a tenth better
+        auto time = [&](int n) { return double((int64_t(rows) * n + warps - 1) / warps) / n; };
+        for (int n = 2; n <= 4 && n <= most; n++) {
+            splits = time(n) < 0.9 * time(splits) ? n : splits;
+        }
+    }
+    s.part_heads = ceil_div(x.heads, splits);
+    s.splits = ceil_div(x.heads, s.part_heads);
+    s.units = int64_t(rows) * s.splits;
     return s;
 }
-int64_t rotary_blocks(const RotaryShape& s, int threads) {
-    const int slots = threads / s.items;
-    return (int64_t(s.rows) * s.hs + slots - 1) / slots;
+// blocks of `threads` that work through it: as many as fit the multiprocessors at once
+int64_t rotary_blocks(const RotaryShape& s, int threads, int sms) {
+    const int64_t all = (s.units + threads / 32 - 1) / (threads / 32), most = int64_t(24) * sms / (threads / 32);
+    return all < most ? all : most;
+}
+size_t rotary_smem(const cck_rotation& r, int threads) {
+    return size_t(threads / 32) * (r.dims / 2) * sizeof(float2);
 }
 
 template <class T>
-cudaError_t launch_rotary(cudaStream_t st, const cck_rotation& r, const RotaryShape& s, int v, int64_t blocks, int threads) {
+cudaError_t launch_rotary(cudaStream_t st, const cck_rotation& r, const RotaryShape& s, int v, int64_t blocks) {
     auto go = [&](auto kernel) {
-        kernel<<<unsigned(blocks), threads, 0, st>>>(r, s);
+        kernel<<<unsigned(blocks), kRotaryThreads, rotary_smem(r, kRotaryThreads), st>>>(r, s);
         return cudaGetLastError();
     };
     constexpr int kMost = 16 / sizeof(T);
-    switch (v) {
-    case 8: return go(rotary_kernel<T, kMost>);
-    case 4: return go(rotary_kernel<T, 4>);
-    case 2: return go(rotary_kernel<T, 2>);
-    default: return go(rotary_kernel<T, 1>);
+    if (r.adjacent) {
+        return v == 8 ? go(rotary_kernel<T, kMost, true>) : v == 4 ? go(rotary_kernel<T, 4, true>) : v == 2 ? go(rotary_kernel<T, 2, true>) : go(rotary_kernel<T, 1, true>);
     }
+    return v == 8 ? go(rotary_kernel<T, kMost, false>) : v == 4 ? go(rotary_kernel<T, 4, false>) : v == 2 ? go(rotary_kernel<T, 2, false>) : go(rotary_kernel<T, 1, false>);
 }
 
+// the attribute that a kernel of more than 48 KB needs, once a device
+template <class K>
+cudaError_t allow_shared(K kernel, int bytes, std::atomic<bool>* ready) {
+    int dev = 0;
+    if (cudaError_t e = cudaGetDevice(&dev)) {
+        return e;
+    }
+    if (!ready[dev].load(std::memory_order_relaxed)) {
+        if (cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) {
+            return e;
+        }
+        ready[dev].store(true, std::memory_order_relaxed);
+    }
+    return cudaSuccess;
+}
 template <class T>
-cudaError_t launch_append(cudaStream_t st, const AppendArgs& a, int v, unsigned blocks, size_t smem) {
-    auto go = [&](auto kernel) {
+cudaError_t launch_append(cudaStream_t st, const AppendArgs& a, bool pages, int v, unsigned blocks, size_t smem) {
+    const int threads = pages && a.group_threads > kAppendThreads ? a.group_threads : kAppendThreads;
+    auto go = [&](auto kernel, std::atomic<bool>* ready) {
         if (smem > 48 * 1024) {
-            if (cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem))) {
+            if (cudaError_t e = allow_shared(kernel, kAppendSmem, ready)) {
                 return e;
             }
         }
-        kernel<<<blocks, kAppendThreads, smem, st>>>(a);
+        kernel<<<blocks, threads, smem, st>>>(a);
         return cudaGetLastError();
     };
+    static std::atomic<bool> ready[12][kMaxDevices];
+    if constexpr (sizeof(T) == 2) {
+        auto of_dim = [&](auto adjacent) {
+            constexpr bool adj = decltype(adjacent)::value;
+            switch (a.cache.dim) {
+            case 32: return go(append_pages_kernel<T, 32, adj>, ready[4 + adj]);
+            case 64: return go(append_pages_kernel<T, 64, adj>, ready[6 + adj]);
+            case 96: return go(append_pages_kernel<T, 96, adj>, ready[8 + adj]);
+            default: return go(append_pages_kernel<T, 128, adj>, ready[10 + adj]);
+            }
+        };
+        if (pages) {
+            return a.rotation.adjacent ? of_dim(std::true_type{}) : of_dim(std::false_type{});
+        }
+    }
     constexpr int kMost = 16 / sizeof(T);
     switch (v) {
-    case 8: return go(append_kernel<T, kMost>);
-    case 4: return go(append_kernel<T, 4>);
-    case 2: return go(append_kernel<T, 2>);
-    default: return go(append_kernel<T, 1>);
+    case 8: return go(append_kernel<T, kMost>, ready[3]);
+    case 4: return go(append_kernel<T, 4>, ready[2]);
+    case 2: return go(append_kernel<T, 2>, ready[1]);
+    default: return go(append_kernel<T, 1>, ready[0]);
     }
 }
 
@@ -238,21 +286,6 @@ Plan make_plan(const cck_cache& c, const cck_batch& b, int q_heads, int sms) {
         p.bytes = p.part_bytes + p.ml_bytes + size_t(p.blocks) * sizeof(Split);
     }
     return p;
-}
-// the attribute that a kernel of more than 48 KB needs, once a device
-template <class K>
-cudaError_t allow_shared(K kernel, int bytes, std::atomic<bool>* ready) {
-    int dev = 0;
-    if (cudaError_t e = cudaGetDevice(&dev)) {
-        return e;
-    }
-    if (!ready[dev].load(std::memory_order_relaxed)) {
-        if (cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) {
-            return e;
-        }
-        ready[dev].store(true, std::memory_order_relaxed);
-    }
-    return cudaSuccess;
 }
 template <class T, int D, int NT>
 cudaError_t launch_decode(cudaStream_t st, const AttentionArgs& a, unsigned blocks) {
@@ -316,19 +349,15 @@ int cck_rotary(void* stream, const cck_rotation* rotation, int rows, int dim, co
     }
     const int v = rotary_vector(*rotation, dim, *x, *y);
     const RotaryShape s = rotary_shape(*rotation, rows, dim, *x, *y, inverse != 0, v, sms);
-    if (s.items == 0) { // in place and nothing turns
+    const int64_t blocks = rotary_blocks(s, kRotaryThreads, sms);
+    if (blocks == 0) {
         return CCK_OK;
-    }
-    const int threads = s.items > 256 ? 512 : 256;
-    const int64_t blocks = rotary_blocks(s, threads);
-    if (blocks > 0x7fffffff) {
-        return refuse(CCK_E_SHAPE, op, "too many rows for one launch");
     }
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (x->dtype) {
-    case CCK_BF16: return launched(op, launch_rotary<__nv_bfloat16>(st, *rotation, s, v, blocks, threads));
-    case CCK_F16: return launched(op, launch_rotary<__half>(st, *rotation, s, v, blocks, threads));
-    default: return launched(op, launch_rotary<float>(st, *rotation, s, v, blocks, threads));
+    case CCK_BF16: return launched(op, launch_rotary<__nv_bfloat16>(st, *rotation, s, v, blocks));
+    case CCK_F16: return launched(op, launch_rotary<__half>(st, *rotation, s, v, blocks));
+    default: return launched(op, launch_rotary<float>(st, *rotation, s, v, blocks));
     }
 }
 
@@ -369,29 +398,58 @@ int cck_cache_append(void* stream, const cck_cache* cache, const cck_batch* batc
     if (rotation) {
         a.rotation = *rotation;
     }
-    const int P = cache->page_tokens;
+    const int P = cache->page_tokens, D = cache->dim, most = batch->max_new < P ? batch->max_new : P; // new rows of a page
     a.blocks_per_seq = batch->max_new ? (batch->max_new + P - 2) / P + 1 : 0;
-    const int64_t kv = int64_t(batch->sequences) * a.blocks_per_seq * cache->heads;
     int64_t more = 0;
-    int vec = 1;
+    int vec = 0;
+    size_t smem = 0;
     if (q && batch->rows) {
-        vec = rotary_vector(*rotation, cache->dim, *q, *q_out);
-        a.q = rotary_shape(*rotation, batch->rows, cache->dim, *q, *q_out, false, vec, sms);
-        more = a.q.items ? rotary_blocks(a.q, kAppendThreads) : 0;
+        vec = rotary_vector(*rotation, D, *q, *q_out);
+        a.q = rotary_shape(*rotation, batch->rows, D, *q, *q_out, false, vec, sms);
+    }
+    const int64_t units = int64_t(batch->sequences) * a.blocks_per_seq;
+    // 16-bit values whose rotated part is whole vectors go through registers
+    const bool pages = k->dtype != CCK_F32 && a.rotation.dims % 16 == 0 && (vec == 0 || vec == 8);
+    int64_t kv;
+    if (pages) {
+        // threads of a (page, head): the fewest whose items cover the new rows; then blocks for a page's heads, as long as multiprocessors are
+        // left for them, or three each where a page's angles, which each computes anew, are few (1, 2, 4, 8 blocks a multiprocessor: 27, 37, 35,
+        // 44 us for the keys and values of eight prompts, 64 tokens of 64 pairs a page; 1, 2: 16.5, 14.5 us for 16 tokens of 32 pairs)
+        const int groups = (most + 14) / 16 + 1 < P / 16 ? (most + 14) / 16 + 1 : P / 16;
+        a.group_threads = 32;
+        while (most * (D / 16) > kKeyItems * a.group_threads || groups * (D / 2) > kValueItems * a.group_threads) {
+            a.group_threads *= 2;
+        }
+        const int passes = ceil_div(cache->heads, a.group_threads < kAppendThreads ? kAppendThreads / a.group_threads : 1);
+        const int angles = most * (a.rotation.dims / 2) / kAppendThreads; // of a thread
+        const int64_t want = units ? ((angles > 4 ? 1 : 3) * int64_t(sms) + units - 1) / units : 1;
+        a.head_splits = int(want < passes ? want : passes);
+        kv = units * a.head_splits;
+        const size_t table = size_t(most) * (a.rotation.dims / 2) * sizeof(float2);
+        smem = table > smem ? table : smem;
+    } else {
+        kv = units * cache->heads;
+        const size_t rows = append_smem(most, D, size_of(k->dtype));
+        smem = rows > smem ? rows : smem;
+    }
+    if (vec) {
+        const int threads = pages && a.group_threads > kAppendThreads ? a.group_threads : kAppendThreads;
+        more = rotary_blocks(a.q, threads, sms);
+        smem = more && rotary_smem(*rotation, threads) > smem ? rotary_smem(*rotation, threads) : smem;
     }
     if (kv + more > 0x7fffffff) {
         return refuse(CCK_E_SHAPE, op, "too many rows for one launch");
     }
+    a.kv_blocks = int(kv);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (kv + more == 0) {
         return CCK_OK;
     }
-    a.kv_blocks = int(kv);
-    const size_t smem = append_smem(batch->max_new < P ? batch->max_new : P, cache->dim, size_of(k->dtype));
-    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const unsigned blocks = unsigned(kv + more);
     switch (k->dtype) {
-    case CCK_BF16: return launched(op, launch_append<__nv_bfloat16>(st, a, vec, unsigned(kv + more), smem));
-    case CCK_F16: return launched(op, launch_append<__half>(st, a, vec, unsigned(kv + more), smem));
-    default: return launched(op, launch_append<float>(st, a, vec, unsigned(kv + more), smem));
+    case CCK_BF16: return launched(op, launch_append<__nv_bfloat16>(st, a, pages, vec, blocks, smem));
+    case CCK_F16: return launched(op, launch_append<__half>(st, a, pages, vec, blocks, smem));
+    default: return launched(op, launch_append<float>(st, a, false, vec, blocks, smem));
     }
 }
 

@@ -53,6 +53,76 @@ template <class T, int N>
 struct alignas(sizeof(T) * N) Vec {
     T v[N];
 };
+// the same as words, which stay packed in registers
+template <int kBytes>
+struct alignas(kBytes) Words {
+    uint32_t w[kBytes / 4];
+};
+template <>
+struct alignas(2) Words<2> {
+    uint16_t w[1];
+};
+
+// two 16-bit values of a word: kept packed, a register holds two of them
+template <class T>
+__device__ __forceinline__ float2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float2 x);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float2 x) {
+    const __half2 h = __float22half2_rn(x);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float2 x) {
+    const __nv_bfloat162 h = __float22bfloat162_rn(x);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// N values of a vector to f32 and back
+template <class T, int N>
+__device__ __forceinline__ void to_floats(const Words<sizeof(T) * N>& v, float (&x)[N]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            x[i] = __uint_as_float(v.w[i]);
+        }
+    } else if constexpr (N == 1) {
+        x[0] = unpack2<T>(v.w[0]).x;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 2; i++) {
+            const float2 y = unpack2<T>(v.w[i]);
+            x[2 * i] = y.x, x[2 * i + 1] = y.y;
+        }
+    }
+}
+template <class T, int N>
+__device__ __forceinline__ Words<sizeof(T) * N> from_floats(const float (&x)[N]) {
+    Words<sizeof(T) * N> v;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            v.w[i] = __float_as_uint(x[i]);
+        }
+    } else if constexpr (N == 1) {
+        v.w[0] = uint16_t(pack2<T>(make_float2(x[0], 0.f)));
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 2; i++) {
+            v.w[i] = pack2<T>(make_float2(x[2 * i], x[2 * i + 1]));
+        }
+    }
+    return v;
+}
 
 // ---- e4m3
 // two f32 to two codes (nearest even, saturating, NaN stays NaN): a in the low byte

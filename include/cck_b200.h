@@ -131,7 +131,7 @@ int cck_rotary(void* stream, const cck_rotation* rotation, int rows, int dim, co
 
 /* Puts the batch's rows of k and v (heads and dim of the cache; bf16, f16 or f32; data and strides multiples of 16 bytes) into the
  * cache, the keys rotated if `rotation` is given. q (may be null; any number of heads) is rotated into q_out (which may be q) by
- * the same launch.
+ * the same call.
  * A page's scale is the smallest power of two that holds the values put into it, at least the one it has if older tokens of the
  * sequence share the page: those are then brought to the new scale. Rounded to nearest even; magnitudes over 448 * 2^40 saturate,
  * what is far below 2^-40 is lost. A token that holds NaN or an infinity in a head's key or value becomes NaN in whole: its key's
