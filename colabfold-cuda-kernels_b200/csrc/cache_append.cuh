@@ -234,10 +234,6 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     }
 }
 
-// Magnitudes of two 16-bit values a word: as signless integers they are in order, infinities and NaN above all others
-__device__ __forceinline__ uint32_t largest_words(uint32_t m, uint32_t a, uint32_t b) {
-    return __vimax3_s16x2(m, a & 0x7FFF7FFFu, b & 0x7FFF7FFFu);
-}
 // The same in registers, for 16-bit values. Thread gt of a group's GT has key items gt + n GT (16 dims of a row: the two vectors that its pairs
 // lie in) and value items (two dims of 16 tokens).
 constexpr int kKeyItems = 2, kValueItems = 1, kPageThreads = 512; // of the widest group

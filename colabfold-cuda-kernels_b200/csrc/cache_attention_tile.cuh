@@ -228,7 +228,7 @@ __device__ __forceinline__ bool next_segment(TileCtl* ctl, Ring<kSegments>& r, S
 template <class T, int D>
 __device__ __forceinline__ void tile_softmax(const AttentionArgs& A, unsigned char* smem, TileCtl* ctl) {
     using S = TileShape<T, D>;
-    const int t = threadIdx.x >> 7, row = threadIdx.x & 127, lane = threadIdx.x & 31;
+    const int t = threadIdx.x >> 7, row = threadIdx.x & 127;
     const uint32_t lanes = uint32_t(row & ~31) << 16, ts = ctl->tmem + lanes + t * 128, to = ctl->tmem + lanes + 256 + t * 128;
     // the scale's sign goes to the queries, so that the largest score of 16 keys is that of the largest product
     const float sign = A.scale_log2 < 0.f ? -1.f : 1.f;
@@ -243,55 +243,48 @@ __device__ __forceinline__ void tile_softmax(const AttentionArgs& A, unsigned ch
             continue;
         }
         const int rt = g.r0 + t * kTileRows, r = rt + row, r1 = g.r0 + g.rows;
-        // Queries in terms, two rows at a time: 16 lanes hold eight dims of a row each; a row that is not there is zero. Scaled to 256 at its
-        // row's largest, a bf16 is an f16 too (down to 2^-32 of that), in which the terms are split off, two at a time.
+        // The row in terms; one that is not there is zero. Scaled to 256 at its largest, a bf16 is an f16 too (down to 2^-32 of that), in which the
+        // terms are split off, two at a time. (Rows dealt out to 16 lanes, with coalesced loads, took 20000 cycles of shuffles and waits.)
         float up = 0.f;
         {
-            const int c = lane & 15, at0 = (row & ~31) + (lane >> 4);
-            unsigned char* to_q = smem + t * S::kTerms * S::kQ + (c >> 1) * 128 + (c & 1) * 8;
-#pragma unroll 1
-            for (int k0 = 0; k0 < 16; k0 += 8) {
-                Vec<T, 8> v[8] = {};
+            uint4 v[D / 8];
+            const T* from = static_cast<const T*>(A.q) + (g.row0 + r / A.group) * A.qr + (g.head * A.group + r % A.group) * A.qh;
 #pragma unroll
-                for (int k = 0; k < 8; k++) { // all loads on their way before the first store
-                    if (const int rr = rt + at0 + 2 * (k0 + k); rr < r1 && 8 * c < D) {
-                        v[k] = *reinterpret_cast<const Vec<T, 8>*>(static_cast<const T*>(A.q) + (g.row0 + rr / A.group) * A.qr + (g.head * A.group + rr % A.group) * A.qh + 8 * c);
-                    }
+            for (int k = 0; k < D / 8; k++) {
+                v[k] = r < r1 ? *reinterpret_cast<const uint4*>(from + 8 * k) : make_uint4(0, 0, 0, 0);
+            }
+            uint32_t most = 0;
+#pragma unroll
+            for (int k = 0; k < D / 8; k++) {
+                most = largest_words(largest_words(most, v[k].x, v[k].y), v[k].z, v[k].w);
+            }
+            const float2 m = unpack2<T>(most);
+            const float top = m.x > m.y || m.x != m.x ? m.x : m.y;
+            const int ex = min(max((__float_as_int(top) >> 23) - 134, -118), 118);
+            const float down = top <= 3.402823466e38f ? sign * exp2_int(-ex) : __int_as_float(0x7fffffff); // not finite: NaN as a whole
+            up = sign * exp2_int(ex);
+            unsigned char* to_q = smem + t * S::kTerms * S::kQ + (row >> 3) * 8 * D + (row & 7) * 16;
+#pragma unroll
+            for (int k = 0; k < D / 16; k++) {
+                __half2 z[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const uint4& w = v[2 * k + e / 4];
+                    const float2 x = unpack2<T>(e % 4 == 0 ? w.x : e % 4 == 1 ? w.y : e % 4 == 2 ? w.z : w.w);
+                    z[e] = __floats2half2_rn(x.x * down, x.y * down);
                 }
 #pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const int at = at0 + 2 * (k0 + k);
-                    float x[8], top = 0.f;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        x[e] = to_f32(v[k].v[e]), top = fmaxf(top, fabsf(x[e]));
-                    }
-#pragma unroll
-                    for (int w = 1; w < 16; w *= 2) {
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-                    }
-                    const int ex = min(max((__float_as_int(top) >> 23) - 134, -118), 118);
-                    const float down = top <= 3.402823466e38f ? sign * exp2_int(-ex) : __int_as_float(0x7fffffff);
-                    const float its = __shfl_sync(0xffffffffu, sign * exp2_int(ex), (lane & 1) * 16);
-                    up = lane >> 1 == k0 + k ? its : up;
-                    __half2 z[4];
+                for (int n = 0; n < S::kTerms; n++) {
+                    uint32_t w[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        z[e] = __floats2half2_rn(x[2 * e] * down, x[2 * e + 1] * down);
+                        w[e] = halves_to_codes(z[2 * e], z[2 * e + 1]);
+                        uint32_t y[2];
+                        unpack_e4m3(w[e], y[0], y[1]);
+                        z[2 * e] = __hsub2(z[2 * e], *reinterpret_cast<const __half2*>(&y[0]));
+                        z[2 * e + 1] = __hsub2(z[2 * e + 1], *reinterpret_cast<const __half2*>(&y[1]));
                     }
-#pragma unroll
-                    for (int m = 0; m < S::kTerms; m++) {
-                        const uint32_t w0 = halves_to_codes(z[0], z[1]), w1 = halves_to_codes(z[2], z[3]);
-                        if (8 * c < D) {
-                            *reinterpret_cast<uint2*>(to_q + m * S::kQ + (at >> 3) * 8 * D + (at & 7) * 16) = make_uint2(w0, w1);
-                        }
-                        uint32_t y[4];
-                        unpack_e4m3(w0, y[0], y[1]), unpack_e4m3(w1, y[2], y[3]);
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            z[e] = __hsub2(z[e], *reinterpret_cast<const __half2*>(&y[e]));
-                        }
-                    }
+                    *reinterpret_cast<uint4*>(to_q + n * S::kQ + k * 128) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

@@ -124,6 +124,11 @@ __device__ __forceinline__ Words<sizeof(T) * N> from_floats(const float (&x)[N])
     return v;
 }
 
+// Magnitudes of two 16-bit values a word: as signless integers they are in order, infinities and NaN above all others
+__device__ __forceinline__ uint32_t largest_words(uint32_t m, uint32_t a, uint32_t b) {
+    return __vimax3_s16x2(m, a & 0x7FFF7FFFu, b & 0x7FFF7FFFu);
+}
+
 // ---- e4m3
 // two f32 to two codes (nearest even, saturating, NaN stays NaN): a in the low byte
 __device__ __forceinline__ uint32_t pack_e4m3(float a, float b) {

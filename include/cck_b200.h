@@ -146,9 +146,9 @@ int cck_cache_append(void* stream, const cck_cache* cache, const cck_batch* batc
  * reads cache head j / (q heads / heads)); q and out are bf16 or f16, both the same, data and strides multiples of 16 bytes.
  * Row i of n of sequence b stands at place len[b]-n+i. causal: it sees places up to its own, else all len[b]; window > 0: of
  * those only the ones later than its place - window. A row that sees nothing gives 0, and -inf in lse. lse (may be null):
- * f32 [rows][q heads], the natural log of the sum of exponentials. Scores, maxima, sums and outputs are accumulated in f32; q is
- * rounded to 11 bits relative to a power of two at the row's largest (bf16 and f16 lose nothing above 2^-14 of it), the
- * probabilities to f16.
+ * f32 [rows][q heads], the natural log of the sum of exponentials. Scores, maxima, sums and outputs are accumulated in f32. q is
+ * exact where it is at least 2^-9 of its row's largest (bf16; f16: 2^-6) and otherwise off by at most 2^-17 of that; the probabilities
+ * are rounded to f16 relative to about the largest. A q that is not finite makes its row NaN.
  * Rows that need a page id outside the cache or past the table's row are NaN. Slots past len[b] may hold anything.
  * ws: cck_cache_attention_workspace_bytes(cache, batch, q_heads) bytes (0 if none is needed, also for arguments that the call
  * refuses), 16-byte aligned, may be uninitialised; its contents mean nothing between calls. Calls that overlap on the GPU, or graphs that may

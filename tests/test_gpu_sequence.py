@@ -6,9 +6,12 @@ Tolerances count roundings. u(t) = finfo(t).eps / 2 is the largest relative erro
             and sine to 2 units in the last place (2^-23), the two products and their sum to 3 * 2^-24.
  append     values are codes times a power of two: equal to the rounding done in 64 bits, bit for bit. Rotated keys: half a step of
             e4m3 (2^-4 |x|, or 2^-10 of the scale below its normal range) plus the rotation's own error.
- attention  E = (D + 8) 2^-23 sum|q k| softmax_scale bounds the error of a score (products in f16 are exact, f32 sums truncate), so a
-            probability is off by 2 E (itself and the sum) + 2^-20 (exponentials, rescaling, the sum); for the matrix product it is
-            rounded to f16, 2^-11 of itself or 2^-25 where it is small, of the largest term; and u(t) |out| for the output.
+ attention  E = (D + 8) 2^-23 sum|q k| softmax_scale bounds the error of a score's sum (products of codes are exact, f32 sums truncate). q,
+            scaled such that its row's largest lies in [128, 256), is split into e4m3 terms, which hold 8 bits of a bf16 (11 of an
+            f16) down to the last term's smallest step of 2^-9, half of which stays open: at most 2^-10 / 128 = 2^-17 of the row's
+            largest a dim, so 2^-17 max|q| sum|k| softmax_scale is added to E. A probability is off by 2 E (itself and the sum) + 2^-20
+            (exponentials, rescaling, the sum); for the matrix product it is rounded to f16, 2^-11 of itself or 2^-25 where it is
+            small, of the largest term; and u(t) |out| for the output.
 """
 import math
 
@@ -416,7 +419,8 @@ def attention_plain(q, k, v, scale, causal, window):
     seen_nan = torch.einsum("nt,ht->nh", seen.double(), (k.isnan().any(-1)).double()) > 0
     out, size_v = mix(v.nan_to_num(0)), mix(v.nan_to_num(0).abs())
     out[seen_nan] = math.nan
-    return out, lse.T, weight.T, size_v, some
+    rest = (q.double().abs().amax(-1).T * k.abs().sum(-1).nan_to_num(0).amax(-1, keepdim=True) * abs(scale)).nan_to_num(0) if size else torch.zeros_like(weight)
+    return out, lse.T, weight.T, rest.T, size_v, some
 
 
 def check_attention(seq, cache, batch, q, dtype, causal=True, window=0, scale=None, out=None, poison=()):
@@ -444,11 +448,11 @@ def check_attention(seq, cache, batch, q, dtype, causal=True, window=0, scale=No
             n = batch.lens[b]
             if n == 0:
                 continue
-        want, want_lse, weight, size_v, some = attention_plain(q[rows], k, v, scale, causal, window)
+        want, want_lse, weight, rest, size_v, some = attention_plain(q[rows], k, v, scale, causal, window)
         got, got_lse = out[rows].double(), lse[rows].double()
         assert torch.equal(got.isnan(), want.isnan().any(-1, keepdim=True).expand_as(got) | want.isnan())
         fine = ~want.isnan()
-        err = (dim + 8) * 2.0**-23 * weight
+        err = (dim + 8) * 2.0**-23 * weight + 2.0**-17 * rest
         rel = 2 * err + 2.0**-20 + 2.0**-11
         vs = cache.vs[batch.lists[b]].double().max()
         bound = half_step(dtype) * want.abs() + rel[..., None] * size_v * 1.01 + batch.lens[b] * 2.0**-25 * 448 * vs
