@@ -12,8 +12,8 @@
 // that waits for nobody hides its copies better. What then counts is the number of instructions, whose fetch a warp pays for
 // anew in every granule; so the codes go to the tensor cores as they lie:
 //   K q^T   mma.m16n8k32 on e4m3. ldmatrix brings four 8 keys x 16 dims pieces at once. q, scaled to 256 at its row's largest, is split into
-//           terms of 4 bits, each the e4m3 rounding of 16 times what the one before left: two terms hold a bf16, three an f16, exactly
-//           down to 2^-13 of the row's largest. Sums of a term are f32 (checked: nothing is cut off in the tensor core).
+//           terms of 4 bits, each the e4m3 rounding of what the one before left: two hold a bf16, three an f16, down to the last one's
+//           smallest step, 2^-17 of the row's largest. Sums are f32 (checked: nothing is cut off in the tensor core).
 //   V^T p   mma.m16n8k16 on f16, to which the codes convert exactly. p needs the range: in terms of e4m3 a key of probability
 //           2^-16 would vanish beside one of 1, and a long tail of such keys can outweigh it.
 // Score rows i and i + 8 of tile u are keys 16 u + 4 (i / 2) + i % 2 and two on, such that transposing a score tile's two 8 x 8 halves
@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DecodeShape<D, NT>::kBlocks
             for (int m = 0; m < kTerms; m++) {
                 q[t][k][m] = pack_e4m3(x.x, x.y, x.z, x.w);
                 const float4 y = codes_to_f32(q[t][k][m]);
-                x = make_float4((x.x - y.x) * 16.f, (x.y - y.y) * 16.f, (x.z - y.z) * 16.f, (x.w - y.w) * 16.f);
+                x = make_float4(x.x - y.x, x.y - y.y, x.z - y.z, x.w - y.w);
             }
         }
 #pragma unroll
@@ -441,37 +441,30 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DecodeShape<D, NT>::kBlocks
             }
             break;
         }
-        float x[kTiles][NT][4];
-        {
-            float z[kTerms][kTiles][NT][4] = {};
+        float x[kTiles][NT][4] = {};
 #pragma unroll
-            for (int k = 0; k < D / 32; k++) {
-#pragma unroll
-                for (int u = 0; u < kTiles; u++) {
-                    uint32_t w[4];
-                    ldmatrix4(w, st + k_at + u * 16 * D + k * 256);
-#pragma unroll
-                    for (int t = 0; t < NT; t++) {
-#pragma unroll
-                        for (int m = 0; m < kTerms; m++) {
-                            mma_e4m3(z[m][u][t], w, q[t][2 * k][m], q[t][2 * k + 1][m]);
-                        }
-                    }
-                }
-            }
+        for (int k = 0; k < D / 32; k++) {
 #pragma unroll
             for (int u = 0; u < kTiles; u++) {
+                uint32_t w[4];
+                ldmatrix4(w, st + k_at + u * 16 * D + k * 256);
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
 #pragma unroll
-                    for (int v = 0; v < 4; v++) {
-                        float y = z[kTerms - 1][u][t][v];
-#pragma unroll
-                        for (int m = kTerms - 2; m >= 0; m--) {
-                            y = fmaf(y, 1.f / 16.f, z[m][u][t][v]);
-                        }
-                        x[u][t][v] = y * (a[u] * qs[t][v & 1]);
+                    for (int m = 0; m < kTerms; m++) {
+                        mma_e4m3(x[u][t], w, q[t][2 * k][m], q[t][2 * k + 1][m]);
                     }
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kTiles; u++) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const float f[2] = {a[u] * qs[t][0], a[u] * qs[t][1]};
+#pragma unroll
+                for (int v = 0; v < 4; v++) {
+                    x[u][t][v] = fmaf(x[u][t][v], f[v & 1], e[u]);
                 }
             }
         }
@@ -497,7 +490,6 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DecodeShape<D, NT>::kBlocks
             for (int u = 0; u < kTiles; u++) {
 #pragma unroll
                 for (int v = 0; v < 4; v++) {
-                    x[u][t][v] += e[u];
                     top[v & 1] = fmaxf(top[v & 1], x[u][t][v]);
                 }
             }
@@ -619,54 +611,126 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DecodeShape<D, NT>::kBlocks
     }
 }
 
-// The shares of a unit together. Blocks x are the shares: the unit that begins in the share and goes on in the next. Its rows are dealt
-// out to the blocks y and to the warps, or, where there are many shares, the shares of a row to the warps.
-constexpr int kMergeWarps = 8;
+// The shares of a unit together. Block x takes the x-th unit that begins in one share and goes on in the next. Its rows are dealt out to the
+// blocks y and to the warps, or, where there are many shares, the shares of a row to the warps.
+constexpr int kMergeWarps = 8, kMostShares = 1024;
 template <class T>
-__global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_constant__ AttentionArgs A) {
+__global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_constant__ AttentionArgs A, int shares) {
     __shared__ float4 so[kMergeWarps][32];
-    __shared__ float2 sm[kMergeWarps];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = A.cache.dim, c0 = blockIdx.x;
+    __shared__ float weights[kMostShares], tops[kMergeWarps], sums[kMergeWarps];
+    __shared__ int before[kMergeWarps], found;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = A.cache.dim;
     wait_for_previous();
-    const Split split = A.splits[c0];
-    if (split.last == c0) {
+    // each thread counts the units that begin in its shares and go on
+    const int each = ceil_div(shares, kMergeWarps * 32), s0 = threadIdx.x * each, s1 = min(shares, s0 + each);
+    int count = 0;
+    for (int c = s0; c < s1; c++) {
+        count += A.splits[c].last != c;
+    }
+    int upto = count;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const int x = __shfl_up_sync(0xffffffffu, upto, o);
+        upto += lane >= o ? x : 0;
+    }
+    if (lane == 31) {
+        before[warp] = upto;
+    }
+    if (threadIdx.x == 0) {
+        found = -1;
+    }
+    __syncthreads();
+    int nth = int(blockIdx.x) - (upto - count);
+    for (int w = 0; w < warp; w++) {
+        nth -= before[w];
+    }
+    if (nth >= 0 && nth < count) {
+        for (int c = s0; c < s1; c++) {
+            if (A.splits[c].last != c && nth-- == 0) {
+                found = c;
+            }
+        }
+    }
+    __syncthreads();
+    const int c0 = found;
+    if (c0 < 0) {
         return;
     }
+    const Split split = A.splits[c0];
     const Tile own = tile_at(A, split.tile);
-    const bool together = split.last - c0 >= 2 * kMergeWarps; // a row by all warps
-    const int stride = together ? gridDim.y : gridDim.y * kMergeWarps;
+    const int n = split.last - c0 + 1;
+    auto slot = [&](int c) { return (2 * int64_t(c0 + c) + (c == 0 ? 1 : 0)) * A.tile_rows; };
+    if (n <= 2 * kMergeWarps) { // a row by a warp
 #pragma unroll 1
-    for (int r = together ? blockIdx.y : blockIdx.y * kMergeWarps + warp; r < own.rows; r += stride) {
-        float top = kNoBase, sum = 0.f;
-        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int r = blockIdx.y * kMergeWarps + warp; r < own.rows; r += gridDim.y * kMergeWarps) {
+            float top = kNoBase, sum = 0.f;
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-        for (int c = together ? c0 + warp : c0; c <= split.last; c += together ? kMergeWarps : 1) {
-            const int64_t at = (2 * int64_t(c) + (c == c0 ? 1 : 0)) * A.tile_rows + r;
-            const float2 ml = *reinterpret_cast<const float2*>(A.part_ml + 2 * at);
-            const float4 z = 4 * lane < D ? *reinterpret_cast<const float4*>(A.part_o + at * D + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
-            const float is = fmaxf(top, ml.x), f = exp2_fast(top - is), w = exp2_fast(ml.x - is);
-            top = is, sum = sum * f + ml.y * w;
-            y.x = y.x * f + z.x * w, y.y = y.y * f + z.y * w, y.z = y.z * f + z.z * w, y.w = y.w * f + z.w * w;
+            for (int c = 0; c < n; c++) {
+                const int64_t at = slot(c) + r;
+                const float2 ml = *reinterpret_cast<const float2*>(A.part_ml + 2 * at);
+                const float4 z = 4 * lane < D ? *reinterpret_cast<const float4*>(A.part_o + at * D + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+                const float is = fmaxf(top, ml.x), f = exp2_fast(top - is), w = exp2_fast(ml.x - is);
+                top = is, sum = sum * f + ml.y * w;
+                y.x = y.x * f + z.x * w, y.y = y.y * f + z.y * w, y.z = y.z * f + z.z * w, y.w = y.w * f + z.w * w;
+            }
+            if (4 * lane < D) {
+                store_out<T>(A, own.s.row0 + (own.r0 + r) / A.group, split.head * A.group + (own.r0 + r) % A.group, 4 * lane, y, top, sum);
+            }
         }
-        if (together) {
-            so[warp][lane] = y;
-            if (lane == 0) {
-                sm[warp] = make_float2(top, sum);
+        return;
+    }
+    // a row by all warps: the weights of all shares first, so that their sums are loaded without waiting for one another
+#pragma unroll 1
+    for (int r = blockIdx.y; r < own.rows; r += gridDim.y) {
+        float top = kNoBase, sum = 0.f;
+        for (int c = threadIdx.x; c < n; c += kMergeWarps * 32) {
+            top = fmaxf(top, A.part_ml[2 * (slot(c) + r)]);
+        }
+#pragma unroll
+        for (int o = 16; o; o /= 2) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        }
+        __syncthreads(); // the last row's weights and shares have been read
+        if (lane == 0) {
+            tops[warp] = top;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kMergeWarps; w++) {
+            top = fmaxf(top, tops[w]);
+        }
+        for (int c = threadIdx.x; c < n; c += kMergeWarps * 32) {
+            const float2 ml = *reinterpret_cast<const float2*>(A.part_ml + 2 * (slot(c) + r));
+            const float w = exp2_fast(ml.x - top);
+            weights[c] = w, sum = fmaf(ml.y, w, sum);
+        }
+#pragma unroll
+        for (int o = 16; o; o /= 2) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        }
+        if (lane == 0) {
+            sums[warp] = sum;
+        }
+        __syncthreads();
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (4 * lane < D) {
+#pragma unroll 8
+            for (int c = warp; c < n; c += kMergeWarps) {
+                const float4 z = *reinterpret_cast<const float4*>(A.part_o + (slot(c) + r) * D + 4 * lane);
+                const float w = weights[c];
+                y.x = fmaf(z.x, w, y.x), y.y = fmaf(z.y, w, y.y), y.z = fmaf(z.z, w, y.z), y.w = fmaf(z.w, w, y.w);
             }
-            __syncthreads();
-            top = kNoBase, sum = 0.f, y = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        so[warp][lane] = y;
+        __syncthreads();
+        if (warp == 0 && 4 * lane < D) {
+            y = make_float4(0.f, 0.f, 0.f, 0.f), sum = 0.f;
+#pragma unroll
             for (int w = 0; w < kMergeWarps; w++) {
-                top = fmaxf(top, sm[w].x);
-            }
-            for (int w = 0; w < kMergeWarps; w++) {
-                const float f = exp2_fast(sm[w].x - top);
                 const float4 z = so[w][lane];
-                sum = fmaf(sm[w].y, f, sum);
-                y.x = fmaf(z.x, f, y.x), y.y = fmaf(z.y, f, y.y), y.z = fmaf(z.z, f, y.z), y.w = fmaf(z.w, f, y.w);
+                y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w, sum += sums[w];
             }
-            __syncthreads();
-        }
-        if (4 * lane < D && (!together || warp == 0)) {
             store_out<T>(A, own.s.row0 + (own.r0 + r) / A.group, split.head * A.group + (own.r0 + r) % A.group, 4 * lane, y, top, sum);
         }
     }

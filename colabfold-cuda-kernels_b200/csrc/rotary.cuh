@@ -119,7 +119,7 @@ __device__ __forceinline__ void rotary_warp(const cck_rotation& R, const RotaryS
             const T* x = static_cast<const T*>(s.x) + row * s.xr + (h_begin + first) * s.xh + i0;
             T* y = static_cast<T*>(s.y) + row * s.yr + (h_begin + first) * s.yh + i0;
             const int over = i1 - i0, mine = item < s.items ? heads : 0;
-            constexpr int kAhead = 4; // heads whose loads are on their way together
+            constexpr int kAhead = 2; // heads whose loads are on their way together
             Vt a[kAhead], b[kAhead];
             auto load = [&](int left) {
 #pragma unroll
@@ -186,7 +186,7 @@ __device__ __forceinline__ void rotary_warp(const cck_rotation& R, const RotaryS
 
 constexpr int kRotaryThreads = 256;
 template <class T, int V, bool kAdjacent>
-__global__ void __launch_bounds__(kRotaryThreads, 3) rotary_kernel(const __grid_constant__ cck_rotation R, const __grid_constant__ RotaryShape s) {
+__global__ void __launch_bounds__(kRotaryThreads, 4) rotary_kernel(const __grid_constant__ cck_rotation R, const __grid_constant__ RotaryShape s) {
     extern __shared__ __align__(128) unsigned char smem[];
     const int warp = threadIdx.x >> 5, warps = kRotaryThreads / 32;
     rotary_warp<T, V, kAdjacent>(R, s, reinterpret_cast<float2*>(smem) + warp * (R.dims / 2), int64_t(blockIdx.x) * warps + warp, int64_t(gridDim.x) * warps);

@@ -158,7 +158,7 @@ int rotary_vector(const cck_rotation& r, int dim, const cck_rows& x, const cck_r
     }
     return 1;
 }
-// How rows and heads are dealt out to warps, of which a multiprocessor holds 24: whole rows, or parts of a row's heads where rows are few, down to
+// How rows and heads are dealt out to warps, of which a multiprocessor holds 32: whole rows, or parts of a row's heads where rows are few, down to
 // one head a lane
 RotaryShape rotary_shape(const cck_rotation& r, int rows, int dim, const cck_rows& x, const cck_rows& y, bool inverse, int v, int sms) {
     RotaryShape s{};
@@ -169,14 +169,14 @@ RotaryShape rotary_shape(const cck_rotation& r, int rows, int dim, const cck_row
     if (s.items == 0) { // in place, and nothing turns
         return s;
     }
-    const int warps = 24 * sms, at_once = s.items < 32 ? 32 / s.items : 1, most = ceil_div(x.heads, at_once);
+    const int warps = 32 * sms, at_once = s.items < 32 ? 32 / s.items : 1, most = ceil_div(x.heads, at_once);
     int splits = 1;
     if (rows < warps) {
         splits = ceil_div(warps, rows) < most ? ceil_div(warps, rows) : most;
-    } else { // a few rounds of rows: parts of a row where they fill the last round by a tenth better
+    } else { // a few rounds of rows: parts of a row where they save a fifth of the rounds
         auto time = [&](int n) { return double((int64_t(rows) * n + warps - 1) / warps) / n; };
         for (int n = 2; n <= 4 && n <= most; n++) {
-            splits = time(n) < 0.9 * time(splits) ? n : splits;
+            splits = time(n) < 0.8 * time(splits) ? n : splits;
         }
     }
     s.part_heads = ceil_div(x.heads, splits);
@@ -186,7 +186,7 @@ RotaryShape rotary_shape(const cck_rotation& r, int rows, int dim, const cck_row
 }
 // blocks of `threads` that work through it: as many as fit the multiprocessors at once
 int64_t rotary_blocks(const RotaryShape& s, int threads, int sms) {
-    const int64_t all = (s.units + threads / 32 - 1) / (threads / 32), most = int64_t(24) * sms / (threads / 32);
+    const int64_t all = (s.units + threads / 32 - 1) / (threads / 32), most = int64_t(32) * sms / (threads / 32);
     return all < most ? all : most;
 }
 size_t rotary_smem(const cck_rotation& r, int threads) {
@@ -264,7 +264,7 @@ struct Plan {
     int row_tiles;          // of a sequence
     int64_t blocks;
     bool shares;
-    int merge_y;
+    unsigned merge_x, merge_y; // units that can be split; blocks for the rows of one
     size_t part_bytes, ml_bytes, bytes; // of the workspace
 };
 Plan make_plan(const cck_cache& c, const cck_batch& b, int q_heads, int sms) {
@@ -276,11 +276,12 @@ Plan make_plan(const cck_cache& c, const cck_batch& b, int q_heads, int sms) {
     const int64_t units = int64_t(b.sequences) * c.heads * p.row_tiles, slots = (p.nt == 0 ? 1 : p.nt == 1 ? 3 : 2) * sms;
     const int64_t granules = int64_t(b.max_len) / p.granule + 2;
     const int least = p.nt ? 2 * kDecodeWarps : 2; // granules of a share
-    p.shares = granules > 2 * least && units < 8 * slots;
+    p.shares = granules > (p.nt ? 4 : 2) * least && units < 8 * slots;
     const int64_t most = (units * granules + least - 1) / least;
     p.blocks = !p.shares ? units : most < slots ? most : slots;
+    p.blocks = p.shares && p.blocks > kMostShares ? kMostShares : p.blocks;
     if (p.shares) {
-        p.merge_y = p.nt == 0 ? 16 : units < 64 ? p.tile_rows : 1;
+        p.merge_x = unsigned(units < p.blocks ? units : p.blocks), p.merge_y = p.nt == 0 ? 16 : p.merge_x < 64 ? p.tile_rows : 1;
         p.part_bytes = size_t(2 * p.blocks) * p.tile_rows * c.dim * 4;
         p.ml_bytes = size_t(2 * p.blocks) * p.tile_rows * 8;
         p.bytes = p.part_bytes + p.ml_bytes + size_t(p.blocks) * sizeof(Split);
@@ -323,8 +324,8 @@ cudaError_t launch_attention(cudaStream_t st, const AttentionArgs& a, const Plan
     cudaLaunchAttribute dependent;
     dependent.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     dependent.val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(unsigned(p.blocks), unsigned(p.merge_y)), cfg.blockDim = dim3(kMergeWarps * 32), cfg.stream = st, cfg.attrs = &dependent, cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, merge_kernel<T>, a);
+    cfg.gridDim = dim3(p.merge_x, p.merge_y), cfg.blockDim = dim3(kMergeWarps * 32), cfg.stream = st, cfg.attrs = &dependent, cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, merge_kernel<T>, a, int(p.blocks));
 }
 
 } // namespace
