@@ -51,6 +51,10 @@ __device__ __forceinline__ PageRows page_rows(const AppendArgs& A, int unit, boo
     r.page = none ? -1 : r.page;
     return r;
 }
+// the queries' units: rows behind the last sequence are left as they are
+__device__ __forceinline__ int64_t query_units(const AppendArgs& A) {
+    return int64_t(min(max(A.batch.first[A.batch.sequences], 0), A.batch.rows)) * A.q.splits;
+}
 // four codes times f (a power of two below 1), rounded again
 __device__ __forceinline__ uint32_t lowered(uint32_t w, float f) {
     uint32_t lo, hi;
@@ -100,9 +104,9 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
         const int64_t unit = int64_t(blockIdx.x - A.kv_blocks) * warps + (tid >> 5), step = int64_t(gridDim.x - A.kv_blocks) * warps;
         float2* table = reinterpret_cast<float2*>(smem) + (tid >> 5) * (A.rotation.dims / 2);
         if (A.rotation.adjacent) {
-            rotary_warp<T, VQ, true>(A.rotation, A.q, table, unit, step);
+            rotary_warp<T, VQ, true>(A.rotation, A.q, table, unit, step, query_units(A));
         } else {
-            rotary_warp<T, VQ, false>(A.rotation, A.q, table, unit, step);
+            rotary_warp<T, VQ, false>(A.rotation, A.q, table, unit, step, query_units(A));
         }
         return;
     }
@@ -158,8 +162,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     for (int i = tid; i < rows * D; i += kAppendThreads) {
         const int u = i / D, d = i % D;
         if (!bad[u]) {
-            const float x = fabsf(fk[u * kp + d]);
-            top_k = is_finite(x) ? fmaxf(top_k, x) : top_k;
+            top_k = fmaxf(top_k, fabsf(fk[u * kp + d]));
             top_v = fmaxf(top_v, fabsf(to_f32(fv[u * vp + d])));
         }
     }
@@ -248,7 +251,8 @@ __global__ void __launch_bounds__(kPageThreads, 1) append_pages_kernel(const __g
     float2* table = reinterpret_cast<float2*>(smem);
     if (int(blockIdx.x) >= A.kv_blocks) {
         const int warps = nt / 32;
-        rotary_warp<T, 8, kAdjacent>(R, A.q, table + (tid >> 5) * (R.dims / 2), int64_t(blockIdx.x - A.kv_blocks) * warps + (tid >> 5), int64_t(gridDim.x - A.kv_blocks) * warps);
+        rotary_warp<T, 8, kAdjacent>(R, A.q, table + (tid >> 5) * (R.dims / 2), int64_t(blockIdx.x - A.kv_blocks) * warps + (tid >> 5), int64_t(gridDim.x - A.kv_blocks) * warps,
+                                    query_units(A));
         return;
     }
     const int P = C.page_tokens, H = C.heads, part = blockIdx.x % A.head_splits;
@@ -367,12 +371,9 @@ __global__ void __launch_bounds__(kPageThreads, 1) append_pages_kernel(const __g
             __syncthreads();
 #pragma unroll
             for (int n = 0; n < kKeyItems; n++) {
-                bool ok = true;
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    ok = ok && is_finite(x[n][e]);
-                }
-                if (!ok) {
+                const float2 m = unpack2<T>(largest_words(largest_words(largest_words(0, ka[n].x, ka[n].y), ka[n].z, ka[n].w), // as they came
+                                                          largest_words(largest_words(0, kb[n].x, kb[n].y), kb[n].z, kb[n].w), 0));
+                if (!is_finite(m.x) || !is_finite(m.y)) {
                     const int u = (gt + n * GT) / strips;
                     atomicOr(&bad[group][u / 32], 1u << (u % 32));
                 }

@@ -44,6 +44,7 @@ struct AttentionArgs {
     float* lse;
     float scale_log2; // softmax_scale * log2(e)
     int q_heads, group, causal, window;
+    int reach; // tokens that a row of the table has pages for
     int granule_shift, page_shift; // keys of a step and tokens of a page are powers of two
     int unit_cost;
     int tile_rows, row_tiles; // a sequence's rows times heads of a group, cut into tiles: `tiles` are those of all sequences, row_tiles each
@@ -52,11 +53,11 @@ struct AttentionArgs {
     struct Split* splits;
 };
 
-// keys [lo, hi) that row i (a place in its sequence) sees
+// keys [lo, hi) that a row at `place` of its sequence sees. Those past the table's reach are not there and make the row NaN: the first of them does
 __device__ __forceinline__ int2 seen_by(const AttentionArgs& A, int place, int len) {
     const int hi = A.causal ? min(len, place + 1) : len;
-    const int lo = A.window > 0 ? max(0, place - A.window + 1) : 0;
-    return make_int2(lo, max(hi, lo));
+    const int lo = A.window > 0 && place >= A.window ? place - A.window + 1 : 0;
+    return make_int2(lo, max(lo, min(hi, max(lo, A.reach) + 1)));
 }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {

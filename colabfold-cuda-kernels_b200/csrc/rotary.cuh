@@ -87,7 +87,7 @@ struct RotaryShape {
     void* y;
 };
 template <class T, int V, bool kAdjacent>
-__device__ __forceinline__ void rotary_warp(const cck_rotation& R, const RotaryShape& s, float2* table, int64_t unit, int64_t step) {
+__device__ __forceinline__ void rotary_warp(const cck_rotation& R, const RotaryShape& s, float2* table, int64_t unit, int64_t step, int64_t units) {
     using Vt = Words<V * sizeof(T)>;
     const int lane = threadIdx.x & 31, pairs = R.dims / 2;
     // the frequencies of this lane's first pairs, and their axes, stay
@@ -103,7 +103,7 @@ __device__ __forceinline__ void rotary_warp(const cck_rotation& R, const RotaryS
     const int stride = s.items < 32 ? 32 / s.items : 1, first = s.items < 32 ? lane / s.items : 0; // heads at once; this lane's
     const int64_t xs = stride * s.xh, ys = stride * s.yh;
 #pragma unroll 1
-    for (; unit < s.units; unit += step) {
+    for (; unit < units; unit += step) {
         const int64_t row = s.splits == 1 ? unit : unit / s.splits;
         const int h_begin = s.splits == 1 ? 0 : int(unit - row * s.splits) * s.part_heads;
         const int heads = first < stride ? max(0, ceil_div(min(s.part_heads, s.heads - h_begin) - first, stride)) : 0; // of this lane
@@ -189,7 +189,7 @@ template <class T, int V, bool kAdjacent>
 __global__ void __launch_bounds__(kRotaryThreads, 4) rotary_kernel(const __grid_constant__ cck_rotation R, const __grid_constant__ RotaryShape s) {
     extern __shared__ __align__(128) unsigned char smem[];
     const int warp = threadIdx.x >> 5, warps = kRotaryThreads / 32;
-    rotary_warp<T, V, kAdjacent>(R, s, reinterpret_cast<float2*>(smem) + warp * (R.dims / 2), int64_t(blockIdx.x) * warps + warp, int64_t(gridDim.x) * warps);
+    rotary_warp<T, V, kAdjacent>(R, s, reinterpret_cast<float2*>(smem) + warp * (R.dims / 2), int64_t(blockIdx.x) * warps + warp, int64_t(gridDim.x) * warps, s.units);
 }
 
 } // namespace seq

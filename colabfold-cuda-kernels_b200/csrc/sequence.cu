@@ -2,6 +2,7 @@
 // Declarations: include/cck_b200.h.
 #include <atomic>
 #include <cstdio>
+#include <initializer_list>
 #include <type_traits>
 
 #include "cache_append.cuh"
@@ -24,8 +25,8 @@ int launched(const char* op, cudaError_t err) {
     return err == cudaSuccess ? CCK_OK : refuse(CCK_E_LAUNCH, op, cudaGetErrorString(err));
 }
 
-// the current device's multiprocessors; `data` has to be its memory
-int device_of(const char* op, const void* data, int& sms) {
+// the current device's multiprocessors; what `data` points to (null: nothing) has to be memory that it can read
+int device_of(const char* op, std::initializer_list<const void*> data, int& sms) {
     static std::atomic<int> known[kMaxDevices];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) {
@@ -42,13 +43,15 @@ int device_of(const char* op, const void* data, int& sms) {
         }
         known[dev].store(sms = count, std::memory_order_relaxed);
     }
-    cudaPointerAttributes at;
-    if (cudaPointerGetAttributes(&at, data) != cudaSuccess || at.type == cudaMemoryTypeUnregistered) {
-        cudaGetLastError();
-        return refuse(CCK_E_DEVICE, op, "a tensor is not in device memory");
-    }
-    if (at.type == cudaMemoryTypeDevice && at.device != dev) {
-        return refuse(CCK_E_DEVICE, op, "a tensor is on another device than the current one");
+    for (const void* p : data) {
+        cudaPointerAttributes at;
+        if (p && (cudaPointerGetAttributes(&at, p) != cudaSuccess || at.type == cudaMemoryTypeUnregistered)) {
+            cudaGetLastError();
+            return refuse(CCK_E_DEVICE, op, "a tensor is not in device memory");
+        }
+        if (p && at.type == cudaMemoryTypeDevice && at.device != dev) {
+            return refuse(CCK_E_DEVICE, op, "a tensor is on another device than the current one");
+        }
     }
     return CCK_OK;
 }
@@ -59,28 +62,28 @@ int size_of(int dtype) {
 bool aligned(const void* p, size_t n) {
     return reinterpret_cast<uintptr_t>(p) % n == 0;
 }
-// what is wrong with a tensor: null, or the text of the refusal; `bytes`: what data and strides are multiples of
-int check_rows(const char* op, const cck_rows* x, const char* name, int bytes, bool f32) {
+// a tensor of `rows` rows; `bytes`: what data and strides are multiples of. One without rows may have no memory either
+int check_rows(const char* op, const cck_rows* x, const char* name, int rows, int bytes, bool f32) {
     char text[128];
     auto say = [&](const char* what) {
         snprintf(text, sizeof text, "%s %s", name, what);
         return text;
     };
-    if (!x || !x->data) {
+    if (!x || (!x->data && rows)) {
         return refuse(CCK_E_SHAPE, op, say("is null"));
     }
     if (x->dtype != CCK_BF16 && x->dtype != CCK_F16 && !(f32 && x->dtype == CCK_F32)) {
         return refuse(CCK_E_FLAGS, op, say("has a type that is not built"));
     }
-    if (x->heads < 1 || x->row_stride < 0 || x->head_stride < 0) {
-        return refuse(CCK_E_SHAPE, op, say("has no heads, or a negative stride"));
+    if (x->heads < 1 || x->heads > kMostHeads || x->row_stride < 0 || x->head_stride < 0) {
+        return refuse(CCK_E_SHAPE, op, say("has no heads, more than 65536, or a negative stride"));
     }
     if (!aligned(x->data, bytes ? bytes : size_of(x->dtype)) || (bytes && (x->row_stride * size_of(x->dtype) % bytes || x->head_stride * size_of(x->dtype) % bytes))) {
         return refuse(CCK_E_SHAPE, op, say("is not aligned"));
     }
     return CCK_OK;
 }
-int check_rotation(const char* op, const cck_rotation* r, int dim) {
+int check_rotation(const char* op, const cck_rotation* r, int rows, int dim) {
     if (r->dims < 0 || r->dims % 2 || r->dims > dim || r->axes < 1 || r->axes > 4) {
         return refuse(CCK_E_SHAPE, op, "rotation: dims is even and at most a head's, axes 1 to 4");
     }
@@ -94,7 +97,7 @@ int check_rotation(const char* op, const cck_rotation* r, int dim) {
     if (pairs != r->dims / 2) {
         return refuse(CCK_E_SHAPE, op, "rotation: the sections do not add up to dims / 2");
     }
-    if (r->dims && (!r->freq || !r->pos || !aligned(r->freq, 4) || !aligned(r->pos, 4))) {
+    if (r->dims && (!r->freq || (!r->pos && rows) || !aligned(r->freq, 4) || !aligned(r->pos, 4))) {
         return refuse(CCK_E_SHAPE, op, "rotation: freq or pos is null or not aligned");
     }
     return CCK_OK;
@@ -103,8 +106,8 @@ int check_cache(const char* op, const cck_cache* c) {
     if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) {
         return refuse(CCK_E_SHAPE, op, "the cache or a part of it is null");
     }
-    if (c->pages < 1 || c->heads < 1) {
-        return refuse(CCK_E_SHAPE, op, "the cache has no pages or no heads");
+    if (c->pages < 1 || c->heads < 1 || c->heads > kMostHeads) {
+        return refuse(CCK_E_SHAPE, op, "the cache has no pages, no heads or more than 65536");
     }
     if (c->page_tokens != 16 && c->page_tokens != 32 && c->page_tokens != 64 && c->page_tokens != 128) {
         return refuse(CCK_E_SHAPE, op, "a page holds 16, 32, 64 or 128 tokens");
@@ -118,11 +121,14 @@ int check_cache(const char* op, const cck_cache* c) {
     return CCK_OK;
 }
 int check_batch(const char* op, const cck_batch* b) {
-    if (!b || !b->first || !b->len || !b->table || !aligned(b->first, 4) || !aligned(b->len, 4) || !aligned(b->table, 4)) {
+    if (!b || !b->first || (b->sequences && (!b->len || !b->table)) || !aligned(b->first, 4) || !aligned(b->len, 4) || !aligned(b->table, 4)) {
         return refuse(CCK_E_SHAPE, op, "the batch or an array of it is null or not aligned");
     }
     if (b->sequences < 0 || b->rows < 0 || b->max_new < 0 || b->max_len < 0 || b->table_pages < 1 || b->table_stride < 0) {
         return refuse(CCK_E_SHAPE, op, "a size of the batch is negative, or its table has no pages");
+    }
+    if (b->max_len > kMostTokens) {
+        return refuse(CCK_E_SHAPE, op, "a sequence has at most 2^30 tokens");
     }
     return CCK_OK;
 }
@@ -269,11 +275,16 @@ struct Plan {
 };
 Plan make_plan(const cck_cache& c, const cck_batch& b, int q_heads, int sms) {
     Plan p{};
-    const int64_t rows = int64_t(b.max_new) * (q_heads / c.heads);
+    const int64_t rows = int64_t(b.max_new < b.rows ? b.max_new : b.rows) * (q_heads / c.heads);
     p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 0;
     p.granule = p.nt ? granule_of(c.dim) : kTileKeys, p.tile_rows = p.nt ? 8 * p.nt : kUnitRows;
-    p.row_tiles = int((rows + p.tile_rows - 1) / p.tile_rows);
-    const int64_t units = int64_t(b.sequences) * c.heads * p.row_tiles, slots = (p.nt == 0 ? 1 : p.nt == 1 ? 3 : 2) * sms;
+    const int64_t row_tiles = (rows + p.tile_rows - 1) / p.tile_rows, tiles = b.sequences * row_tiles; // below 2^31 * 2^43 / 2^3
+    if (rows > kMostTokens || tiles * c.heads > 0x7fffffff) {
+        p.blocks = int64_t(1) << 32; // refused
+        return p;
+    }
+    p.row_tiles = int(row_tiles);
+    const int64_t units = tiles * c.heads, slots = (p.nt == 0 ? 1 : p.nt == 1 ? 3 : 2) * sms;
     const int64_t granules = int64_t(b.max_len) / p.granule + 2;
     const int least = p.nt ? 2 * kDecodeWarps : 2; // granules of a share
     p.shares = granules > (p.nt ? 4 : 2) * least && units < 8 * slots;
@@ -338,11 +349,11 @@ int cck_rotary(void* stream, const cck_rotation* rotation, int rows, int dim, co
         return refuse(CCK_E_SHAPE, op, "rotation is null, rows is negative or dim is not 1 to 1024");
     }
     int e;
-    if ((e = check_rotation(op, rotation, dim)) || (e = check_rows(op, x, "x", 0, true)) || (e = check_rows(op, y, "y", 0, true)) || (e = check_pair(op, x, y, rows, dim))) {
+    if ((e = check_rotation(op, rotation, rows, dim)) || (e = check_rows(op, x, "x", rows, 0, true)) || (e = check_rows(op, y, "y", rows, 0, true)) || (e = check_pair(op, x, y, rows, dim))) {
         return e;
     }
     int sms = 0;
-    if ((e = device_of(op, x->data, sms)) || (e = device_of(op, y->data, sms))) {
+    if ((e = device_of(op, {x->data, y->data, rotation->dims ? rotation->freq : nullptr, rotation->dims ? rotation->pos : nullptr}, sms))) {
         return e;
     }
     if (rows == 0) {
@@ -366,20 +377,22 @@ int cck_cache_append(void* stream, const cck_cache* cache, const cck_batch* batc
                      const cck_rows* q_out, int32_t* status) {
     const char* op = "cck_cache_append";
     int e;
-    if ((e = check_cache(op, cache)) || (e = check_batch(op, batch)) || (e = check_rows(op, k, "k", 16, true)) || (e = check_rows(op, v, "v", 16, true))) {
+    if ((e = check_cache(op, cache)) || (e = check_batch(op, batch)) || (e = check_rows(op, k, "k", batch->rows, 16, true)) ||
+        (e = check_rows(op, v, "v", batch->rows, 16, true))) {
         return e;
     }
     if (k->dtype != v->dtype || k->heads != cache->heads || v->heads != cache->heads) {
         return refuse(CCK_E_SHAPE, op, "k and v have the cache's heads and one type");
     }
-    if (rotation && (e = check_rotation(op, rotation, cache->dim))) {
+    if (rotation && (e = check_rotation(op, rotation, batch->rows, cache->dim))) {
         return e;
     }
     if (q) {
         if (!rotation) {
             return refuse(CCK_E_SHAPE, op, "queries are rotated, but there is no rotation");
         }
-        if ((e = check_rows(op, q, "q", 0, true)) || (e = check_rows(op, q_out, "q_out", 0, true)) || (e = check_pair(op, q, q_out, batch->rows, cache->dim))) {
+        if ((e = check_rows(op, q, "q", batch->rows, 0, true)) || (e = check_rows(op, q_out, "q_out", batch->rows, 0, true)) ||
+            (e = check_pair(op, q, q_out, batch->rows, cache->dim))) {
             return e;
         }
         if (q->dtype != k->dtype) {
@@ -390,7 +403,10 @@ int cck_cache_append(void* stream, const cck_cache* cache, const cck_batch* batc
         return refuse(CCK_E_SHAPE, op, "status is not aligned");
     }
     int sms = 0;
-    if ((e = device_of(op, cache->k, sms)) || (e = device_of(op, k->data, sms))) {
+    const bool turns = rotation && rotation->dims;
+    if ((e = device_of(op, {cache->k, cache->v, cache->k_scale, cache->v_scale, batch->first, batch->len, batch->table, k->data, v->data, turns ? rotation->freq : nullptr,
+                            turns ? rotation->pos : nullptr, q ? q->data : nullptr, q ? q_out->data : nullptr, status},
+                       sms))) {
         return e;
     }
     AppendArgs a{};
@@ -399,8 +415,10 @@ int cck_cache_append(void* stream, const cck_cache* cache, const cck_batch* batc
     if (rotation) {
         a.rotation = *rotation;
     }
-    const int P = cache->page_tokens, D = cache->dim, most = batch->max_new < P ? batch->max_new : P; // new rows of a page
-    a.blocks_per_seq = batch->max_new ? (batch->max_new + P - 2) / P + 1 : 0;
+    const int max_new = batch->max_new < batch->rows ? batch->max_new : batch->rows;
+    const int P = cache->page_tokens, D = cache->dim, most = max_new < P ? max_new : P; // new rows of a page
+    a.batch.max_new = max_new;
+    a.blocks_per_seq = max_new ? int((int64_t(max_new) + P - 2) / P + 1) : 0;
     int64_t more = 0;
     int vec = 0;
     size_t smem = 0;
@@ -409,6 +427,9 @@ int cck_cache_append(void* stream, const cck_cache* cache, const cck_batch* batc
         a.q = rotary_shape(*rotation, batch->rows, D, *q, *q_out, false, vec, sms);
     }
     const int64_t units = int64_t(batch->sequences) * a.blocks_per_seq;
+    if (units > 0x7fffffff) {
+        return refuse(CCK_E_SHAPE, op, "too many rows for one launch");
+    }
     // 16-bit values whose rotated part is whole vectors go through registers
     const bool pages = k->dtype != CCK_F32 && a.rotation.dims % 16 == 0 && (vec == 0 || vec == 8);
     int64_t kv;
@@ -457,7 +478,7 @@ int cck_cache_append(void* stream, const cck_cache* cache, const cck_batch* batc
 size_t cck_cache_attention_workspace_bytes(const cck_cache* cache, const cck_batch* batch, int q_heads) {
     const char* op = "cck_cache_attention_workspace_bytes";
     int sms = 0;
-    if (check_cache(op, cache) || check_batch(op, batch) || q_heads < 1 || q_heads % cache->heads || device_of(op, cache->k, sms)) {
+    if (check_cache(op, cache) || check_batch(op, batch) || q_heads < 1 || q_heads % cache->heads || device_of(op, {}, sms)) {
         return 0;
     }
     return make_plan(*cache, *batch, q_heads, sms).bytes;
@@ -467,7 +488,8 @@ int cck_cache_attention(void* stream, const cck_cache* cache, const cck_batch* b
                         int window, void* ws, size_t ws_bytes) {
     const char* op = "cck_cache_attention";
     int e;
-    if ((e = check_cache(op, cache)) || (e = check_batch(op, batch)) || (e = check_rows(op, q, "q", 16, false)) || (e = check_rows(op, out, "out", 16, false)) ||
+    if ((e = check_cache(op, cache)) || (e = check_batch(op, batch)) || (e = check_rows(op, q, "q", batch->rows, 16, false)) ||
+        (e = check_rows(op, out, "out", batch->rows, 16, false)) ||
         (e = check_pair(op, q, out, batch->rows, cache->dim))) {
         return e;
     }
@@ -481,24 +503,29 @@ int cck_cache_attention(void* stream, const cck_cache* cache, const cck_batch* b
         return refuse(CCK_E_SHAPE, op, "lse is not aligned");
     }
     int sms = 0;
-    if ((e = device_of(op, cache->k, sms)) || (e = device_of(op, q->data, sms)) || (e = device_of(op, out->data, sms))) {
+    if ((e = device_of(op, {cache->k, cache->v, cache->k_scale, cache->v_scale, batch->first, batch->len, batch->table, q->data, out->data, lse}, sms))) {
         return e;
     }
     if (batch->sequences == 0 || batch->rows == 0 || batch->max_new == 0) {
         return CCK_OK;
     }
     const Plan p = make_plan(*cache, *batch, q->heads, sms);
+    if (p.blocks > 0x7fffffff) {
+        return refuse(CCK_E_SHAPE, op, "too many rows for one launch");
+    }
     if (ws_bytes < p.bytes || (p.bytes && (!ws || !aligned(ws, 16)))) {
         return refuse(CCK_E_WORKSPACE, op, "the workspace is too small, null or not aligned");
     }
-    if (p.blocks > 0x7fffffff) {
-        return refuse(CCK_E_SHAPE, op, "too many rows for one launch");
+    if (p.bytes && (e = device_of(op, {ws}, sms))) {
+        return e;
     }
     AttentionArgs a{};
     a.cache = *cache, a.batch = *batch, a.q = q->data, a.out = out->data, a.lse = lse;
     a.qr = q->row_stride, a.qh = q->head_stride, a.or_ = out->row_stride, a.oh = out->head_stride;
     a.scale_log2 = softmax_scale * 1.4426950408889634f;
     a.q_heads = q->heads, a.group = q->heads / cache->heads, a.causal = causal != 0, a.window = window;
+    const int64_t reach = int64_t(batch->table_pages) * cache->page_tokens;
+    a.reach = int(reach < kMostTokens ? reach : kMostTokens);
     a.granule_shift = __builtin_ctz(p.granule), a.unit_cost = p.nt ? 8 : 3, a.page_shift = __builtin_ctz(cache->page_tokens);
     a.tile_rows = p.tile_rows, a.row_tiles = p.row_tiles;
     if (p.shares) {

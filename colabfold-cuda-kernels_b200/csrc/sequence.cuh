@@ -14,6 +14,8 @@ namespace cck {
 namespace seq {
 
 constexpr int kMinExp = -40, kMaxExp = 40; // exponents of a cache's scales
+constexpr int kMostTokens = 1 << 30;       // of a sequence
+constexpr int kMostHeads = 1 << 16;
 
 __host__ __device__ constexpr int ceil_div(int a, int b) {
     return (a + b - 1) / b;
@@ -151,7 +153,7 @@ __device__ __forceinline__ int scale_exponent(float top) {
         return kMinExp;
     }
     int x;
-    const float m = frexpf(top, &x);
+    const float m = frexpf(fminf(top, 3.402823466e38f), &x); // a rotation can bring finite values over the largest
     return min(max(x - 9 + (m > 0.875f ? 1 : 0), kMinExp), kMaxExp);
 }
 __device__ __forceinline__ float exp2_int(int e) { // |e| <= 126
@@ -176,9 +178,9 @@ struct Sequence {
 __device__ __forceinline__ Sequence sequence_of(const cck_batch& b, int i) {
     Sequence s;
     const int first = b.first[i], all = b.first[i + 1] - first;
-    s.row0 = first, s.len = max(b.len[i], 0), s.place0 = s.len - all;
+    s.row0 = first, s.len = min(max(b.len[i], 0), kMostTokens), s.place0 = s.len - all;
     s.rows = first < 0 || first > b.rows ? 0 : max(0, min(all, min(b.max_new, b.rows - first)));
-    s.cut = s.rows != all || s.place0 < 0;
+    s.cut = s.rows != all || s.place0 < 0 || s.len != b.len[i];
     return s;
 }
 

@@ -75,7 +75,7 @@ size_t cck_static_workspace_bytes(void);
  * caller's, one or two kernels enqueued on `stream` (a stream of the current device), no allocation, no synchronisation, an
  * error code and cck_last_error(); every call can be captured into a CUDA graph. All descriptors are read before a call
  * returns; what their pointers point to (cck_rows::data, freq, pos, first, len, table, ...) is device memory that the kernels
- * read. Arguments that cannot be right are refused before anything is enqueued: CCK_E_SHAPE (null pointers, sizes, strides,
+ * read; it may be null where there are no rows or no sequences. Heads are at most 65536. Arguments that cannot be right are refused before anything is enqueued: CCK_E_SHAPE (null pointers, sizes, strides,
  * alignment), CCK_E_FLAGS (a type that is not built), CCK_E_WORKSPACE, CCK_E_DEVICE (memory of another device, or not device
  * memory). */
 enum { CCK_BF16 = 0, CCK_F16 = 1, CCK_F32 = 2 };
@@ -112,7 +112,7 @@ typedef struct cck_cache {
 } cck_cache;
 
 /* The sequences of a call. Rows first[b] .. first[b+1]-1 are sequence b's newest first[b+1]-first[b] tokens (none is fine), len[b]
- * is its length with them: both calls of a step take the same batch. Token t of it lies in page table[b * table_stride + t /
+ * is its length with them, at most 2^30: both calls of a step take the same batch. Token t of it lies in page table[b * table_stride + t /
  * page_tokens], slot t % page_tokens. first is not decreasing, from 0 up. Rows from first[sequences] on belong to nobody and are
  * neither read nor written. */
 typedef struct cck_batch {

@@ -395,6 +395,58 @@ def test_append_leaves_out_what_has_no_place(seq, rng, what):
         assert ((got - v[21:23].double()).abs() <= 2.0**-4 * v[21:23].double().abs() + 2.0**-10 * cache.vs.double().max()).all()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("other", [1.0, math.nan])
+def test_append_rotation_past_the_largest(seq, rng, dtype, other):
+    """A pair whose rotation is over the largest float saturates like every other magnitude, whatever other tokens hold."""
+    batch = Batch(seq, [2], [2], 16, rng)
+    cache = Cache(seq, batch.pages, 16, 1, 32, fill=0)
+    k = torch.full((2, 1, 32), 3e38, device="cuda").to(T[dtype])
+    k[1] = other
+    pos, freq = i32([[1, 0]]), torch.full((16,), math.pi / 4, device="cuda")  # (0, 1.4) * 3e38
+    r = seq.Rotation(32, [16], freq.data_ptr(), pos.data_ptr())
+    seq.cache_append(stream(), cache.desc, batch.desc, rows_of(seq, k), rows_of(seq, torch.ones_like(k)), r)
+    got = cache.views()[0].view(torch.float8_e4m3fn)[batch.lists[0][0], 0, :2].float()
+    assert cache.ks[batch.lists[0][0], 0].item() == 2.0**40
+    assert (got[0, 16:] == 448).all() and not got[0].isnan().any() and got[1].isnan().all() == math.isnan(other)
+
+
+@pytest.mark.parametrize("dtype, offset", [("bf16", 0), ("bf16", 1), ("f32", 0)])
+def test_append_leaves_rows_of_nobody(seq, rng, dtype, offset):
+    """Queries behind the last sequence stay, and positions of theirs do not matter; an odd alignment of q takes another kernel."""
+    batch = Batch(seq, [3, 20], [40, 20], 32, rng, rows=40)
+    cache = Cache(seq, batch.pages, 32, 2, 64, fill=0)
+    cache.ks.fill_(1.0), cache.vs.fill_(1.0)
+    k, v = (torch.randn(40, 2, 64, device="cuda", generator=rng).to(T[dtype]) for _ in range(2))
+    q, out = (torch.randn(40 * 320 + 1, device="cuda", generator=rng).to(T[dtype])[offset : offset + 40 * 320].unflatten(0, (40, 5, 64)) for _ in range(2))
+    old = out.clone()
+    pos = torch.randint(0, 1000, (1, 40), device="cuda", generator=rng, dtype=torch.int32)
+    freq = torch.rand(32, device="cuda", generator=rng)
+    r = seq.Rotation(64, [32], freq.data_ptr(), pos.data_ptr())
+    seq.cache_append(stream(), cache.desc, batch.desc, rows_of(seq, k), rows_of(seq, v), r, rows_of(seq, q), rows_of(seq, out))
+    want = torch.empty(23, 5, 64, device="cuda").to(T[dtype])
+    seq.rotary(stream(), r, 23, 64, rows_of(seq, q), rows_of(seq, want))
+    assert torch.equal(out[:23], want) and torch.equal(out[23:], old[23:])
+    codes = [c.clone() for c in cache.views()]
+    again = Cache(seq, batch.pages, 32, 2, 64, fill=0)
+    again.ks.fill_(1.0), again.vs.fill_(1.0)
+    seq.cache_append(stream(), again.desc, batch.desc, rows_of(seq, k), rows_of(seq, v), r)
+    assert all(torch.equal(a, b) for a, b in zip(codes, again.views())) and torch.equal(cache.ks, again.ks)
+
+
+@pytest.mark.parametrize("length", [(1 << 31) - 1, (1 << 30) + 1, -5, -(1 << 31)])
+def test_append_length_that_cannot_be(seq, rng, length):
+    batch = Batch(seq, [3, 3], [40, 20], 32, rng)
+    cache, _ = filled(seq, rng, batch, 32, 2, 64)
+    k = torch.randn(6, 2, 64, device="cuda", generator=rng).bfloat16()
+    batch.len[0] = length
+    old, status = [c.clone() for c in cache.views()], i32([0])
+    seq.cache_append(stream(), cache.desc, batch.desc, rows_of(seq, k), rows_of(seq, k), status=status.data_ptr())
+    assert status.item() == 1
+    for a, b in zip(old, cache.views()):
+        assert torch.equal(a[batch.lists[0]], b[batch.lists[0]]) and not torch.equal(a[batch.lists[1]], b[batch.lists[1]])
+
+
 # ---- attention
 
 
@@ -491,6 +543,44 @@ def test_attention_masks(seq, rng, new, lens, page, heads, group, dim, causal, w
     cache = Cache(seq, batch.pages, page, heads, dim).random(rng)
     q = torch.randn(batch.rows, heads * group, dim, device="cuda", generator=rng).bfloat16()
     check_attention(seq, cache, batch, q, "bf16", causal, window)
+
+
+@pytest.mark.parametrize("causal, window", [(True, 0), (True, 70), (False, 33)])
+@pytest.mark.parametrize("new, lens, page, heads, group, dim", [([150, 20], [900, 33], 16, 1, 2, 96), ([40], [800], 128, 3, 7, 32), ([2, 2], [700, 50], 128, 2, 6, 32)])
+def test_attention_masks_and_pages(seq, rng, new, lens, page, heads, group, dim, causal, window):
+    batch = Batch(seq, new, lens, page, rng)
+    cache = Cache(seq, batch.pages, page, heads, dim).random(rng)
+    q = torch.randn(batch.rows, heads * group, dim, device="cuda", generator=rng).to(torch.float16)
+    check_attention(seq, cache, batch, q, "f16", causal, window)
+
+
+@pytest.mark.parametrize("sequences, new, most, heads, dim", [(70, 1, 2300, 1, 128), (40, 20, 700, 1, 64), (112, 1, 2300, 32, 32), (75, 18, 500, 16, 32), (33, 40, 500, 1, 96)])
+def test_attention_many_sequences(seq, rng, sequences, new, most, heads, dim):
+    """More than a warp looks over at once, cut into shares and, with many heads, in whole units; some have nothing new, some no tokens."""
+    lens = torch.randint(0, 200, (sequences,), generator=rng, device="cuda").tolist()
+    lens[1], lens[-1] = most, most // 2
+    news = [min(n, 0 if b % 7 == 5 else 1 + b % new) for b, n in enumerate(lens)]
+    batch = Batch(seq, news, lens, 16, rng)
+    batch.desc.max_new = new
+    cache = Cache(seq, batch.pages, 16, heads, dim).random(rng)
+    q = torch.randn(batch.rows, heads, dim, device="cuda", generator=rng).bfloat16()
+    check_attention(seq, cache, batch, q, "bf16")
+
+
+@pytest.mark.parametrize("causal, window", [(True, 0), (True, 17), (False, 0), (True, (1 << 31) - 1)])
+@pytest.mark.parametrize("new", [[1, 1, 1], [60, 30, 50]])
+def test_attention_length_that_cannot_be(seq, rng, new, causal, window):
+    """Rows past the table are NaN, rows before the first place see nothing, and both come to an end; the others are as they were."""
+    batch = Batch(seq, new, [200, 300, 90], 32, rng)
+    cache = Cache(seq, batch.pages, 32, 2, 64).random(rng)
+    q = torch.randn(batch.rows, 2, 64, device="cuda", generator=rng).bfloat16()
+    want = check_attention(seq, cache, batch, q, "bf16", causal, window).clone()
+    batch.len[0], batch.len[2] = (1 << 31) - 1, -(1 << 31)
+    out, need = torch.empty_like(q), seq.cache_attention_workspace_bytes(cache.desc, batch.desc, 2)
+    ws = torch.empty(need + 16, dtype=torch.uint8, device="cuda")
+    seq.cache_attention(stream(), cache.desc, batch.desc, rows_of(seq, q), rows_of(seq, out), 0.125, ws.data_ptr(), need, causal=causal, window=window)
+    a, b = new[0], new[0] + new[1]
+    assert out[:a].isnan().all() and torch.equal(out[a:b], want[a:b]) and (out[b:] == 0).all()
 
 
 def test_attention_window_leaves_old_pages_alone(seq, rng):
@@ -620,7 +710,7 @@ def test_attention_sizes_that_are_only_bounds(seq, rng):
     batch = Batch(seq, [1, 3], [2000, 600], 32, rng)
     cache = Cache(seq, batch.pages, 32, 2, 64).random(rng)
     q = torch.randn(4, 8, 64, device="cuda", generator=rng).bfloat16()
-    for max_new, max_len in ((3, 2000), (9, 100000), (200, 2000), (3, 100)):
+    for max_new, max_len in ((3, 2000), (9, 100000), (200, 2000), (3, 100), ((1 << 31) - 1, 1 << 30)):
         batch.desc.max_new, batch.desc.max_len = max_new, max_len
         check_attention(seq, cache, batch, q, "bf16")
 
@@ -791,6 +881,19 @@ def test_refusals_that_need_a_device(seq, rng):
     for ptr, size in ((ws.data_ptr(), need - 1), (None, need), (ws.data_ptr() + 4, need)):
         with pytest.raises(ValueError, match="workspace"):
             seq.cache_attention(stream(), cache.desc, batch.desc, rows_of(seq, q), rows_of(seq, q), 1.0, ptr, size)
+    memory = torch.zeros(64, dtype=torch.int32)  # of the host
+    for owner, name in [(cache.desc, n) for n in ("k", "v", "k_scale", "v_scale")] + [(batch.desc, n) for n in ("first", "len", "table")]:
+        was = getattr(owner, name)
+        setattr(owner, name, memory.data_ptr())
+        with pytest.raises(RuntimeError, match="device memory"):
+            seq.cache_attention(stream(), cache.desc, batch.desc, rows_of(seq, q), rows_of(seq, q), 1.0, ws.data_ptr(), need)
+        with pytest.raises(RuntimeError, match="device memory"):
+            seq.cache_append(stream(), cache.desc, batch.desc, rows_of(seq, q), rows_of(seq, q))
+        setattr(owner, name, was)
+    with pytest.raises(RuntimeError, match="device memory"):
+        seq.cache_attention(stream(), cache.desc, batch.desc, rows_of(seq, q), rows_of(seq, q), 1.0, ws.data_ptr(), need, lse=memory.data_ptr())
+    with pytest.raises(RuntimeError, match="device memory"):
+        seq.rotary(stream(), seq.Rotation(64, [32], ws.data_ptr(), memory.data_ptr()), 1, 64, rows_of(seq, q), rows_of(seq, q))
     host = torch.zeros(1, 1, 64).bfloat16()
     with pytest.raises(RuntimeError, match="device memory"):
         seq.cache_attention(stream(), cache.desc, batch.desc, rows_of(seq, host), rows_of(seq, q), 1.0, ws.data_ptr(), need)

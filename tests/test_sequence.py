@@ -61,13 +61,13 @@ def entry(name, value):
 ROTATION = [field("rotation", "dims", 63), field("rotation", "dims", 66), field("rotation", "dims", -2), field("rotation", "axes", 0), field("rotation", "axes", 5),
             field("rotation", "freq", None), field("rotation", "pos", None), field("rotation", "pos", P + 2)]  # fmt: skip
 CACHE = [field("cache", n, None) for n in ("k", "v", "k_scale", "v_scale")] + [
-    field("cache", "pages", 0), field("cache", "heads", 0), field("cache", "page_tokens", 48), field("cache", "page_tokens", 256), field("cache", "page_tokens", 0),
+    field("cache", "pages", 0), field("cache", "heads", 0), field("cache", "heads", 65537), field("cache", "page_tokens", 48), field("cache", "page_tokens", 256), field("cache", "page_tokens", 0),
     field("cache", "dim", 48), field("cache", "dim", 256), field("cache", "k", P + 8), field("cache", "v_scale", P + 2), entry("cache", None),
 ]  # fmt: skip
 BATCH = [field("batch", n, None) for n in ("first", "len", "table")] + [field("batch", n, -1) for n in ("sequences", "rows", "max_new", "max_len", "table_stride")] + [
-    field("batch", "table_pages", 0), field("batch", "first", P + 1), entry("batch", None),
+    field("batch", "table_pages", 0), field("batch", "max_len", (1 << 30) + 1), field("batch", "first", P + 1), entry("batch", None),
 ]  # fmt: skip
-QUERIES = [field("q", "data", None), field("out", "data", None), field("q", "dtype", 1), field("out", "heads", 2), field("q", "dtype", 3), field("q", "dtype", -1),
+QUERIES = [field("q", "heads", 1 << 17), field("q", "data", None), field("out", "data", None), field("q", "dtype", 1), field("out", "heads", 2), field("q", "dtype", 3), field("q", "dtype", -1),
            field("q", "row_stride", -64), field("q", "data", P + 1), apart("row_stride", 248), apart("row_stride", 0), apart("head_stride", 56), apart("head_stride", 0)]  # fmt: skip
 REFUSED = (
     [("rotary", c) for c in ROTATION + QUERIES + [entry("rows", -1), entry("dim", 0), entry("dim", 1025), field("out", "row_stride", 8), entry("q", None), entry("rotation", None)]]
@@ -85,6 +85,18 @@ def test_refused(seq, op, change):
     a = good(seq)
     change(a)
     with pytest.raises(ValueError, match="cck_"):
+        call(seq, op, a)
+
+
+@pytest.mark.parametrize("op", ["rotary", "append", "attention"])
+def test_tensors_without_rows_may_be_null(seq, op):
+    """They get as far as the device."""
+    a = good(seq)
+    a["rows"] = a["batch"].rows = 0
+    for name in "q", "out", "k", "v":
+        a[name].data = None
+    a["rotation"].pos = None
+    with pytest.raises(RuntimeError, match="device"):
         call(seq, op, a)
 
 
