@@ -7,7 +7,8 @@
 // each (page, head) and as many heads at once as a block has groups; the angles of the page's rows are computed once, into shared memory,
 // for all heads that a block goes through. It wants 16-bit values and rotated parts that are whole vectors. append_kernel takes everything
 // else through shared memory, a block for each (page, head). Each row is read once, each code written once: bound by memory for
-// prompts, by latency for single tokens.
+// prompts (eight of about 900 tokens, 32 + 8 + 8 heads of 128: 49 us, 3.2 TB/s), by latency for single tokens (64: 10 us with the launch) and for small pages,
+// where a block is a chain of loads, angles, the largest value and the codes (2000 tokens of 3 x 20 heads of 64 in pages of 16: 16 us).
 #pragma once
 
 #include "rotary.cuh"
@@ -25,8 +26,9 @@ struct AppendArgs {
     int blocks_per_seq; // (page, head) units: [sequences][blocks_per_seq][heads]
     int kv_blocks;      // of the grid; the others rotate queries
     RotaryShape q;
-    // of append_pages_kernel: threads for a (page, head), and blocks that share a page's heads
+    // of append_pages_kernel: threads for a (page, head), blocks that share a page's heads
     int group_threads, head_splits;
+    int apart; // blocks of query_kernel; 0: queries are rotated by the blocks from kv_blocks on
 };
 
 constexpr int kAppendThreads = 256;
@@ -155,7 +157,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
         const float2 cs = cos_sin(A.rotation.pos[axis_of(A.rotation, p) * A.rotation.pos_stride + row0 + u], turns_of(A.rotation.freq[p]));
         float* a = fk + u * kp + (A.rotation.adjacent ? 2 * p : p);
         float* c = a + (A.rotation.adjacent ? 1 : half);
-        const float2 z = rotate(*a, *c, cs);
+        const float2 z = rotate_exactly(*a, *c, cs);
         *a = z.x, *c = z.y;
     }
     __syncthreads();
@@ -255,6 +257,9 @@ __global__ void __launch_bounds__(kPageThreads, 1) append_pages_kernel(const __g
                                     query_units(A));
         return;
     }
+    if (A.apart) {
+        let_next_start();
+    }
     const int P = C.page_tokens, H = C.heads, part = blockIdx.x % A.head_splits;
     const PageRows pr = page_rows(A, blockIdx.x / A.head_splits, part == 0 && tid == 0);
     if (pr.page < 0) {
@@ -322,7 +327,7 @@ __global__ void __launch_bounds__(kPageThreads, 1) append_pages_kernel(const __g
                     const float4 w = cs[e];
                     float &a0 = kAdjacent ? x[n][4 * e] : x[n][2 * e], &b0 = kAdjacent ? x[n][4 * e + 1] : x[n][8 + 2 * e];
                     float &a1 = kAdjacent ? x[n][4 * e + 2] : x[n][2 * e + 1], &b1 = kAdjacent ? x[n][4 * e + 3] : x[n][9 + 2 * e];
-                    const float2 z0 = rotate(a0, b0, make_float2(w.x, w.y)), z1 = rotate(a1, b1, make_float2(w.z, w.w));
+                    const float2 z0 = rotate_exactly(a0, b0, make_float2(w.x, w.y)), z1 = rotate_exactly(a1, b1, make_float2(w.z, w.w));
                     a0 = z0.x, b0 = z0.y, a1 = z1.x, b1 = z1.y;
                 }
             }
@@ -503,6 +508,17 @@ __global__ void __launch_bounds__(kPageThreads, 1) append_pages_kernel(const __g
             }
         }
     }
+}
+
+// Many queries: beside append_pages_kernel instead of in its blocks, whose registers would leave them half of the warps. Reads and writes nothing
+// that it does; the wait at the end is for what comes after both.
+template <class T, bool kAdjacent>
+__global__ void __launch_bounds__(kRotaryThreads, 4) query_kernel(const __grid_constant__ AppendArgs A) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    const int warp = threadIdx.x >> 5, warps = kRotaryThreads / 32;
+    rotary_warp<T, 8, kAdjacent>(A.rotation, A.q, reinterpret_cast<float2*>(smem) + warp * (A.rotation.dims / 2), int64_t(blockIdx.x) * warps + warp, int64_t(gridDim.x) * warps,
+                                 query_units(A));
+    wait_for_previous();
 }
 
 } // namespace seq

@@ -1,10 +1,10 @@
-// Attention over the paged 8-bit cache for few rows: decode steps, guessed tokens.
+// Attention over the paged 8-bit cache for few rows (up to 24 a head of the cache): decode steps, guessed tokens.
 //
 //   x(r, t) = softmax_scale log2(e) k_scale(t) (q_r . k_t) + log2 v_scale(t)          (k_t, v_t: codes)
 //   m = max_t x,  p = 2^(x - m),  out = sum_t p v_t / sum_t p / v_scale(t)
 //
-// The values' scale rides in the exponent: p stays in [0, 1] whatever the scales of the pages are, goes to the tensor cores as f16
-// and what it loses there (below 2^-24) is small against the largest term of the sum. One pass with running maximum and sum.
+// The values' scale rides in the exponent: p does not grow with the scales of the pages, goes to the tensor cores as f16 and what it
+// loses there is small against the largest term of the sum. One pass with running maximum and sum.
 //
 // Bound by memory: 2 * dim bytes a key and head, read once. Every warp runs on its own: it takes granules of 32 or 64 keys, which lie in one
 // piece in a page, through a ring of bulk copies into its own shared memory. Keys are the 16 rows of its tiles, the 8 columns are query
@@ -18,11 +18,13 @@
 //           2^-16 would vanish beside one of 1, and a long tail of such keys can outweigh it.
 // Score rows i and i + 8 of tile u are keys 16 u + 4 (i / 2) + i % 2 and two on, such that transposing a score tile's two 8 x 8 halves
 // gives p in the order in which a word of V holds four keys.
-// The running maximum is only a reference: it moves when a score is 2^8 over it, so that shuffles and the rescaling of the sums
-// are rare; p is at most 2^14 and what f16 loses of it lies below 2^-30 of the largest.
+// The running maximum is only a reference: it moves when a score is 2^8 over the largest it was set by, so that shuffles and the
+// rescaling of the sums are rare; p is at most 2^14, the largest at least 2^6, and what f16 loses (2^-25) lies below 2^-30 of that.
+// 64 sequences of up to 8192 tokens, 32 heads on 8 of 128: 140 us, 5.7 TB/s, 0.87 of a copy's rate. One sequence of 700 in pages of 16: 14 us, a
+// chain of a launch, a look at the table, a copy, six granules a warp, each fetching its instructions anew, and the way out.
 #pragma once
 
-#include <climits>
+#include <type_traits>
 
 #include "sequence.cuh"
 
@@ -94,15 +96,10 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) { // an 8 x 8 matrix 
 constexpr int kDecodeWarps = 4;
 // p = 2^(x - base); base = largest x - kHeadroom when it is set, and is set anew when an x is over base + kSlack. It begins below all scores
 constexpr float kHeadroom = 6.f, kSlack = 14.f, kNoBase = -1e30f;
-// NT: tiles of 8 query rows. Blocks of threads an SM: what registers (32 NT of sums, 16 NT of queries at 128 dims) and shared memory hold
+// terms of 4 bits that hold a query
 template <class T>
-constexpr bool T_is_f16() {
-    return false;
-}
-template <>
-constexpr bool T_is_f16<__half>() {
-    return true;
-}
+constexpr int kTermsOf = std::is_same_v<T, __half> ? 3 : 2;
+// NT: tiles of 8 query rows. Blocks of threads an SM: what registers (32 NT of sums, 16 NT of queries at 128 dims) and shared memory hold
 template <int D, int NT>
 struct DecodeShape {
     static constexpr int kBlocks = NT == 1 ? 3 : 2;
@@ -264,7 +261,7 @@ __device__ __noinline__ void clear_values(uint32_t v, int lo, int hi, uint32_t a
 template <class T, int D, int NT>
 __global__ void __launch_bounds__(kDecodeWarps * 32, DecodeShape<D, NT>::kBlocks) decode_kernel(const __grid_constant__ AttentionArgs A) {
     using S = DecodeShape<D, NT>;
-    constexpr int kTerms = sizeof(T) == 2 && T_is_f16<T>() ? 3 : 2;
+    constexpr int kTerms = kTermsOf<T>;
     constexpr int kRows = 8 * NT, kTiles = S::kKeys / 16, kKeysShift = S::kKeys == 64 ? 6 : 5; // kTiles: of 16 keys
     extern __shared__ __align__(128) unsigned char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n8 = lane >> 2, c4 = lane & 3;
@@ -294,318 +291,318 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DecodeShape<D, NT>::kBlocks
     int slot = 0, phase = 0;
 #pragma unroll 1
     while (left > 0) {
-    const Tile own = tile_at(A, tile);
-    if (own.rows == 0) {
-        if (!A.part_o) {
-            return;
-        }
-        tile++, head = 0;
-        continue;
-    }
-    const Sequence s = own.s;
-    const int b = tile / A.row_tiles, r0 = own.r0, r1 = r0 + own.rows;
-    const TileKeys keys = keys_of_tile(A, s, r0, r1);
-    const int all = max(1, keys.g1 - keys.g0);
-    // what of the unit's stretch of the line is the share's, without the cost at its head
-    const int64_t to = A.part_o ? min(int64_t(all + A.unit_cost), done + left) : all + A.unit_cost, unit_at = at - done;
-    const int ga = keys.g0 + max(0, int(done) - A.unit_cost), gb = keys.g0 + max(0, int(to) - A.unit_cost);
-    left -= to - done, at = unit_at + to, done = 0;
-    if (gb == ga) { // the cost alone: the next share begins with the unit
-        break;
-    }
-    const bool alone = gb - ga == all; // a unit of this block only
-    if (ga == keys.g0 && !alone) {
-        split.tile = tile, split.head = head, split.last = int((unit_at + all + A.unit_cost - 1) / size);
-    }
-    const int part = 2 * blockIdx.x + (ga == keys.g0 ? 1 : 0);
-
-    // this warp's granules: ga + warp, + kDecodeWarps, ...; a granule is one piece of a page, or several of small pages. A lane looks
-    // one piece up, so that 32 are known at a time: `now` for the granule worked on, `next` for copies ahead of it
-    const int mine = max(0, ceil_div(gb - ga - warp, kDecodeWarps));
-    const int piece_shift = min(A.page_shift, kKeysShift), pieces_shift = kKeysShift - piece_shift, pieces = 1 << pieces_shift;
-    auto look_up = [&](int first) {
-        const int j = first + lane, key = (ga + warp + (j >> pieces_shift) * kDecodeWarps) * S::kKeys + ((j & (pieces - 1)) << piece_shift);
-        return piece_at(A, b, head, key, j < mine << pieces_shift && key < keys.hi && key + (1 << piece_shift) > keys.lo);
-    };
-    Piece now = look_up(0), next = look_up(32);
-    int batch = 0; // `now` holds pieces 32 batch ..
-    auto issue = [&](int i, int slot) { // granule i into its stage
-        const uint32_t st = ring + slot * S::kStage, bar = bars + slot * 8, bytes = D << piece_shift;
-        if (lane == 0) {
-            bar_expect(bar, S::kStage);
-        }
-#pragma unroll 1
-        for (int h = 0; h < pieces; h++) {
-            const int j = (i << pieces_shift) + h;
-            const int64_t at = __shfl_sync(0xffffffffu, j >> 5 == batch ? now.at : next.at, j & 31);
-            if (lane == 0) {
-                bulk_load(st + h * bytes, static_cast<const char*>(A.cache.k) + at, bytes, bar);
-                bulk_load(st + S::kKeys * D + h * bytes, static_cast<const char*>(A.cache.v) + at, bytes, bar);
+        const Tile own = tile_at(A, tile);
+        if (own.rows == 0) {
+            if (!A.part_o) {
+                return;
             }
+            tile++, head = 0;
+            continue;
         }
-    };
-#pragma unroll 1
-    for (int i = 0; i < min(mine, S::kStages); i++) {
-        issue(i, (slot + i) % S::kStages);
-    }
-
-    // queries: lane n holds its dims of row 8 t + n, in terms; scores of rows 8 t + 2 c and the next come out in the lane
-    uint32_t q[NT][D / 16][kTerms];
-    float qs[NT][2];
-    int lo[NT][2], hi[NT][2];
-#pragma unroll
-    for (int t = 0; t < NT; t++) {
-        const int r = r0 + t * 8 + n8;
-        Vec<T, 4> v[D / 16] = {};
-        float top = 0.f;
-        if (r < r1) {
-            const T* from = static_cast<const T*>(A.q) + (s.row0 + r / G) * A.qr + (head * G + r % G) * A.qh + 4 * c4;
-#pragma unroll
-            for (int k = 0; k < D / 16; k++) {
-                v[k] = *reinterpret_cast<const Vec<T, 4>*>(from + 16 * k);
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < D / 16; k++) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                top = fmaxf(top, fabsf(to_f32(v[k].v[e])));
-            }
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // 2^-ex brings the largest to [128, 256); an infinity makes the row NaN
-        const int ex = min(max((__float_as_int(top) >> 23) - 134, -118), 118);
-        const float down = top <= 3.402823466e38f ? exp2_int(-ex) : __int_as_float(0x7fffffff), up = exp2_int(ex);
-#pragma unroll
-        for (int k = 0; k < D / 16; k++) {
-            float4 x = make_float4(to_f32(v[k].v[0]) * down, to_f32(v[k].v[1]) * down, to_f32(v[k].v[2]) * down, to_f32(v[k].v[3]) * down);
-#pragma unroll
-            for (int m = 0; m < kTerms; m++) {
-                q[t][k][m] = pack_e4m3(x.x, x.y, x.z, x.w);
-                const float4 y = codes_to_f32(q[t][k][m]);
-                x = make_float4(x.x - y.x, x.y - y.y, x.z - y.z, x.w - y.w);
-            }
-        }
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int row = r0 + t * 8 + 2 * c4 + h;
-            qs[t][h] = __shfl_sync(0xffffffffu, up, 4 * (2 * c4 + h));
-            lo[t][h] = hi[t][h] = 0;
-            if (row < r1) {
-                const int2 see = seen_by(A, s.place0 + row / G, s.len);
-                lo[t][h] = see.x, hi[t][h] = see.y;
-            }
-        }
-    }
-
-    float o[D / 16][NT][4] = {}, base[NT][2], l[NT][2] = {};
-#pragma unroll
-    for (int t = 0; t < NT; t++) {
-        base[t][0] = base[t][1] = kNoBase;
-    }
-    const int tok = 4 * (n8 >> 1) + (n8 & 1); // the first key of the lane's score rows
-    // the row of a stage that this lane names to ldmatrix: keys in the order of the score rows; dims
-    const int mk = 4 * ((lane & 7) >> 1) + (lane & 1) + 2 * (lane >> 3 & 1);
-    const uint32_t k_at = (mk >> 3) * 8 * D + (mk & 7) * 16 + (lane >> 4) * 128, v_at = S::kKeys * D + (lane >> 4) * 16 * D + (lane & 15) * 16;
-#pragma unroll 1
-    for (int i = 0; i < mine; i++) {
-        if ((i << pieces_shift) >> 5 != batch) {
-            now = next, batch++;
-            next = look_up(32 * (batch + 1));
-        }
-        float a[kTiles], e[kTiles], iv[kTiles];
-        uint32_t absent = 0;
-        if (pieces == 1) {
-            const float ks = __shfl_sync(0xffffffffu, now.ks, i & 31), vs = __shfl_sync(0xffffffffu, now.vs, i & 31);
-            absent = ks == ks ? 0u : ~0u;
-            a[0] = ks * A.scale_log2, e[0] = log2_fast(vs), iv[0] = inverse_fast(vs);
-#pragma unroll
-            for (int u = 1; u < kTiles; u++) {
-                a[u] = a[0], e[u] = e[0], iv[u] = iv[0];
-            }
-        } else {
-#pragma unroll
-            for (int u = 0; u < kTiles; u++) {
-                const int from = ((i << pieces_shift) + (u * 16 >> piece_shift)) & 31;
-                const float ks = __shfl_sync(0xffffffffu, now.ks, from), vs = __shfl_sync(0xffffffffu, now.vs, from);
-                absent |= ks == ks ? 0u : 1u << u;
-                a[u] = ks * A.scale_log2, e[u] = log2_fast(vs), iv[u] = inverse_fast(vs);
-            }
-        }
-        const uint32_t st = ring + slot * S::kStage;
-        const int key0 = (ga + warp + i * kDecodeWarps) * S::kKeys;
-        if (!bar_wait(bars + slot * 8, phase)) {
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                l[t][0] = l[t][1] = __int_as_float(0x7fffffff); // a copy got lost: rows come out as NaN
-            }
+        const Sequence s = own.s;
+        const int b = tile / A.row_tiles, r0 = own.r0, r1 = r0 + own.rows;
+        const TileKeys keys = keys_of_tile(A, s, r0, r1);
+        const int all = max(1, keys.g1 - keys.g0);
+        // what of the unit's stretch of the line is the share's, without the cost at its head
+        const int64_t to = A.part_o ? min(int64_t(all + A.unit_cost), done + left) : all + A.unit_cost, unit_at = at - done;
+        const int ga = keys.g0 + max(0, int(done) - A.unit_cost), gb = keys.g0 + max(0, int(to) - A.unit_cost);
+        left -= to - done, at = unit_at + to, done = 0;
+        if (gb == ga) { // the cost alone: the next share begins with the unit
             break;
         }
-        float x[kTiles][NT][4] = {};
-#pragma unroll
-        for (int k = 0; k < D / 32; k++) {
-#pragma unroll
-            for (int u = 0; u < kTiles; u++) {
-                uint32_t w[4];
-                ldmatrix4(w, st + k_at + u * 16 * D + k * 256);
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-#pragma unroll
-                    for (int m = 0; m < kTerms; m++) {
-                        mma_e4m3(x[u][t], w, q[t][2 * k][m], q[t][2 * k + 1][m]);
-                    }
+        const bool alone = gb - ga == all; // a unit of this block only
+        if (ga == keys.g0 && !alone) {
+            split.tile = tile, split.head = head, split.last = int((unit_at + all + A.unit_cost - 1) / size);
+        }
+        const int part = 2 * blockIdx.x + (ga == keys.g0 ? 1 : 0);
+
+        // this warp's granules: ga + warp, + kDecodeWarps, ...; a granule is one piece of a page, or several of small pages. A lane looks
+        // one piece up, so that 32 are known at a time: `now` for the granule worked on, `next` for copies ahead of it
+        const int mine = max(0, ceil_div(gb - ga - warp, kDecodeWarps));
+        const int piece_shift = min(A.page_shift, kKeysShift), pieces_shift = kKeysShift - piece_shift, pieces = 1 << pieces_shift;
+        auto look_up = [&](int first) {
+            const int j = first + lane, key = (ga + warp + (j >> pieces_shift) * kDecodeWarps) * S::kKeys + ((j & (pieces - 1)) << piece_shift);
+            return piece_at(A, b, head, key, j < mine << pieces_shift && key < keys.hi && key + (1 << piece_shift) > keys.lo);
+        };
+        Piece now = look_up(0), next = look_up(32);
+        int batch = 0; // `now` holds pieces 32 batch ..
+        auto issue = [&](int i, int slot) { // granule i into its stage
+            const uint32_t st = ring + slot * S::kStage, bar = bars + slot * 8, bytes = D << piece_shift;
+            if (lane == 0) {
+                bar_expect(bar, S::kStage);
+            }
+#pragma unroll 1
+            for (int h = 0; h < pieces; h++) {
+                const int j = (i << pieces_shift) + h;
+                const int64_t at = __shfl_sync(0xffffffffu, j >> 5 == batch ? now.at : next.at, j & 31);
+                if (lane == 0) {
+                    bulk_load(st + h * bytes, static_cast<const char*>(A.cache.k) + at, bytes, bar);
+                    bulk_load(st + S::kKeys * D + h * bytes, static_cast<const char*>(A.cache.v) + at, bytes, bar);
                 }
             }
+        };
+#pragma unroll 1
+        for (int i = 0; i < min(mine, S::kStages); i++) {
+            issue(i, (slot + i) % S::kStages);
         }
-#pragma unroll
-        for (int u = 0; u < kTiles; u++) {
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                const float f[2] = {a[u] * qs[t][0], a[u] * qs[t][1]};
-#pragma unroll
-                for (int v = 0; v < 4; v++) {
-                    x[u][t][v] = fmaf(x[u][t][v], f[v & 1], e[u]);
-                }
-            }
-        }
-        // masked scores are -inf
-        if (key0 < keys.all_lo || key0 + S::kKeys > keys.all_hi) {
-#pragma unroll
-            for (int u = 0; u < kTiles; u++) {
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-#pragma unroll
-                    for (int v = 0; v < 4; v++) {
-                        const int key = key0 + 16 * u + tok + (v & 2);
-                        x[u][t][v] = key >= lo[t][v & 1] && key < hi[t][v & 1] ? x[u][t][v] : -INFINITY;
-                    }
-                }
-            }
-        }
-        uint32_t p[kTiles][NT][2];
+
+        // queries: lane n holds its dims of row 8 t + n, in terms; scores of rows 8 t + 2 c and the next come out in the lane
+        uint32_t q[NT][D / 16][kTerms];
+        float qs[NT][2];
+        int lo[NT][2], hi[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            float top[2] = {-INFINITY, -INFINITY};
+            const int r = r0 + t * 8 + n8;
+            Vec<T, 4> v[D / 16] = {};
+            float top = 0.f;
+            if (r < r1) {
+                const T* from = static_cast<const T*>(A.q) + (s.row0 + r / G) * A.qr + (head * G + r % G) * A.qh + 4 * c4;
+#pragma unroll
+                for (int k = 0; k < D / 16; k++) {
+                    v[k] = *reinterpret_cast<const Vec<T, 4>*>(from + 16 * k);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < D / 16; k++) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    top = fmaxf(top, fabsf(to_f32(v[k].v[e])));
+                }
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // 2^-ex brings the largest to [128, 256); an infinity makes the row NaN
+            const int ex = min(max((__float_as_int(top) >> 23) - 134, -118), 118);
+            const float down = top <= 3.402823466e38f ? exp2_int(-ex) : __int_as_float(0x7fffffff), up = exp2_int(ex);
+#pragma unroll
+            for (int k = 0; k < D / 16; k++) {
+                float4 x = make_float4(to_f32(v[k].v[0]) * down, to_f32(v[k].v[1]) * down, to_f32(v[k].v[2]) * down, to_f32(v[k].v[3]) * down);
+#pragma unroll
+                for (int m = 0; m < kTerms; m++) {
+                    q[t][k][m] = pack_e4m3(x.x, x.y, x.z, x.w);
+                    const float4 y = codes_to_f32(q[t][k][m]);
+                    x = make_float4(x.x - y.x, x.y - y.y, x.z - y.z, x.w - y.w);
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int row = r0 + t * 8 + 2 * c4 + h;
+                qs[t][h] = __shfl_sync(0xffffffffu, up, 4 * (2 * c4 + h));
+                lo[t][h] = hi[t][h] = 0;
+                if (row < r1) {
+                    const int2 see = seen_by(A, s.place0 + row / G, s.len);
+                    lo[t][h] = see.x, hi[t][h] = see.y;
+                }
+            }
+        }
+
+        float o[D / 16][NT][4] = {}, base[NT][2], l[NT][2] = {};
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            base[t][0] = base[t][1] = kNoBase;
+        }
+        const int tok = 4 * (n8 >> 1) + (n8 & 1); // the first key of the lane's score rows
+        // the row of a stage that this lane names to ldmatrix: keys in the order of the score rows; dims
+        const int mk = 4 * ((lane & 7) >> 1) + (lane & 1) + 2 * (lane >> 3 & 1);
+        const uint32_t k_at = (mk >> 3) * 8 * D + (mk & 7) * 16 + (lane >> 4) * 128, v_at = S::kKeys * D + (lane >> 4) * 16 * D + (lane & 15) * 16;
+#pragma unroll 1
+        for (int i = 0; i < mine; i++) {
+            if ((i << pieces_shift) >> 5 != batch) {
+                now = next, batch++;
+                next = look_up(32 * (batch + 1));
+            }
+            float a[kTiles], e[kTiles], iv[kTiles];
+            uint32_t absent = 0;
+            if (pieces == 1) {
+                const float ks = __shfl_sync(0xffffffffu, now.ks, i & 31), vs = __shfl_sync(0xffffffffu, now.vs, i & 31);
+                absent = ks == ks ? 0u : ~0u;
+                a[0] = ks * A.scale_log2, e[0] = log2_fast(vs), iv[0] = inverse_fast(vs);
+#pragma unroll
+                for (int u = 1; u < kTiles; u++) {
+                    a[u] = a[0], e[u] = e[0], iv[u] = iv[0];
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < kTiles; u++) {
+                    const int from = ((i << pieces_shift) + (u * 16 >> piece_shift)) & 31;
+                    const float ks = __shfl_sync(0xffffffffu, now.ks, from), vs = __shfl_sync(0xffffffffu, now.vs, from);
+                    absent |= ks == ks ? 0u : 1u << u;
+                    a[u] = ks * A.scale_log2, e[u] = log2_fast(vs), iv[u] = inverse_fast(vs);
+                }
+            }
+            const uint32_t st = ring + slot * S::kStage;
+            const int key0 = (ga + warp + i * kDecodeWarps) * S::kKeys;
+            if (!bar_wait(bars + slot * 8, phase)) {
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    l[t][0] = l[t][1] = __int_as_float(0x7fffffff); // a copy got lost: rows come out as NaN
+                }
+                break;
+            }
+            float x[kTiles][NT][4] = {};
+#pragma unroll
+            for (int k = 0; k < D / 32; k++) {
+#pragma unroll
+                for (int u = 0; u < kTiles; u++) {
+                    uint32_t w[4];
+                    ldmatrix4(w, st + k_at + u * 16 * D + k * 256);
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+#pragma unroll
+                        for (int m = 0; m < kTerms; m++) {
+                            mma_e4m3(x[u][t], w, q[t][2 * k][m], q[t][2 * k + 1][m]);
+                        }
+                    }
+                }
+            }
 #pragma unroll
             for (int u = 0; u < kTiles; u++) {
 #pragma unroll
-                for (int v = 0; v < 4; v++) {
-                    top[v & 1] = fmaxf(top[v & 1], x[u][t][v]);
+                for (int t = 0; t < NT; t++) {
+                    const float f[2] = {a[u] * qs[t][0], a[u] * qs[t][1]};
+#pragma unroll
+                    for (int v = 0; v < 4; v++) {
+                        x[u][t][v] = fmaf(x[u][t][v], f[v & 1], e[u]);
+                    }
                 }
             }
-            if (__any_sync(0xffffffffu, top[0] > base[t][0] + kSlack || top[1] > base[t][1] + kSlack)) {
-                float corr[2];
+            // masked scores are -inf
+            if (key0 < keys.all_lo || key0 + S::kKeys > keys.all_hi) {
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const float was = base[t][h];
+                for (int u = 0; u < kTiles; u++) {
 #pragma unroll
-                    for (int w = 4; w <= 16; w *= 2) {
-                        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], w));
+                    for (int t = 0; t < NT; t++) {
+#pragma unroll
+                        for (int v = 0; v < 4; v++) {
+                            const int key = key0 + 16 * u + tok + (v & 2);
+                            x[u][t][v] = key >= lo[t][v & 1] && key < hi[t][v & 1] ? x[u][t][v] : -INFINITY;
+                        }
                     }
-                    base[t][h] = fmaxf(was, top[h] - kHeadroom);
-                    corr[h] = exp2_fast(was - base[t][h]);
-                    l[t][h] *= corr[h];
+                }
+            }
+            uint32_t p[kTiles][NT][2];
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int u = 0; u < kTiles; u++) {
+#pragma unroll
+                    for (int v = 0; v < 4; v++) {
+                        top[v & 1] = fmaxf(top[v & 1], x[u][t][v]);
+                    }
+                }
+                if (__any_sync(0xffffffffu, top[0] > base[t][0] + kSlack || top[1] > base[t][1] + kSlack)) {
+                    float corr[2];
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const float was = base[t][h];
+#pragma unroll
+                        for (int w = 4; w <= 16; w *= 2) {
+                            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], w));
+                        }
+                        base[t][h] = fmaxf(was, top[h] - kHeadroom);
+                        corr[h] = exp2_fast(was - base[t][h]);
+                        l[t][h] *= corr[h];
+                    }
+#pragma unroll
+                    for (int d = 0; d < D / 16; d++) {
+                        o[d][t][0] *= corr[0], o[d][t][1] *= corr[1], o[d][t][2] *= corr[0], o[d][t][3] *= corr[1];
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < kTiles; u++) {
+                    const float p0 = exp2_fast(x[u][t][0] - base[t][0]), p1 = exp2_fast(x[u][t][1] - base[t][1]);
+                    const float p2 = exp2_fast(x[u][t][2] - base[t][0]), p3 = exp2_fast(x[u][t][3] - base[t][1]);
+                    l[t][0] = fmaf(p0 + p2, iv[u], l[t][0]), l[t][1] = fmaf(p1 + p3, iv[u], l[t][1]);
+                    p[u][t][0] = transpose8(pack_f16(p0, p1)), p[u][t][1] = transpose8(pack_f16(p2, p3));
+                }
+            }
+            if (key0 < keys.lo || key0 + S::kKeys > keys.hi || absent) {
+                clear_values<D, S::kKeys>(st + S::kKeys * D, keys.lo - key0, keys.hi - key0, absent);
+            }
+#pragma unroll
+            for (int u = 0; u < kTiles; u += 2) {
+#pragma unroll
+                for (int d = 0; d < D / 16; d++) {
+                    uint32_t w[4], f[2][4]; // 16 dims of 32 keys; as f16, of 16 keys each
+                    ldmatrix4(w, st + v_at + u * 16 * D + d * 256);
+                    unpack_e4m3(w[0], f[0][0], f[0][2]), unpack_e4m3(w[1], f[0][1], f[0][3]);
+                    unpack_e4m3(w[2], f[1][0], f[1][2]), unpack_e4m3(w[3], f[1][1], f[1][3]);
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        mma_f16(o[d][t], f[0], p[u][t][0], p[u][t][1]);
+                        mma_f16(o[d][t], f[1], p[u + 1][t][0], p[u + 1][t][1]);
+                    }
+                }
+            }
+            __syncwarp(); // the stage has been read
+            if (i + S::kStages < mine) {
+                issue(i + S::kStages, slot);
+            }
+            if (++slot == S::kStages) {
+                slot = 0, phase ^= 1;
+            }
+        }
+
+        // the warps' shares together, through the ring
+        constexpr int kPitch = D + 4;
+        static_assert(kDecodeWarps * kRows * (kPitch + 2) * 4 <= S::kRing, "the shares fit the ring");
+        float* so = reinterpret_cast<float*>(smem);
+        float* sm = so + kDecodeWarps * kRows * kPitch;
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                float sum = l[t][h];
+#pragma unroll
+                for (int w = 4; w <= 16; w *= 2) {
+                    sum += __shfl_xor_sync(0xffffffffu, sum, w);
+                }
+                const int row = warp * kRows + t * 8 + 2 * c4 + h;
+                if (n8 == 0) {
+                    sm[2 * row] = base[t][h], sm[2 * row + 1] = sum;
                 }
 #pragma unroll
                 for (int d = 0; d < D / 16; d++) {
-                    o[d][t][0] *= corr[0], o[d][t][1] *= corr[1], o[d][t][2] *= corr[0], o[d][t][3] *= corr[1];
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < kTiles; u++) {
-                const float p0 = exp2_fast(x[u][t][0] - base[t][0]), p1 = exp2_fast(x[u][t][1] - base[t][1]);
-                const float p2 = exp2_fast(x[u][t][2] - base[t][0]), p3 = exp2_fast(x[u][t][3] - base[t][1]);
-                l[t][0] = fmaf(p0 + p2, iv[u], l[t][0]), l[t][1] = fmaf(p1 + p3, iv[u], l[t][1]);
-                p[u][t][0] = transpose8(pack_f16(p0, p1)), p[u][t][1] = transpose8(pack_f16(p2, p3));
-            }
-        }
-        if (key0 < keys.lo || key0 + S::kKeys > keys.hi || absent) {
-            clear_values<D, S::kKeys>(st + S::kKeys * D, keys.lo - key0, keys.hi - key0, absent);
-        }
-#pragma unroll
-        for (int u = 0; u < kTiles; u += 2) {
-#pragma unroll
-            for (int d = 0; d < D / 16; d++) {
-                uint32_t w[4], f[2][4]; // 16 dims of 32 keys; as f16, of 16 keys each
-                ldmatrix4(w, st + v_at + u * 16 * D + d * 256);
-                unpack_e4m3(w[0], f[0][0], f[0][2]), unpack_e4m3(w[1], f[0][1], f[0][3]);
-                unpack_e4m3(w[2], f[1][0], f[1][2]), unpack_e4m3(w[3], f[1][1], f[1][3]);
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    mma_f16(o[d][t], f[0], p[u][t][0], p[u][t][1]);
-                    mma_f16(o[d][t], f[1], p[u + 1][t][0], p[u + 1][t][1]);
+                    so[row * kPitch + 16 * d + n8] = o[d][t][h], so[row * kPitch + 16 * d + 8 + n8] = o[d][t][2 + h];
                 }
             }
         }
-        __syncwarp(); // the stage has been read
-        if (i + S::kStages < mine) {
-            issue(i + S::kStages, slot);
-        }
-        if (++slot == S::kStages) {
-            slot = 0, phase ^= 1;
-        }
-    }
-
-    // the warps' shares together, through the ring
-    constexpr int kPitch = D + 4;
-    static_assert(kDecodeWarps * kRows * (kPitch + 2) * 4 <= S::kRing, "the shares fit the ring");
-    float* so = reinterpret_cast<float*>(smem);
-    float* sm = so + kDecodeWarps * kRows * kPitch;
-    __syncthreads();
-#pragma unroll
-    for (int t = 0; t < NT; t++) {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            float sum = l[t][h];
-#pragma unroll
-            for (int w = 4; w <= 16; w *= 2) {
-                sum += __shfl_xor_sync(0xffffffffu, sum, w);
-            }
-            const int row = warp * kRows + t * 8 + 2 * c4 + h;
-            if (n8 == 0) {
-                sm[2 * row] = base[t][h], sm[2 * row + 1] = sum;
-            }
-#pragma unroll
-            for (int d = 0; d < D / 16; d++) {
-                so[row * kPitch + 16 * d + n8] = o[d][t][h], so[row * kPitch + 16 * d + 8 + n8] = o[d][t][2 + h];
-            }
-        }
-    }
-    __syncthreads();
-    constexpr int kLanes = D / 4; // threads of a row, four dims each
+        __syncthreads();
+        constexpr int kLanes = D / 4; // threads of a row, four dims each
 #pragma unroll 1
-    for (int i = threadIdx.x; i < own.rows * kLanes; i += kDecodeWarps * 32) {
-        const int r = i / kLanes, d = i % kLanes * 4;
-        float top = kNoBase, sum = 0.f;
+        for (int i = threadIdx.x; i < own.rows * kLanes; i += kDecodeWarps * 32) {
+            const int r = i / kLanes, d = i % kLanes * 4;
+            float top = kNoBase, sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < kDecodeWarps; w++) {
-            top = fmaxf(top, sm[2 * (w * kRows + r)]);
-        }
-        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int w = 0; w < kDecodeWarps; w++) {
+                top = fmaxf(top, sm[2 * (w * kRows + r)]);
+            }
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < kDecodeWarps; w++) {
-            const float f = exp2_fast(sm[2 * (w * kRows + r)] - top);
-            const float4 z = *reinterpret_cast<const float4*>(so + (w * kRows + r) * kPitch + d);
-            sum = fmaf(sm[2 * (w * kRows + r) + 1], f, sum);
-            y.x = fmaf(z.x, f, y.x), y.y = fmaf(z.y, f, y.y), y.z = fmaf(z.z, f, y.z), y.w = fmaf(z.w, f, y.w);
-        }
-        if (alone) {
-            store_out<T>(A, s.row0 + (r0 + r) / G, head * G + (r0 + r) % G, d, y, top, sum);
-        } else {
-            *reinterpret_cast<float4*>(A.part_o + (int64_t(part) * kRows + r) * D + d) = y;
-            if (d == 0) {
-                *reinterpret_cast<float2*>(A.part_ml + 2 * (int64_t(part) * kRows + r)) = make_float2(top, sum);
+            for (int w = 0; w < kDecodeWarps; w++) {
+                const float f = exp2_fast(sm[2 * (w * kRows + r)] - top);
+                const float4 z = *reinterpret_cast<const float4*>(so + (w * kRows + r) * kPitch + d);
+                sum = fmaf(sm[2 * (w * kRows + r) + 1], f, sum);
+                y.x = fmaf(z.x, f, y.x), y.y = fmaf(z.y, f, y.y), y.z = fmaf(z.z, f, y.z), y.w = fmaf(z.w, f, y.w);
+            }
+            if (alone) {
+                store_out<T>(A, s.row0 + (r0 + r) / G, head * G + (r0 + r) % G, d, y, top, sum);
+            } else {
+                *reinterpret_cast<float4*>(A.part_o + (int64_t(part) * kRows + r) * D + d) = y;
+                if (d == 0) {
+                    *reinterpret_cast<float2*>(A.part_ml + 2 * (int64_t(part) * kRows + r)) = make_float2(top, sum);
+                }
             }
         }
-    }
-    if (!A.part_o) {
-        return;
-    }
-    __syncthreads(); // the ring is free again
-    if (++head == H) {
-        head = 0, tile++;
-    }
+        if (!A.part_o) {
+            return;
+        }
+        __syncthreads(); // the ring is free again
+        if (++head == H) {
+            head = 0, tile++;
+        }
     }
     if (A.part_o && threadIdx.x == 0) {
         A.splits[blockIdx.x] = split;

@@ -251,7 +251,17 @@ cudaError_t launch_append(cudaStream_t st, const AppendArgs& a, bool pages, int 
             }
         };
         if (pages) {
-            return a.rotation.adjacent ? of_dim(std::true_type{}) : of_dim(std::false_type{});
+            const cudaError_t e = a.rotation.adjacent ? of_dim(std::true_type{}) : of_dim(std::false_type{});
+            if (e || !a.apart) {
+                return e;
+            }
+            cudaLaunchConfig_t cfg{};
+            cudaLaunchAttribute beside;
+            beside.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            beside.val.programmaticStreamSerializationAllowed = 1;
+            cfg.gridDim = dim3(a.apart), cfg.blockDim = dim3(kRotaryThreads), cfg.dynamicSmemBytes = rotary_smem(a.rotation, kRotaryThreads), cfg.stream = st;
+            cfg.attrs = &beside, cfg.numAttrs = 1;
+            return a.rotation.adjacent ? cudaLaunchKernelEx(&cfg, query_kernel<T, true>, a) : cudaLaunchKernelEx(&cfg, query_kernel<T, false>, a);
         }
     }
     constexpr int kMost = 16 / sizeof(T);
@@ -276,7 +286,9 @@ struct Plan {
 Plan make_plan(const cck_cache& c, const cck_batch& b, int q_heads, int sms) {
     Plan p{};
     const int64_t rows = int64_t(b.max_new < b.rows ? b.max_new : b.rows) * (q_heads / c.heads);
-    p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 0;
+    // up to 24 rows by warps of their own, 17 and more in two passes over the keys, the second from L2: 49 | 54 us against the tile kernel at 20 rows, 62 | 54 at
+    // 32 (16 sequences of up to 4096, 8 heads of 128)
+    p.nt = rows <= 8 ? 1 : rows <= 24 ? 2 : 0;
     p.granule = p.nt ? granule_of(c.dim) : kTileKeys, p.tile_rows = p.nt ? 8 * p.nt : kUnitRows;
     const int64_t row_tiles = (rows + p.tile_rows - 1) / p.tile_rows, tiles = b.sequences * row_tiles; // below 2^31 * 2^43 / 2^3
     if (rows > kMostTokens || tiles * c.heads > 0x7fffffff) {
@@ -287,7 +299,10 @@ Plan make_plan(const cck_cache& c, const cck_batch& b, int q_heads, int sms) {
     const int64_t units = tiles * c.heads, slots = (p.nt == 0 ? 1 : p.nt == 1 ? 3 : 2) * sms;
     const int64_t granules = int64_t(b.max_len) / p.granule + 2;
     const int least = p.nt ? 2 * kDecodeWarps : 2; // granules of a share
-    p.shares = granules > (p.nt ? 4 : 2) * least && units < 8 * slots;
+    // Shares cost a launch and the way through the workspace, whole units leave multiprocessors idle. us whole | in shares, 8 heads of 128, one token: 1000 keys
+    // 13 | 16, 1500 15 | 15, 3000 27 | 15; 64 sequences of 700 29 | 32, of 2048 52 | 48; 256 rows: 512 keys 23 | 28, 1024 25 | 25. Of very many units the
+    // last ones hardly show (1000 sequences of 2048: 511 | 549).
+    p.shares = granules > (p.nt ? 6 : 5) * least && units < 8 * slots;
     const int64_t most = (units * granules + least - 1) / least;
     p.blocks = !p.shares ? units : most < slots ? most : slots;
     p.blocks = p.shares && p.blocks > kMostShares ? kMostShares : p.blocks;
@@ -454,7 +469,12 @@ int cck_cache_append(void* stream, const cck_cache* cache, const cck_batch* batc
         const size_t rows = append_smem(most, D, size_of(k->dtype));
         smem = rows > smem ? rows : smem;
     }
-    if (vec) {
+    if (vec && pages && units && batch->rows >= 32 * sms) {
+        // a launch of their own for queries that fill the GPU: 55 -> 49 us for eight prompts of about 900 tokens, 32 heads of 128; with 2000 rows of
+        // 20 heads of 64 it took 19 us instead of 16
+        a.apart = int(rotary_blocks(a.q, kRotaryThreads, sms));
+    }
+    if (vec && !a.apart) {
         const int threads = pages && a.group_threads > kAppendThreads ? a.group_threads : kAppendThreads;
         more = rotary_blocks(a.q, threads, sms);
         smem = more && rotary_smem(*rotation, threads) > smem ? rotary_smem(*rotation, threads) : smem;

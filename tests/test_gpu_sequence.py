@@ -434,6 +434,43 @@ def test_append_leaves_rows_of_nobody(seq, rng, dtype, offset):
     assert all(torch.equal(a, b) for a, b in zip(codes, again.views())) and torch.equal(cache.ks, again.ks)
 
 
+@pytest.mark.parametrize("adjacent", [False, True])
+def test_append_many_queries(seq, rng, adjacent):
+    """Queries that get a launch of their own: as rotated alone, keys as appended alone, what is behind them stays; in a graph too."""
+    new = [2000, 1, 2900, 500]
+    batch = Batch(seq, new, [2000, 90, 3000, 517], 64, rng, rows=sum(new) + 30)
+    k, v = (torch.randn(batch.rows, 2, 64, device="cuda", generator=rng).bfloat16() for _ in range(2))
+    q = torch.randn(batch.rows, 6, 64, device="cuda", generator=rng).bfloat16()
+    pos = torch.randint(0, 5000, (1, batch.rows), device="cuda", generator=rng, dtype=torch.int32)
+    freq = torch.rand(32, device="cuda", generator=rng)
+    r = seq.Rotation(64, [32], freq.data_ptr(), pos.data_ptr(), adjacent=adjacent)
+    caches = []
+    for _ in range(2):
+        caches.append(Cache(seq, batch.pages, 64, 2, 64, fill=0))
+        caches[-1].ks.fill_(1.0), caches[-1].vs.fill_(1.0)
+    want, out = torch.full_like(q, 5.0), torch.full_like(q, 5.0)
+    seq.rotary(stream(), r, sum(new), 64, rows_of(seq, q), rows_of(seq, want))
+    seq.cache_append(stream(), caches[0].desc, batch.desc, rows_of(seq, k), rows_of(seq, v), r)
+    seq.cache_append(stream(), caches[1].desc, batch.desc, rows_of(seq, k), rows_of(seq, v), r, rows_of(seq, q), rows_of(seq, out))
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    same = lambda: all(torch.equal(getattr(caches[0], n), getattr(caches[1], n)) for n in ("k", "v", "ks", "vs"))  # noqa: E731
+    assert same()
+    for x in (caches[1].k, caches[1].v, caches[1].ks, caches[1].vs):
+        x.fill_(1)
+    for c in caches:
+        c.k.zero_(), c.v.zero_(), c.ks.fill_(1.0), c.vs.fill_(1.0)
+    seq.cache_append(stream(), caches[0].desc, batch.desc, rows_of(seq, k), rows_of(seq, v), r)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out.fill_(7.0)
+        seq.cache_append(stream(), caches[1].desc, batch.desc, rows_of(seq, k), rows_of(seq, v), r, rows_of(seq, q), rows_of(seq, out))
+        copy = out.clone()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(copy[: sum(new)], want[: sum(new)]) and (copy[sum(new) :] == 7.0).all() and same()
+
+
 @pytest.mark.parametrize("length", [(1 << 31) - 1, (1 << 30) + 1, -5, -(1 << 31)])
 def test_append_length_that_cannot_be(seq, rng, length):
     batch = Batch(seq, [3, 3], [40, 20], 32, rng)
@@ -524,6 +561,7 @@ ATTENTION = [
     ([1], [1], 16, 1, 1, 32), ([1], [700], 16, 8, 4, 128), ([1, 1, 1], [33, 0, 64], 32, 2, 8, 64), ([1, 0, 1], [129, 50, 31], 64, 3, 3, 96), ([2, 1, 5], [2, 300, 77], 128, 2, 7, 128),
     ([5, 5], [4000, 5], 32, 5, 1, 64), ([1], [9001], 128, 2, 16, 128), ([3, 9], [200, 1500], 64, 1, 20, 96), ([40, 1, 0, 17], [100, 5000, 9, 17], 64, 2, 4, 128),
     ([130, 61], [130, 700], 16, 2, 2, 64), ([257], [1025], 64, 1, 3, 128), ([300, 7], [300, 4096], 32, 2, 5, 32), ([3, 4], [2, 0], 16, 2, 2, 64),
+    ([5, 5], [300, 4000], 32, 2, 4, 64), ([3, 1, 0, 2], [900, 40, 7, 2], 64, 3, 8, 128), ([1, 1], [5000, 33], 16, 1, 17, 96),
 ]  # fmt: skip
 
 
