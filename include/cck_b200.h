@@ -143,7 +143,8 @@ int cck_cache_append(void* stream, const cck_cache* cache, const cck_batch* batc
                      const cck_rotation* rotation, const cck_rows* q, const cck_rows* q_out, int32_t* status);
 
 /* out = softmax(softmax_scale * q K^T) V over the cache, for the batch's rows; q heads are a multiple of the cache's heads (head j
- * reads cache head j / (q heads / heads)); q and out are bf16 or f16, both the same, data and strides multiples of 16 bytes.
+ * reads cache head j / (q heads / heads)); q and out are bf16 or f16, both the same, data and strides multiples of 16 bytes. out may be
+ * q (same data and strides); otherwise they do not overlap.
  * Row i of n of sequence b stands at place len[b]-n+i. causal: it sees places up to its own, else all len[b]; window > 0: of
  * those only the ones later than its place - window. A row that sees nothing gives 0, and -inf in lse. lse (may be null):
  * f32 [rows][q heads], the natural log of the sum of exponentials. Scores, maxima, sums and outputs are accumulated in f32. q is

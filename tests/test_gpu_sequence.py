@@ -886,6 +886,39 @@ def test_two_streams_and_two_graphs(seq, rng, new):
             assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("new, heads, group, dim", [([1, 1, 1], 2, 4, 128), ([5, 1, 3], 1, 4, 64), ([150, 40, 300], 2, 2, 64)])
+def test_in_place_and_replayed_with_other_lengths(seq, rng, new, heads, group, dim):
+    """Queries overwritten by the answer, and a captured call whose sequences' lengths and rows have changed since, both cut into shares."""
+    most = [5000, 3000, 7000]
+    batch = Batch(seq, new, most, 32, rng)
+    cache = Cache(seq, batch.pages, 32, heads, dim).random(rng)
+    q = torch.randn(batch.rows, heads * group, dim, device="cuda", generator=rng).bfloat16()
+    need = seq.cache_attention_workspace_bytes(cache.desc, batch.desc, heads * group)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    assert need > 0
+
+    def attend(out):
+        seq.cache_attention(stream(), cache.desc, batch.desc, rows_of(seq, q if out is not place else place), rows_of(seq, out), 0.1, ws.data_ptr(), need)
+
+    place, out = q.clone(), torch.empty_like(q)
+    attend(out), attend(place)
+    assert torch.equal(out, place)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        attend(out)
+    for lens, rows in (([700, 3000, 20], new), ([0, 17, 6999], [0, 1, new[2]]), ([5000, 1, 1], [new[0], 1, 0])):
+        batch.len.copy_(i32(lens)), batch.first.copy_(i32([0, rows[0], rows[0] + rows[1], sum(rows)]))
+        out.fill_(5.0)
+        graph.replay()
+        replayed = out.clone()
+        out.fill_(5.0)
+        attend(out)
+        torch.cuda.synchronize()
+        assert torch.equal(replayed, out)
+        batch.new, batch.lens = rows, lens
+        check_attention(seq, cache, batch, q, "bf16", scale=0.1)
+
+
 def test_same_result_every_time(seq, rng):
     batch = Batch(seq, [1, 2, 150], [5000, 40, 900], 32, rng)
     cache = Cache(seq, batch.pages, 32, 2, 128).random(rng)
