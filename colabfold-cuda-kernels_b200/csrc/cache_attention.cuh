@@ -599,7 +599,10 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DecodeShape<D, NT>::kBlocks
         if (!A.part_o) {
             return;
         }
-        __syncthreads(); // the ring is free again
+        // The ring is free again for the next unit's copies, which write through the async proxy what was written and read here by ordinary
+        // stores and loads: those are ordered before them by each thread's fence and the barrier
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();
         if (++head == H) {
             head = 0, tile++;
         }
