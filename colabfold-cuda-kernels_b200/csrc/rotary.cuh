@@ -38,18 +38,22 @@ __device__ __forceinline__ Turns turns_of(float freq) {
     return {f < 1.0 ? __double2ull_rn(f * 18446744073709551616.0) : 0, freq - freq == 0.f};
 }
 // The nearest quarter turn is taken off in integers; what is left, at most pi / 4, goes through the Taylor series of sine and cosine about
-// zero to the ninth and tenth power (the terms after them are below 2e-9 of the result). It is held in two floats, x + e, and the last
-// additions carry what they round off, so that both come out as exact as rounded once (0.29 of the last place, root mean square). Keys turned with
-// them are rounded to 4 bits: of 12 batches of 2000 rows of 20 heads of 64, 31 codes are not the ones of 64 bits; 48 were with an angle of one
-// float and three roundings in rotate(), in the same time.
+// zero to the ninth and tenth power (the terms after them are below 2e-9 of the result). It is held in two floats, x + e, down to 2^-58 of a turn,
+// so that a small angle keeps its digits, and the last additions carry what they round off: both come out within a few units of the last place of
+// themselves, however small the sine is, as far as the angle itself is known (2^-52 of position times frequency). Keys turned with them are rounded to 4
+// bits: of 12 batches of 2000 rows of 20 heads of 64, 31 codes are not the ones of 64 bits. With 2^-32 of a turn it took the same time, and a sine of 1e-4
+// was off by 1e-5 of itself.
 __device__ __forceinline__ float2 cos_sin(int pos, Turns t) {
-    const int32_t angle = int32_t((t.per * uint64_t(int64_t(pos))) >> 32);     // of a turn, in 2^-32
-    const int32_t quarter = int32_t(uint32_t(angle) + 0x20000000u) >> 30;       // -2 .. 1
-    const int32_t rest = int32_t(uint32_t(angle) - (uint32_t(quarter) << 30));  // at most 2^29 either way
+    const uint64_t angle = t.per * uint64_t(int64_t(pos)); // of a turn, in 2^-64
+    const uint32_t top = uint32_t(angle >> 32);
+    const int32_t quarter = int32_t(top + 0x20000000u) >> 30;          // -2 .. 1
+    const int32_t rest = int32_t(top - (uint32_t(quarter) << 30));     // at most 2^29 either way
+    const int32_t coarse = (rest + 32) & ~63;                          // 24 bits; the other 38, in 2^-58 of a turn, are 32 with a sign
+    const int32_t fine = int32_t(__funnelshift_r(uint32_t(angle), uint32_t(rest - coarse), 6));
     constexpr double kUnit = 6.283185307179586477 / 4294967296.0;
-    constexpr float kHigh = float(kUnit), kLow = float(kUnit - double(kHigh));
-    const float high = __int2float_rn(rest & ~63), low = __int2float_rn(rest & 63); // both exact
-    const float x = high * kHigh, e = fmaf(high, kHigh, -x) + fmaf(high, kLow, low * kHigh);
+    constexpr float kHigh = float(kUnit), kLow = float(kUnit - double(kHigh)), kFine = float(kUnit / 67108864.0);
+    const float high = __int2float_rn(coarse), low = __int2float_rn(fine); // the first is exact
+    const float x = high * kHigh, e = fmaf(high, kHigh, -x) + fmaf(high, kLow, low * kFine);
     const float y = x * x, z = fmaf(x, x, -y);
     float s = fmaf(y, 1.f / 362880.f, -1.f / 5040.f), c = fmaf(y, -1.f / 3628800.f, 1.f / 40320.f);
     s = fmaf(y, s, 1.f / 120.f), c = fmaf(y, c, -1.f / 720.f);
