@@ -49,6 +49,7 @@ struct AttentionArgs {
     int reach; // tokens that a row of the table has pages for
     int granule_shift, page_shift; // keys of a step and tokens of a page are powers of two
     int unit_cost;
+    int lose; // test door: the barriers of this block's first copies wait for an arrival that nobody makes; -1: none
     int tile_rows, row_tiles; // a sequence's rows times heads of a group, cut into tiles: `tiles` are those of all sequences, row_tiles each
     // shares of units that several blocks work on: sums [2 blocks][tile rows][dim], reference and sum [..][2]; null: a block takes a unit
     float *part_o, *part_ml;
@@ -258,23 +259,43 @@ __device__ __noinline__ void clear_values(uint32_t v, int lo, int hi, uint32_t a
     __syncwarp();
 }
 
+// A warp whose copy got lost: says so for the rest of the block's share and waits for its other copies, as long as they can take, so that none lands
+// where somebody else has gone on
+__device__ __noinline__ void give_up(int* lost, uint32_t bars, int slot, int phase, int others, int stages) {
+    if ((threadIdx.x & 31) == 0) {
+        *lost = 1;
+    }
+#pragma unroll 1
+    for (int i = 0; i < others; i++) {
+        if (++slot == stages) {
+            slot = 0, phase ^= 1;
+        }
+        bar_wait(bars + slot * 8, phase, kDrainTries);
+    }
+    __syncwarp();
+}
+
 template <class T, int D, int NT>
 __global__ void __launch_bounds__(kDecodeWarps * 32, DecodeShape<D, NT>::kBlocks) decode_kernel(const __grid_constant__ AttentionArgs A) {
     using S = DecodeShape<D, NT>;
     constexpr int kTerms = kTermsOf<T>;
     constexpr int kRows = 8 * NT, kTiles = S::kKeys / 16, kKeysShift = S::kKeys == 64 ? 6 : 5; // kTiles: of 16 keys
     extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ int4 lost; // a word for each warp, written by itself and read by all between the barriers of a unit's end
+    static_assert(kDecodeWarps == 4, "words of lost");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n8 = lane >> 2, c4 = lane & 3;
     const int H = A.cache.heads, G = A.group;
     const uint32_t ring = shared_u32(smem) + warp * S::kStages * S::kStage;
     const uint32_t bars = shared_u32(smem) + S::kRing + warp * S::kStages * 8;
     if (lane == 0) {
         for (int i = 0; i < S::kStages; i++) {
-            bar_init(bars + 8 * i, 1);
+            bar_init(bars + 8 * i, warp == 0 && int(blockIdx.x) == A.lose ? 2 : 1);
         }
         bar_init_done();
+        reinterpret_cast<int*>(&lost)[warp] = 0;
     }
     __syncwarp();
+    bool gone = false; // a copy of this block got lost: the rest of its share is NaN, nothing is copied or waited for any more
     // what is left of this block's share, and where it is: tile, head, granules done of the unit
     int64_t left = 1, done = 0, size = 0, at = 0; // at: on the line
     int tile = blockIdx.x / H, head = blockIdx.x % H;
@@ -318,7 +339,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DecodeShape<D, NT>::kBlocks
 
         // this warp's granules: ga + warp, + kDecodeWarps, ...; a granule is one piece of a page, or several of small pages. A lane looks
         // one piece up, so that 32 are known at a time: `now` for the granule worked on, `next` for copies ahead of it
-        const int mine = max(0, ceil_div(gb - ga - warp, kDecodeWarps));
+        const int mine = gone ? 0 : max(0, ceil_div(gb - ga - warp, kDecodeWarps));
         const int piece_shift = min(A.page_shift, kKeysShift), pieces_shift = kKeysShift - piece_shift, pieces = 1 << pieces_shift;
         auto look_up = [&](int first) {
             const int j = first + lane, key = (ga + warp + (j >> pieces_shift) * kDecodeWarps) * S::kKeys + ((j & (pieces - 1)) << piece_shift);
@@ -432,11 +453,8 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DecodeShape<D, NT>::kBlocks
             }
             const uint32_t st = ring + slot * S::kStage;
             const int key0 = (ga + warp + i * kDecodeWarps) * S::kKeys;
-            if (!bar_wait(bars + slot * 8, phase)) {
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    l[t][0] = l[t][1] = __int_as_float(0x7fffffff); // a copy got lost: rows come out as NaN
-                }
+            if (!__all_sync(0xffffffffu, bar_wait(bars + slot * 8, phase))) {
+                give_up(reinterpret_cast<int*>(&lost) + warp, bars, slot, phase, min(mine - i, S::kStages) - 1, S::kStages);
                 break;
             }
             float x[kTiles][NT][4] = {};
@@ -570,6 +588,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DecodeShape<D, NT>::kBlocks
             }
         }
         __syncthreads();
+        gone = lost.x | lost.y | lost.z | lost.w;
         constexpr int kLanes = D / 4; // threads of a row, four dims each
 #pragma unroll 1
         for (int i = threadIdx.x; i < own.rows * kLanes; i += kDecodeWarps * 32) {
@@ -587,6 +606,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DecodeShape<D, NT>::kBlocks
                 sum = fmaf(sm[2 * (w * kRows + r) + 1], f, sum);
                 y.x = fmaf(z.x, f, y.x), y.y = fmaf(z.y, f, y.y), y.z = fmaf(z.z, f, y.z), y.w = fmaf(z.w, f, y.w);
             }
+            sum = gone ? __int_as_float(0x7fffffff) : sum; // which makes the row NaN, here or when its shares are joined
             if (alone) {
                 store_out<T>(A, s.row0 + (r0 + r) / G, head * G + (r0 + r) % G, d, y, top, sum);
             } else {

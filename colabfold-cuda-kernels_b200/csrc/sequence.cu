@@ -15,6 +15,7 @@ using namespace cck::seq;
 namespace {
 
 constexpr int kMaxDevices = 64;
+std::atomic<int> g_lose{-1}; // cck_set_lost_copy_test
 
 int refuse(int code, const char* op, const char* what) {
     char text[256];
@@ -547,13 +548,17 @@ int cck_cache_attention(void* stream, const cck_cache* cache, const cck_batch* b
     const int64_t reach = int64_t(batch->table_pages) * cache->page_tokens;
     a.reach = int(reach < kMostTokens ? reach : kMostTokens);
     a.granule_shift = __builtin_ctz(p.granule), a.unit_cost = p.nt ? 8 : 3, a.page_shift = __builtin_ctz(cache->page_tokens);
-    a.tile_rows = p.tile_rows, a.row_tiles = p.row_tiles;
+    a.tile_rows = p.tile_rows, a.row_tiles = p.row_tiles, a.lose = g_lose.load(std::memory_order_relaxed);
     if (p.shares) {
         a.part_o = static_cast<float*>(ws), a.part_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + p.part_bytes);
         a.splits = reinterpret_cast<Split*>(static_cast<char*>(ws) + p.part_bytes + p.ml_bytes);
     }
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     return launched(op, q->dtype == CCK_BF16 ? launch_attention<__nv_bfloat16>(st, a, p) : launch_attention<__half>(st, a, p));
+}
+
+void cck_set_lost_copy_test(int block) {
+    g_lose.store(block, std::memory_order_relaxed);
 }
 
 } // extern "C"

@@ -205,10 +205,11 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(__cvta_generic_to_global(src)), "r"(bytes), "r"(bar)
                  : "memory");
 }
-// Waits for the phase with this parity; gives up (false) after about a second, which nothing but a lost copy can cause.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+// Waits for the phase with this parity; gives up (false) after about a second, which nothing but a lost copy can cause, or after `tries` times 4 us.
+constexpr int kWaitTries = 1 << 18, kDrainTries = 1 << 12; // kDrainTries: for copies that are on their way when another one got lost
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, int tries = kWaitTries) {
 #pragma unroll 1
-    for (int i = 0; i < 1 << 18; i++) {
+    for (int i = 0; i < tries; i++) {
         uint32_t ok;
         asm volatile(
             "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"

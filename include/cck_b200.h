@@ -158,6 +158,10 @@ size_t cck_cache_attention_workspace_bytes(const cck_cache* cache, const cck_bat
 int cck_cache_attention(void* stream, const cck_cache* cache, const cck_batch* batch, const cck_rows* q, const cck_rows* out, float* lse,
                         float softmax_scale, int causal, int window, void* ws, size_t ws_bytes);
 
+/* Test door: in the calls of cck_cache_attention that follow, the copies of the first warp that makes any in this block of threads never count
+ * as done. Its wait gives up after about a second, and the rows of that block's share from there on are NaN. -1 restores production. */
+void cck_set_lost_copy_test(int block);
+
 /* Workspace size for a shape bucket; 0 if the sizes do not describe a supported model
  * (src/diffusion/host.cuh:376-379). */
 size_t mk_workspace_bytes(int S, int Nb, int NSb, int nsteps, int flags, const size_t* bytes);

@@ -49,3 +49,67 @@ def test_small_sines_have_their_digits(seq, rng, far, freq, adjacent):  # noqa: 
     for got, want in ((y[:, 0, a], angle.cos()), (y[:, 0, b], angle.sin())):
         err = (got.double() - want).abs()
         assert (err <= 10 * 2.0**-24 * want.abs() + off).all(), (err / (2.0**-24 * want.abs() + off)).max().item()
+
+
+@pytest.fixture
+def lose(seq):  # noqa: F811
+    """Lets a copy of one block of threads never count as done, for the calls of a test."""
+    set_block = seq._lib.cck_set_lost_copy_test
+    set_block.restype = None
+    yield set_block
+    set_block(-1)
+
+
+def attend(seq, cache, batch, q, out, lse):  # noqa: F811
+    need = seq.cache_attention_workspace_bytes(cache.desc, batch.desc, q.shape[1])
+    ws = torch.full((need + 16,), 0, dtype=torch.uint8, device="cuda")  # sums of zero, were slots not written
+    seq.cache_attention(stream(), cache.desc, batch.desc, rows_of(seq, q), rows_of(seq, out), 0.1, ws.data_ptr(), need, lse=lse.data_ptr())
+    torch.cuda.synchronize()
+
+
+def lost_rows(seq, cache, batch, q, lose, block):  # noqa: F811
+    """(row, head) that are NaN when a copy of this block gets lost; all others, and all in the next call, are as they were."""
+    want, lse = torch.empty_like(q), torch.empty(q.shape[:2], device="cuda")
+    attend(seq, cache, batch, q, want, lse)
+    assert not want.isnan().any()
+    out, lost_lse = torch.full_like(q, 5.0), torch.full_like(lse, 5.0)
+    for places in range(2):  # apart, and the answer in the queries' place
+        x = out if places == 0 else q.clone()
+        lose(block)
+        attend(seq, cache, batch, q if places == 0 else x, x, lost_lse)
+        lose(-1)
+        gone = lost_lse.isnan()
+        assert torch.equal(gone, x.isnan().any(-1)) and torch.equal(gone, x.isnan().all(-1))
+        assert torch.equal(x[~gone], want[~gone]) and torch.equal(lost_lse[~gone], lse[~gone])
+    again = torch.empty_like(q)
+    attend(seq, cache, batch, q, again, lost_lse)
+    assert torch.equal(again, want)
+    return gone
+
+
+@pytest.mark.parametrize("group, new", [(1, 1), (5, 2)])
+def test_lost_copy_few_rows(seq, rng, lose, group, new):  # noqa: F811
+    """A wait that gives up makes the rows NaN that the rest of the block's share has a part of, and no other."""
+    sequences, heads = 125, 16
+    lens = torch.randint(40, 160, (sequences,), generator=rng, device="cuda").tolist()
+    batch = Batch(seq, [new] * sequences, lens, 32, rng)
+    cache = Cache(seq, batch.pages, 32, heads, 64).random(rng)
+    q = torch.randn(batch.rows, heads * group, 64, device="cuda", generator=rng).bfloat16()
+    whole = lost_rows(seq, cache, batch, q, lose, 23)  # a block for each (sequence, head): sequence 1, head 7
+    want = torch.zeros_like(whole)
+    want[new : 2 * new, 7 * group : 8 * group] = True
+    assert torch.equal(whole, want)
+    batch.desc.max_len = 4000  # equal shares of 4 units and more
+    gone = lost_rows(seq, cache, batch, q, lose, 100)
+    units = gone.view(sequences, new, heads, group).any(3).any(1).flatten()  # in the order of the line
+    assert torch.equal(units, gone.view(sequences, new, heads, group).all(3).all(1).flatten())
+    first, last, count = units.nonzero().min().item(), units.nonzero().max().item(), units.sum().item()
+    assert count == last - first + 1 and 4 <= count <= 12
+
+
+def test_lost_copy_of_one_long_sequence(seq, rng, lose):  # noqa: F811
+    batch = Batch(seq, [1], [30000], 64, rng)
+    cache = Cache(seq, batch.pages, 64, 2, 128).random(rng)
+    q = torch.randn(1, 8, 128, device="cuda", generator=rng).bfloat16()
+    gone = lost_rows(seq, cache, batch, q, lose, 3)  # of the first head's shares
+    assert gone[0].tolist() == [True] * 4 + [False] * 4
