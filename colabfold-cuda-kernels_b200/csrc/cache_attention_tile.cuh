@@ -58,6 +58,7 @@ struct TileCtl {
     uint64_t q_full[2], k_full[3], k_empty[3], v_full[2], v_empty[2], h_full[2], h_empty[2];
     uint64_t s_full[2][2], p_full[2][2], o_done[2][2]; // [tile][buffer of S]
     uint64_t seg_full[kSegments], seg_empty[kSegments];
+    uint64_t drained[4]; // the products of a warp that gave up: S of tile 0 and 1, p V of tile 0 and 1
     Segment seg[kSegments];
     TileScale scale[kScaleSlots][kTileKeys / 16];
     uint32_t absent[kScaleSlots]; // a bit for each 16 keys whose page is not there, or that nobody sees
@@ -66,10 +67,11 @@ struct TileCtl {
 };
 static_assert(sizeof(TileCtl) <= kCtlBytes, "control block");
 
-// A wait that gives up after about a second, which nothing but a lost copy can cause; then every later one returns at once
+// A wait that gives up after about a second, which nothing but a lost copy can cause; then every later one of the block returns at once: the
+// roles run to the end of their segment on whatever is there, nothing is copied any more, and the block's whole share becomes NaN (give_up_share)
 __device__ __forceinline__ void tile_wait(uint32_t b, uint32_t parity, volatile int* abort) {
 #pragma unroll 1
-    for (int i = 0; i < 1 << 18; i++) {
+    for (int i = 0; i < kWaitTries; i++) {
         uint32_t ok;
         asm volatile(
             "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
@@ -87,6 +89,9 @@ __device__ __forceinline__ void tile_wait(uint32_t b, uint32_t parity, volatile 
 }
 __device__ __forceinline__ void tile_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
     tile_wait(shared_u32(bar), parity, abort);
+}
+__device__ __forceinline__ bool gave_up(TileCtl* ctl) { // a whole warp calls
+    return __any_sync(0xffffffffu, *static_cast<volatile int*>(&ctl->abort));
 }
 // position in a ring
 template <int N>
@@ -225,7 +230,7 @@ __device__ __forceinline__ bool next_segment(TileCtl* ctl, Ring<kSegments>& r, S
         bar_arrive(shared_u32(&ctl->seg_empty[r.i]));
     }
     r.next();
-    return g.gb > g.ga && !*static_cast<volatile int*>(&ctl->abort);
+    return g.gb > g.ga && !gave_up(ctl);
 }
 
 template <class T, int D>
@@ -418,55 +423,103 @@ __device__ __forceinline__ void tile_softmax(const AttentionArgs& A, unsigned ch
     }
 }
 
+// A block's way through its share of the line, or its one unit: those of the last rows, which see the most keys, come first
+struct Walk {
+    int64_t left, done, size, at; // at: on the line
+    int tile, head;
+    Split split;
+};
+__device__ __forceinline__ Walk walk_from_start(const AttentionArgs& A) { // a whole warp calls
+    const int H = A.cache.heads;
+    Walk w{1, 0, 0, 0, int(A.batch.sequences * A.row_tiles - 1 - blockIdx.x / H), int(blockIdx.x % H), {0, 0, int(blockIdx.x), 0}};
+    if (A.part_o) {
+        const Line line = line_of(A, blockIdx.x, gridDim.x);
+        w.left = line.left, w.size = line.size, w.at = line.size * blockIdx.x, w.tile = line.tile;
+        if (w.left > 0) {
+            const int g = weight_of(A, w.tile);
+            w.head = int((w.at - line.start) / g), w.done = w.at - line.start - int64_t(w.head) * g;
+        }
+    }
+    return w;
+}
+// the next unit, or part of one, and its sequence; false: there is none
+__device__ __forceinline__ bool next_unit(const AttentionArgs& A, Walk& w, Segment& g, int& b) {
+    g = Segment{}, b = 0;
+    while (w.left > 0) {
+        const Tile own = tile_at(A, w.tile);
+        if (own.rows == 0) {
+            w.left = A.part_o ? w.left : 0;
+            w.tile++, w.head = 0;
+            continue;
+        }
+        const TileKeys keys = keys_of_tile(A, own.s, own.r0, own.r0 + own.rows);
+        const int all = max(1, keys.g1 - keys.g0);
+        // what of the unit's stretch of the line is the share's, without the cost at its head
+        const int64_t to = A.part_o ? min(int64_t(all + A.unit_cost), w.done + w.left) : all + A.unit_cost, unit_at = w.at - w.done;
+        const int ga = max(0, int(w.done) - A.unit_cost), gb = max(0, int(to) - A.unit_cost);
+        w.left = A.part_o ? w.left - (to - w.done) : 0, w.at = unit_at + to, w.done = 0;
+        b = A.row_tiles == 1 ? w.tile : w.tile / A.row_tiles;
+        g.head = w.head, g.r0 = own.r0, g.rows = own.rows, g.row0 = own.s.row0, g.place0 = own.s.place0, g.len = own.s.len, g.lo = keys.lo, g.hi = keys.hi;
+        g.ga = keys.g0 + ga, g.gb = keys.g0 + gb;
+        g.part = gb - ga == all ? -1 : 2 * int(blockIdx.x) + (ga == 0 ? 1 : 0);
+        if (A.part_o && ga == 0 && gb > 0 && gb < all) {
+            w.split.tile = w.tile, w.split.head = w.head, w.split.last = int((unit_at + all + A.unit_cost - 1) / w.size);
+        }
+        if (++w.head == A.cache.heads) {
+            w.head = 0, w.tile++;
+        }
+        break;
+    }
+    return g.gb > g.ga;
+}
+
+// NaN for every row of the block's share, in the result or in its part of the workspace; all threads call, when all roles have ended
+template <class T, int D>
+__device__ __noinline__ void give_up_share(const AttentionArgs& A) {
+    const float nan = __int_as_float(0x7fffffff);
+    Walk w = walk_from_start(A);
+    Segment g;
+    int b;
+#pragma unroll 1
+    while (next_unit(A, w, g, b)) {
+#pragma unroll 1
+        for (int r = threadIdx.x; r < g.rows; r += kTileThreads) {
+            const int64_t row = g.row0 + (g.r0 + r) / A.group;
+            const int head = g.head * A.group + (g.r0 + r) % A.group;
+            if (g.part >= 0) {
+                *reinterpret_cast<float2*>(A.part_ml + 2 * (int64_t(g.part) * kUnitRows + r)) = make_float2(0.f, nan);
+                continue;
+            }
+            T* y = static_cast<T*>(A.out) + row * A.or_ + head * A.oh;
+#pragma unroll 1
+            for (int d = 0; d < D; d++) {
+                y[d] = from_f32<T>(nan);
+            }
+            if (A.lse) {
+                A.lse[row * A.q_heads + head] = nan;
+            }
+        }
+    }
+    if (A.part_o && threadIdx.x == 0) {
+        A.splits[blockIdx.x] = w.split;
+    }
+}
+
 template <class T, int D>
 __device__ __forceinline__ void tile_load(const AttentionArgs& A, unsigned char* smem, TileCtl* ctl) {
     using S = TileShape<T, D>;
-    const int lane = threadIdx.x & 31, H = A.cache.heads;
+    const int lane = threadIdx.x & 31;
     uint32_t step = 0;
     Ring<S::kKStages> kr;
     Ring<S::kVStages> vr;
     Ring<kSegments> segments;
-    // the block's share, or its unit: those of the last rows, which see the most keys, come first
-    int64_t left = 1, done = 0, size = 0, at = 0; // at: on the line
-    int tile = A.batch.sequences * A.row_tiles - 1 - blockIdx.x / H, head = blockIdx.x % H;
-    Split split{0, 0, int(blockIdx.x), 0};
-    if (A.part_o) {
-        const Line line = line_of(A, blockIdx.x, gridDim.x);
-        left = line.left, size = line.size, at = size * blockIdx.x, tile = line.tile;
-        if (left > 0) {
-            const int g = weight_of(A, tile);
-            head = int((at - line.start) / g), done = at - line.start - int64_t(head) * g;
-        }
-    }
+    Walk walk = walk_from_start(A);
+    bool stop = false;
 #pragma unroll 1
-    while (true) {
-        Segment g{};
-        int b = 0;
-        while (left > 0) {
-            const Tile own = tile_at(A, tile);
-            if (own.rows == 0) {
-                left = A.part_o ? left : 0;
-                tile++, head = 0;
-                continue;
-            }
-            const TileKeys keys = keys_of_tile(A, own.s, own.r0, own.r0 + own.rows);
-            const int all = max(1, keys.g1 - keys.g0);
-            // what of the unit's stretch of the line is the share's, without the cost at its head
-            const int64_t to = A.part_o ? min(int64_t(all + A.unit_cost), done + left) : all + A.unit_cost, unit_at = at - done;
-            const int ga = max(0, int(done) - A.unit_cost), gb = max(0, int(to) - A.unit_cost);
-            left = A.part_o ? left - (to - done) : 0, at = unit_at + to, done = 0;
-            b = A.row_tiles == 1 ? tile : tile / A.row_tiles;
-            g.head = head, g.r0 = own.r0, g.rows = own.rows, g.row0 = own.s.row0, g.place0 = own.s.place0, g.len = own.s.len, g.lo = keys.lo, g.hi = keys.hi;
-            g.ga = keys.g0 + ga, g.gb = keys.g0 + gb;
-            g.part = gb - ga == all ? -1 : 2 * int(blockIdx.x) + (ga == 0 ? 1 : 0);
-            if (A.part_o && ga == 0 && gb > 0 && gb < all) {
-                split.tile = tile, split.head = head, split.last = int((unit_at + all + A.unit_cost - 1) / size);
-            }
-            if (++head == H) {
-                head = 0, tile++;
-            }
-            break;
-        }
+    while (!stop) {
+        Segment g;
+        int b;
+        const bool more = next_unit(A, walk, g, b);
         tile_wait(&ctl->seg_empty[segments.i], segments.phase ^ 1, &ctl->abort);
         if (lane == 0) {
             ctl->seg[segments.i] = g;
@@ -474,7 +527,7 @@ __device__ __forceinline__ void tile_load(const AttentionArgs& A, unsigned char*
         }
         segments.next();
         const int n = g.gb - g.ga;
-        if (n == 0 || *static_cast<volatile int*>(&ctl->abort)) {
+        if (!more || gave_up(ctl)) {
             break;
         }
         // a lane looks 16 keys up, 8 lanes a tile, four tiles at a time
@@ -496,6 +549,10 @@ __device__ __forceinline__ void tile_load(const AttentionArgs& A, unsigned char*
             const bool leads = in_page && mine == group + __ffs(in_page) - 1 && lane >> 3 == (i & 3);
             const uint32_t bytes = uint32_t(__popc(in_page)) * 16 * D;
             tile_wait(&ctl->k_empty[kr.i], kr.phase ^ 1, &ctl->abort);
+            if (gave_up(ctl)) { // no barrier is armed that may not be empty
+                stop = true;
+                break;
+            }
             if (lane >> 3 == (i & 3)) {
                 TileScale sc;
                 sc.a = now.ks * A.scale_log2, sc.e = log2_fast(now.vs), sc.iv = inverse_fast(now.vs), sc.unused = 0.f;
@@ -513,7 +570,12 @@ __device__ __forceinline__ void tile_load(const AttentionArgs& A, unsigned char*
             if (leads) {
                 bulk_load(shared_u32(smem + S::kOffK + kr.i * S::kCodes + mine * 16 * D), static_cast<const char*>(A.cache.k) + now.at, bytes, kb);
             }
+            kr.next();
             tile_wait(&ctl->v_empty[vr.i], vr.phase ^ 1, &ctl->abort);
+            if (gave_up(ctl)) {
+                stop = true;
+                break;
+            }
             if (lane == 0) {
                 bar_expect(vb, __popc(there) * 16 * D);
             }
@@ -521,12 +583,23 @@ __device__ __forceinline__ void tile_load(const AttentionArgs& A, unsigned char*
             if (leads) {
                 bulk_load(shared_u32(smem + S::kOffV + vr.i * S::kCodes + mine * 16 * D), static_cast<const char*>(A.cache.v) + now.at, bytes, vb);
             }
-            kr.next(), vr.next();
+            vr.next();
         }
         step += n;
     }
+    if (gave_up(ctl)) { // copies that are on their way land before the block ends; a stage that was never armed passes
+#pragma unroll 1
+        for (int i = 0; i < S::kKStages; i++) {
+            bar_wait(shared_u32(&ctl->k_full[i]), i < kr.i ? kr.phase : kr.phase ^ 1, kDrainTries);
+        }
+#pragma unroll 1
+        for (int i = 0; i < S::kVStages; i++) {
+            bar_wait(shared_u32(&ctl->v_full[i]), i < vr.i ? vr.phase : vr.phase ^ 1, kDrainTries);
+        }
+        __syncwarp();
+    }
     if (A.part_o && lane == 0) {
-        A.splits[blockIdx.x] = split;
+        A.splits[blockIdx.x] = walk.split;
     }
 }
 
@@ -585,6 +658,14 @@ __device__ __forceinline__ void tile_convert(unsigned char* smem, TileCtl* ctl) 
     }
 }
 
+// a warp that issued products and gave up waits for them, so that tensor memory is free when it is given back
+__device__ __forceinline__ void drain_products(TileCtl* ctl, uint32_t el, int which) {
+    if (gave_up(ctl)) {
+        mma_commit(el, shared_u32(&ctl->drained[which]));
+        bar_wait(shared_u32(&ctl->drained[which]), 0, kDrainTries);
+        __syncwarp();
+    }
+}
 // The products, a warp for each kind and tile: S as soon as p V has read p from its buffer, p V as soon as p is there. What a warp runs
 // between two batches is fetched anew each time, some 5 cycles an instruction: one warp that polled for whatever was ready held the tiles
 // up to 5500 cycles a step, one warp for each tile to 4000.
@@ -636,6 +717,7 @@ __device__ __forceinline__ void tile_scores(unsigned char* smem, TileCtl* ctl, u
             kr.next();
         }
     }
+    drain_products(ctl, el, t);
 }
 template <class T, int D>
 __device__ __forceinline__ void tile_sums(unsigned char* smem, TileCtl* ctl, uint32_t t) {
@@ -673,6 +755,7 @@ __device__ __forceinline__ void tile_sums(unsigned char* smem, TileCtl* ctl, uin
             hr.next();
         }
     }
+    drain_products(ctl, el, 2 + t);
 }
 
 template <class T, int D>
@@ -694,7 +777,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
             init(ctl->v_full[t], 1), init(ctl->v_empty[t], kConvertWarps), init(ctl->h_full[t], kConvertWarps), init(ctl->h_empty[t], 2);
         }
         for (int i = 0; i < 3; i++) {
-            init(ctl->k_full[i], 1), init(ctl->k_empty[i], 2);
+            init(ctl->k_full[i], int(blockIdx.x) == A.lose ? 2 : 1), init(ctl->k_empty[i], 2);
+        }
+        for (int i = 0; i < 4; i++) {
+            init(ctl->drained[i], 1);
         }
         for (int i = 0; i < kSegments; i++) {
             init(ctl->seg_full[i], 1), init(ctl->seg_empty[i], kReaders);
@@ -725,6 +811,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
     if (warp == 9) {
         tm_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(ctl->tmem), "r"(512) : "memory");
+    }
+    if (*static_cast<volatile int*>(&ctl->abort)) {
+        give_up_share<T, D>(A);
     }
 }
 

@@ -113,3 +113,37 @@ def test_lost_copy_of_one_long_sequence(seq, rng, lose):  # noqa: F811
     q = torch.randn(1, 8, 128, device="cuda", generator=rng).bfloat16()
     gone = lost_rows(seq, cache, batch, q, lose, 3)  # of the first head's shares
     assert gone[0].tolist() == [True] * 4 + [False] * 4
+
+
+@pytest.mark.parametrize("dim, dtype", [(64, "bf16"), (128, "f16")])
+@pytest.mark.parametrize("group, new", [(1, 40), (2, 140)])
+def test_lost_copy_many_rows(seq, rng, lose, group, new, dim, dtype):  # noqa: F811
+    """The same for the kernel of many rows: a unit is 256 rows of a head, two of them where a sequence has 280; the block's whole share is NaN."""
+    sequences, heads = 60 // group, 8
+    lens = torch.randint(new, 300, (sequences,), generator=rng, device="cuda").tolist()
+    batch = Batch(seq, [new] * sequences, lens, 32, rng)
+    cache = Cache(seq, batch.pages, 32, heads, dim).random(rng)
+    q = torch.randn(batch.rows, heads * group, dim, device="cuda", generator=rng).to(T[dtype])
+    tiles = -(-new * group // 256)
+    unit = torch.arange(new * group, device="cuda").view(new, group) // 256  # of a sequence's rows
+
+    def units(gone):
+        """Whether each unit is NaN, in the order of the line: sequence, tile, head."""
+        x = gone.view(sequences, new, heads, group)
+        parts = [x.permute(0, 2, 1, 3)[..., unit == t] for t in range(tiles)]
+        assert all(torch.equal(p.any(-1), p.all(-1)) for p in parts)
+        return torch.stack([p.all(-1) for p in parts], 1).flatten()
+
+    whole = units(lost_rows(seq, cache, batch, q, lose, 21))  # a block for each unit, the last tile first
+    assert whole.nonzero().flatten().tolist() == [(sequences * tiles - 1 - 21 // heads) * heads + 21 % heads]
+    batch.desc.max_len = 4000  # equal shares of 2 units and more
+    some = units(lost_rows(seq, cache, batch, q, lose, 70)).nonzero().flatten().tolist()
+    assert some == list(range(some[0], some[-1] + 1)) and 2 <= len(some) <= 10
+
+
+def test_lost_copy_of_one_long_prompt(seq, rng, lose):  # noqa: F811
+    batch = Batch(seq, [200], [9000], 64, rng)
+    cache = Cache(seq, batch.pages, 64, 2, 64).random(rng)
+    q = torch.randn(200, 2, 64, device="cuda", generator=rng).bfloat16()
+    gone = lost_rows(seq, cache, batch, q, lose, 3)  # of the first head's shares
+    assert gone[:, 0].all() and not gone[:, 1].any()
