@@ -434,7 +434,8 @@ int cck_cache_append(void* stream, const cck_cache* cache, const cck_batch* batc
     const int max_new = batch->max_new < batch->rows ? batch->max_new : batch->rows;
     const int P = cache->page_tokens, D = cache->dim, most = max_new < P ? max_new : P; // new rows of a page
     a.batch.max_new = max_new;
-    a.blocks_per_seq = max_new ? int((int64_t(max_new) + P - 2) / P + 1) : 0;
+    // without room for rows, a block for each sequence still says so if there are any
+    a.blocks_per_seq = max_new ? int((int64_t(max_new) + P - 2) / P + 1) : status ? 1 : 0;
     int64_t more = 0;
     int vec = 0;
     size_t smem = 0;

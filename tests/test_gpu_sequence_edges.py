@@ -147,3 +147,18 @@ def test_lost_copy_of_one_long_prompt(seq, rng, lose):  # noqa: F811
     q = torch.randn(200, 2, 64, device="cuda", generator=rng).bfloat16()
     gone = lost_rows(seq, cache, batch, q, lose, 3)  # of the first head's shares
     assert gone[:, 0].all() and not gone[:, 1].any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("what, value, status", [("max_new", 0, 1), ("rows", 0, 1), ("max_new", 0, 0)])
+def test_append_without_room_says_so(seq, rng, what, value, status, dtype):  # noqa: F811
+    """max_new or rows of zero leave every row out: the cache stays, the status is set if there were any."""
+    batch = Batch(seq, [3, 0, 2] if status else [0, 0, 0], [40, 9, 20], 32, rng)
+    cache = Cache(seq, batch.pages, 32, 2, 64).random(rng)
+    old = [x.clone() for x in (cache.k, cache.v, cache.ks, cache.vs)]
+    k = torch.randn(5, 2, 64, device="cuda", generator=rng).to(T[dtype])
+    setattr(batch.desc, what, value)
+    got = torch.zeros(1, dtype=torch.int32, device="cuda")
+    seq.cache_append(stream(), cache.desc, batch.desc, rows_of(seq, k), rows_of(seq, k), status=got.data_ptr())
+    assert got.item() == status
+    assert all(torch.equal(a, b) for a, b in zip(old, (cache.k, cache.v, cache.ks, cache.vs)))
