@@ -98,7 +98,7 @@ int check_rotation(const char* op, const cck_rotation* r, int rows, int dim) {
     if (pairs != r->dims / 2) {
         return refuse(CCK_E_SHAPE, op, "rotation: the sections do not add up to dims / 2");
     }
-    if (r->dims && (!r->freq || (!r->pos && rows) || !aligned(r->freq, 4) || !aligned(r->pos, 4))) {
+    if (r->dims && ((rows && (!r->freq || !r->pos)) || !aligned(r->freq, 4) || !aligned(r->pos, 4))) {
         return refuse(CCK_E_SHAPE, op, "rotation: freq or pos is null or not aligned");
     }
     return CCK_OK;
@@ -122,7 +122,7 @@ int check_cache(const char* op, const cck_cache* c) {
     return CCK_OK;
 }
 int check_batch(const char* op, const cck_batch* b) {
-    if (!b || !b->first || (b->sequences && (!b->len || !b->table)) || !aligned(b->first, 4) || !aligned(b->len, 4) || !aligned(b->table, 4)) {
+    if (!b || (b->sequences && (!b->first || !b->len || !b->table)) || !aligned(b->first, 4) || !aligned(b->len, 4) || !aligned(b->table, 4)) {
         return refuse(CCK_E_SHAPE, op, "the batch or an array of it is null or not aligned");
     }
     if (b->sequences < 0 || b->rows < 0 || b->max_new < 0 || b->max_len < 0 || b->table_pages < 1 || b->table_stride < 0) {
@@ -439,7 +439,7 @@ int cck_cache_append(void* stream, const cck_cache* cache, const cck_batch* batc
     int64_t more = 0;
     int vec = 0;
     size_t smem = 0;
-    if (q && batch->rows) {
+    if (q && batch->rows && batch->sequences) { // without sequences all rows are nobody's
         vec = rotary_vector(*rotation, D, *q, *q_out);
         a.q = rotary_shape(*rotation, batch->rows, D, *q, *q_out, false, vec, sms);
     }

@@ -75,7 +75,8 @@ size_t cck_static_workspace_bytes(void);
  * caller's, one or two kernels enqueued on `stream` (a stream of the current device), no allocation, no synchronisation, an
  * error code and cck_last_error(); every call can be captured into a CUDA graph. All descriptors are read before a call
  * returns; what their pointers point to (cck_rows::data, freq, pos, first, len, table, ...) is device memory that the kernels
- * read; it may be null where there are no rows or no sequences. Heads are at most 65536. Arguments that cannot be right are refused before anything is enqueued: CCK_E_SHAPE (null pointers, sizes, strides,
+ * read. data, freq and pos may be null where there are no rows, first, len and table where there are no sequences. Heads are at
+ * most 65536. Arguments that cannot be right are refused before anything is enqueued: CCK_E_SHAPE (null pointers, sizes, strides,
  * alignment), CCK_E_FLAGS (a type that is not built), CCK_E_WORKSPACE, CCK_E_DEVICE (memory of another device, or not device
  * memory). */
 enum { CCK_BF16 = 0, CCK_F16 = 1, CCK_F32 = 2 };

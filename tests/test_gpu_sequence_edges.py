@@ -162,3 +162,18 @@ def test_append_without_room_says_so(seq, rng, what, value, status, dtype):  # n
     seq.cache_append(stream(), cache.desc, batch.desc, rows_of(seq, k), rows_of(seq, k), status=got.data_ptr())
     assert got.item() == status
     assert all(torch.equal(a, b) for a, b in zip(old, (cache.k, cache.v, cache.ks, cache.vs)))
+
+
+def test_nothing_of_a_batch_without_sequences_is_read(seq, rng):  # noqa: F811
+    """Rows of nobody, and no arrays: nothing is written, queries stay."""
+    cache = Cache(seq, 2, 32, 2, 64).random(rng)
+    old = [x.clone() for x in (cache.k, cache.ks)]
+    x, q = (torch.randn(6, n, 64, device="cuda", generator=rng).bfloat16() for n in (2, 4))
+    out, freq, pos = torch.full_like(q, 5.0), torch.rand(32, device="cuda", generator=rng), torch.zeros(1, 6, dtype=torch.int32, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    batch = seq.Batch(0, 6, 3, 40, 1, None, None, None)
+    r = seq.Rotation(64, [32], freq.data_ptr(), pos.data_ptr())
+    seq.cache_append(stream(), cache.desc, batch, rows_of(seq, x), rows_of(seq, x), r, rows_of(seq, q), rows_of(seq, out), status=status.data_ptr())
+    seq.cache_attention(stream(), cache.desc, batch, rows_of(seq, q), rows_of(seq, out), 0.1)
+    torch.cuda.synchronize()
+    assert (out == 5.0).all() and status.item() == 0 and all(torch.equal(a, b) for a, b in zip(old, (cache.k, cache.ks)))
