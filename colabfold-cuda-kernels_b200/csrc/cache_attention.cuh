@@ -95,8 +95,9 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) { // an 8 x 8 matrix 
 }
 
 constexpr int kDecodeWarps = 4;
-// p = 2^(x - base); base = largest x - kHeadroom when it is set, and is set anew when an x is over base + kSlack. It begins below all scores
-constexpr float kHeadroom = 6.f, kSlack = 14.f, kNoBase = -1e30f;
+// p = 2^(x - base); base = largest x - kHeadroom when it is set, and is set anew when x - base is over kSlack (the difference: base + kSlack would
+// round up to an x that f16 has no 2^(x - base) for, where scores are past 2^27). It begins at the lowest float, below all scores
+constexpr float kHeadroom = 6.f, kSlack = 14.f, kNoBase = -3.402823466e38f;
 // terms of 4 bits that hold a query
 template <class T>
 constexpr int kTermsOf = std::is_same_v<T, __half> ? 3 : 2;
@@ -509,7 +510,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, DecodeShape<D, NT>::kBlocks
                         top[v & 1] = fmaxf(top[v & 1], x[u][t][v]);
                     }
                 }
-                if (__any_sync(0xffffffffu, top[0] > base[t][0] + kSlack || top[1] > base[t][1] + kSlack)) {
+                if (__any_sync(0xffffffffu, top[0] - base[t][0] > kSlack || top[1] - base[t][1] > kSlack)) {
                     float corr[2];
 #pragma unroll
                     for (int h = 0; h < 2; h++) {

@@ -27,6 +27,9 @@ namespace seq {
 
 constexpr int kTileKeys = 128, kHalfKeys = 64, kTileRows = 128, kUnitRows = 2 * kTileRows, kTileThreads = 512;
 constexpr int kConvertWarps = 3;
+// Up to this, a score's last place is at most a half, and x - base is one fused operation. Where scores could be larger (q is at most 256, a code 448), x is
+// rounded first, as base was: the fused difference would have digits that base has lost, and 2^(x - base) of the largest score itself could be past f16
+constexpr float kFine = 4194304.f;
 
 constexpr int kCtlBytes = 2048;
 template <class T, int D>
@@ -319,8 +322,10 @@ __device__ __forceinline__ void tile_softmax(const AttentionArgs& A, unsigned ch
             for (int u = 0; u < 4; u++) {
                 f[u] = sc[u].a * up, e[u] = sc[u].e;
             }
+            const bool large = max3(f[0], f[1], fmaxf(f[2], f[3])) > kFine / (256.f * 448.f * D);
             tm_ld_wait(x), tm_ld_wait(x + 32);
-            if (key0 < all_lo || key0 + kHalfKeys > all_hi) { // masked scores are -inf; scaled first: a page that is not there has a NaN scale, which they must not take
+            // masked scores are -inf; scaled first: a page that is not there has a NaN scale, which they must not take
+            if (key0 < all_lo || key0 + kHalfKeys > all_hi || large) {
 #pragma unroll
                 for (int c = 0; c < 64; c++) {
                     const float y = fmaf(__uint_as_float(x[c]), f[c / 16], e[c / 16]);
@@ -338,9 +343,9 @@ __device__ __forceinline__ void tile_softmax(const AttentionArgs& A, unsigned ch
                 const float m1 = max3(max3(y[9], y[10], y[11]), max3(y[12], y[13], y[14]), y[15]);
                 top = fmaxf(top, fmaf(fmaxf(m0, m1), f[u], e[u]));
             }
-            if (__any_sync(0xffffffffu, top > base + kSlack)) {
+            if (__any_sync(0xffffffffu, top - base > kSlack)) {
                 const float was = base;
-                base = top > base + kSlack ? top - kHeadroom : base;
+                base = top - base > kSlack ? top - kHeadroom : base;
                 const float corr = exp2_fast(was - base);
                 l *= corr;
                 if (j > 0) { // O is whole when the last p V is done; the next one waits for this p

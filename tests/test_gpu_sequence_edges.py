@@ -177,3 +177,65 @@ def test_nothing_of_a_batch_without_sequences_is_read(seq, rng):  # noqa: F811
     seq.cache_attention(stream(), cache.desc, batch, rows_of(seq, q), rows_of(seq, out), 0.1)
     torch.cuda.synchronize()
     assert (out == 5.0).all() and status.item() == 0 and all(torch.equal(a, b) for a, b in zip(old, (cache.k, cache.ks)))
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("power", [4, 20, 24, 26, 27, 28, 30, 60, 100, 118])
+@pytest.mark.parametrize("dtype, new, dim", [("bf16", 1, 128), ("f16", 3, 64), ("bf16", 40, 128), ("f16", 33, 64), ("bf16", 70, 32)])
+def test_scores_of_any_size(seq, rng, dtype, new, dim, power, sign):  # noqa: F811
+    """Scores of up to 2^127 either way, all of one sign: one key is ahead of all others by 2^power, and the row is that key's values.
+
+    q is one dimension, a power of two; products with the codes are exact. The probability of the key is rounded to f16 in the product and not in
+    the sum, 2^-11, and the result to its type; that of the others is 2^-2^power or less each, so that they add at most 700 times that to the
+    logarithm of the sum."""
+    length = 700
+    batch = Batch(seq, [new], [length], 32, rng)
+    cache = Cache(seq, batch.pages, 32, 1, dim).random(rng)
+    k, v = (c.clone() for c in cache.views())
+    codes = torch.tensor([64.0, 128, 256, 448] if sign < 0 else [64.0, 128, 256], device="cuda")[torch.randint(0, 3 + (sign < 0), (length,), device="cuda", generator=rng)]
+    best = 400
+    codes[best] = 32 if sign < 0 else 416
+    at = torch.tensor(batch.lists[0], device="cuda")[torch.arange(length, device="cuda") // 32], torch.arange(length, device="cuda") % 32
+    k[at[0], 0, at[1], 5] = codes.to(torch.float8_e4m3fn).view(torch.uint8)
+    cache.put(k, v, torch.full_like(cache.ks, 2.0**30), cache.vs.clone())
+    q = torch.zeros(new, 2, dim, device="cuda")
+    q[:, :, 5] = sign * 4.0
+    scale = 1.1 * 2.0 ** (power - 5 - 30 - 2) / 1.4426950408889634  # the least distance of codes is 32
+    q = q.to(T[dtype])
+    out, lse = torch.full_like(q, 5.0), torch.full((new, 2), 5.0, device="cuda")
+    need = seq.cache_attention_workspace_bytes(cache.desc, batch.desc, 2)
+    ws = torch.empty(need + 16, dtype=torch.uint8, device="cuda")
+    seq.cache_attention(stream(), cache.desc, batch.desc, rows_of(seq, q), rows_of(seq, out), scale, ws.data_ptr(), need, lse=lse.data_ptr())
+    want = cache.token_values(batch.lists[0], length)[1][0, best].expand_as(out)
+    assert ((out.double() - want).abs() <= (2.0**-11 + torch.finfo(T[dtype]).eps / 2 + length * 2.0 ** -(2.0**power)) * 1.01 * 448 * cache.vs.double().max()).all()
+    top = sign * 4.0 * 2.0**30 * codes[best].item() * scale
+    assert ((lse.double() - top).abs() <= 2.0**-20 * (1 + abs(top)) + length * 2.0 ** -(2.0**power)).all()
+
+
+@pytest.mark.parametrize("dtype, new, dim", [("bf16", 1, 128), ("f16", 3, 64), ("bf16", 40, 128), ("f16", 33, 64)])
+def test_scores_whose_last_place_is_sixteen(seq, rng, dtype, new, dim):  # noqa: F811
+    """Scores (times log2 e) of 2^27 + 16, then one of 2^27 + 32: as far ahead as a last place, and 2^16 times as probable.
+
+    q, codes and scale are powers of two, so that scores are exact and probabilities powers of two, which f16 holds. What is left is one rounding of
+    the result to its type (2^-8 of itself for bf16, of up to 448 here: more than 0.875) and the sums of 501 products in f32, truncated: 501 * 2^-23 of
+    the largest, below 2^-14."""
+    length, first, best = 700, 500, 600
+    batch = Batch(seq, [new], [length], 32, rng)
+    cache = Cache(seq, batch.pages, 32, 1, dim).random(rng)
+    k, v = (c.clone() for c in cache.views())
+    rows = torch.zeros(length, dim, device="cuda")
+    rows[:first, 0] = rows[best, 0] = 256
+    rows[:first, 1], rows[best, 1] = 2.0**-6, 2.0**-5
+    at = torch.tensor(batch.lists[0], device="cuda")[torch.arange(length, device="cuda") // 32], torch.arange(length, device="cuda") % 32
+    k[at[0], 0, at[1]] = rows.to(torch.float8_e4m3fn).view(torch.uint8)
+    cache.put(k, v, torch.ones_like(cache.ks), torch.ones_like(cache.vs))
+    q = torch.zeros(new, 1, dim, device="cuda").to(T[dtype])
+    q[..., 0], q[..., 1] = 4.0, 2.0**-7
+    scale = 2.0**17 * 0.6931471824645996  # times log2 e in f32: 2^17
+    out = torch.full_like(q, 5.0)
+    need = seq.cache_attention_workspace_bytes(cache.desc, batch.desc, 1)
+    ws = torch.empty(need + 16, dtype=torch.uint8, device="cuda")
+    seq.cache_attention(stream(), cache.desc, batch.desc, rows_of(seq, q), rows_of(seq, out), scale, ws.data_ptr(), need)
+    values = cache.token_values(batch.lists[0], length)[1][0]
+    want = (values[best] + values[:first].sum(0) * 2.0**-16) / (1 + first * 2.0**-16)
+    assert ((out.double() - want).abs() <= torch.finfo(T[dtype]).eps / 2 * want.abs() + 2.0**-14 * 448).all()
