@@ -1,9 +1,11 @@
 """The sequence operators where one call meets what another leaves: shares of many short units, and the like. Plain forms in 64 bits and
 tolerances are test_gpu_sequence.py's, where they are derived, unless a test says otherwise."""
+import math
+
 import pytest
 
 torch = pytest.importorskip("torch")
-from test_gpu_sequence import T, Batch, Cache, check_attention, rng, rows_of, seq, stream  # noqa: E402, F401
+from test_gpu_sequence import T, Batch, Cache, append_plain, check_attention, pair_size, rng, rows_of, seq, stream, turned  # noqa: E402, F401
 
 pytestmark = pytest.mark.gpu
 
@@ -239,3 +241,44 @@ def test_scores_whose_last_place_is_sixteen(seq, rng, dtype, new, dim):  # noqa:
     values = cache.token_values(batch.lists[0], length)[1][0]
     want = (values[best] + values[:first].sum(0) * 2.0**-16) / (1 + first * 2.0**-16)
     assert ((out.double() - want).abs() <= torch.finfo(T[dtype]).eps / 2 * want.abs() + 2.0**-14 * 448).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("adjacent", [False, True])
+@pytest.mark.parametrize(
+    "new, lens, page, dim, rot",
+    [([128, 1, 70], [128, 257, 300], 128, 128, 128), ([128], [255], 128, 128, 64), ([64, 5, 0, 33], [64, 70, 9, 100], 64, 96, 96), ([20, 1], [50, 33], 16, 96, 48),
+     ([40, 3], [40, 1000], 32, 32, 32), ([1, 1, 1], [1, 128, 129], 128, 128, 128), ([17, 16], [17, 48], 16, 64, 48), ([33], [95], 32, 128, 96)],
+)  # fmt: skip
+def test_append_rotates_every_size(seq, rng, new, lens, page, dim, rot, adjacent, dtype):  # noqa: F811
+    """Rotated keys of all dimensions, types and pairings, pages that are filled at once among them: half a step of e4m3 (2^-4 of itself, or 2^-10 of the
+    page's scale) beside the rotation's 2^-20 (|a| + |b|), which half a step more can follow: 1 + 2^-4. Queries to half a step of their type."""
+    heads = 3
+    batch = Batch(seq, new, lens, page, rng)
+    cache = Cache(seq, batch.pages, page, heads, dim).random(rng)
+    before = [(c.view(torch.float8_e4m3fn).double(), s.double().clone()) for c, s in zip(cache.views(), (cache.ks, cache.vs))]
+    q, k, v = (torch.randn(batch.rows, n, dim, device="cuda", generator=rng).to(T[dtype]) for n in (5, heads, heads))
+    pos = torch.randint(-(1 << 20), 1 << 20, (3, batch.rows), device="cuda", generator=rng, dtype=torch.int32)
+    freq = torch.rand(rot // 2, device="cuda", generator=rng)
+    sections = [rot // 2 - 9, 4, 5]
+    r = seq.Rotation(rot, sections, freq.data_ptr(), pos.data_ptr(), batch.rows, adjacent=adjacent)
+    out = torch.full_like(q, math.nan)
+    seq.cache_append(stream(), cache.desc, batch.desc, rows_of(seq, k), rows_of(seq, v), r, rows_of(seq, q), rows_of(seq, out))
+    want_q, want_k = turned(q, pos, freq, sections, adjacent), turned(k, pos, freq, sections, adjacent)
+    assert ((out.double() - want_q).abs() <= torch.finfo(T[dtype]).eps / 2 * want_q.abs() + 2.0**-20 * pair_size(q, rot, adjacent)).all()
+    want, scale = append_plain(cache, batch, v.double(), before[1])
+    assert torch.equal(cache.vs.double(), scale) and torch.equal(cache.views()[1].view(torch.float8_e4m3fn).double(), want)
+    want, scale = append_plain(cache, batch, want_k, before[0])
+    assert torch.equal(cache.ks.double(), scale)
+    got, off = cache.views()[0].view(torch.float8_e4m3fn).double(), pair_size(k, rot, adjacent)
+    written = torch.zeros(cache.n, page, dtype=torch.bool, device="cuda")
+    for b, n in enumerate(new):
+        for i in range(n):
+            place = lens[b] - n + i
+            p, slot, row = batch.lists[b][place // page], place % page, batch.start(b) + i
+            written[p, slot] = True
+            s = scale[p][:, None]
+            bound = torch.maximum(2.0**-4 * want_k[row].abs(), 2.0**-10 * s) + (1 + 2.0**-4) * 2.0**-20 * off[row]
+            assert ((got[p, :, slot] * s - want_k[row]).abs() <= bound).all(), (b, i)
+    rest = ~written[:, None, :, None].expand_as(got)  # older tokens, brought to the new scale, and slots of nobody
+    assert torch.equal(got[rest], want[rest])
