@@ -77,28 +77,25 @@ __device__ __forceinline__ float2 rotate(float a, float b, float2 cs) {
     return make_float2(fmaf(a, cs.x, -b * cs.y), fmaf(b, cs.x, a * cs.y));
 }
 
-// Cosines and sines of `rows` rows from row0 on, all pairs: table[row][pair]. The block's threads t of nt
+// Cosines and sines of `rows` rows from row0 on, all pairs: table[row][pair]. The block's threads t of nt, which are more than the pairs: one stays with a
+// pair, whose frequency it converts once
 __device__ __forceinline__ void fill_table(const cck_rotation& R, float2* table, int64_t row0, int rows, int t, int nt) {
-    const int pairs = R.dims / 2;
-    const int step = nt > pairs ? nt / pairs : 1; // rows at once
-    // a thread stays with a pair where it can: its frequency is converted once
-    for (int p = t % pairs; p < pairs; p += nt) {
-        const Turns f = turns_of(R.freq[p]);
-        const int* pos = R.pos + axis_of(R, p) * R.pos_stride + row0;
-        if (nt > pairs && t >= step * pairs) {
-            return;
-        }
+    const int pairs = R.dims / 2, step = nt / pairs, p = t % pairs; // step: rows at once
+    if (t >= step * pairs) {
+        return;
+    }
+    const Turns f = turns_of(R.freq[p]);
+    const int* pos = R.pos + axis_of(R, p) * R.pos_stride + row0;
 #pragma unroll 4
-        for (int r = nt > pairs ? t / pairs : 0; r < rows; r += step) {
-            table[r * pairs + p] = cos_sin(pos[r], f);
-        }
+    for (int r = t / pairs; r < rows; r += step) {
+        table[r * pairs + p] = cos_sin(pos[r], f);
     }
 }
 
 // x rotated into y, a unit (one of `splits` parts of a row's heads) after the other: those of warp `unit`, + step, ... A head of a row has `items`
 // items: pairs [V p, V p + V) for p < rot_items, then 2V copied dimensions each. table: the warp's own, dims / 2 entries.
 struct RotaryShape {
-    int rows, dim, heads, rot_items, items, splits, part_heads, sign;
+    int dim, heads, rot_items, items, splits, part_heads, sign;
     int64_t units;
     int64_t xr, xh, yr, yh;
     const void* x;

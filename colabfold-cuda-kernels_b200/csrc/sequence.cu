@@ -169,7 +169,7 @@ int rotary_vector(const cck_rotation& r, int dim, const cck_rows& x, const cck_r
 // one head a lane
 RotaryShape rotary_shape(const cck_rotation& r, int rows, int dim, const cck_rows& x, const cck_rows& y, bool inverse, int v, int sms) {
     RotaryShape s{};
-    s.rows = rows, s.dim = dim, s.heads = x.heads, s.sign = inverse ? -1 : 1;
+    s.dim = dim, s.heads = x.heads, s.sign = inverse ? -1 : 1;
     s.x = x.data, s.y = y.data, s.xr = x.row_stride, s.xh = x.head_stride, s.yr = y.row_stride, s.yh = y.head_stride;
     s.rot_items = r.dims / 2 / v;
     s.items = s.rot_items + (x.data == y.data ? 0 : ceil_div(dim - r.dims, 2 * v));
@@ -240,15 +240,15 @@ cudaError_t launch_append(cudaStream_t st, const AppendArgs& a, bool pages, int 
         kernel<<<blocks, threads, smem, st>>>(a);
         return cudaGetLastError();
     };
-    static std::atomic<bool> ready[12][kMaxDevices];
+    static std::atomic<bool> ready[11][kMaxDevices];
     if constexpr (sizeof(T) == 2) {
         auto of_dim = [&](auto adjacent) {
             constexpr bool adj = decltype(adjacent)::value;
             switch (a.cache.dim) {
-            case 32: return go(append_pages_kernel<T, 32, adj>, ready[4 + adj]);
-            case 64: return go(append_pages_kernel<T, 64, adj>, ready[6 + adj]);
-            case 96: return go(append_pages_kernel<T, 96, adj>, ready[8 + adj]);
-            default: return go(append_pages_kernel<T, 128, adj>, ready[10 + adj]);
+            case 32: return go(append_pages_kernel<T, 32, adj>, ready[3 + adj]);
+            case 64: return go(append_pages_kernel<T, 64, adj>, ready[5 + adj]);
+            case 96: return go(append_pages_kernel<T, 96, adj>, ready[7 + adj]);
+            default: return go(append_pages_kernel<T, 128, adj>, ready[9 + adj]);
             }
         };
         if (pages) {
@@ -265,9 +265,7 @@ cudaError_t launch_append(cudaStream_t st, const AppendArgs& a, bool pages, int 
             return a.rotation.adjacent ? cudaLaunchKernelEx(&cfg, query_kernel<T, true>, a) : cudaLaunchKernelEx(&cfg, query_kernel<T, false>, a);
         }
     }
-    constexpr int kMost = 16 / sizeof(T);
-    switch (v) {
-    case 8: return go(append_kernel<T, kMost>, ready[3]);
+    switch (v) { // vectors of 8 queries go with append_pages_kernel
     case 4: return go(append_kernel<T, 4>, ready[2]);
     case 2: return go(append_kernel<T, 2>, ready[1]);
     default: return go(append_kernel<T, 1>, ready[0]);
