@@ -498,7 +498,7 @@ int cck_cache_append(void* stream, const cck_cache* cache, const cck_batch* batc
 size_t cck_cache_attention_workspace_bytes(const cck_cache* cache, const cck_batch* batch, int q_heads) {
     const char* op = "cck_cache_attention_workspace_bytes";
     int sms = 0;
-    if (check_cache(op, cache) || check_batch(op, batch) || q_heads < 1 || q_heads % cache->heads || device_of(op, {}, sms)) {
+    if (check_cache(op, cache) || check_batch(op, batch) || q_heads < 1 || q_heads > kMostHeads || q_heads % cache->heads || device_of(op, {}, sms)) {
         return 0;
     }
     return make_plan(*cache, *batch, q_heads, sms).bytes;

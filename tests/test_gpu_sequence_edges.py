@@ -282,3 +282,10 @@ def test_append_rotates_every_size(seq, rng, new, lens, page, dim, rot, adjacent
             assert ((got[p, :, slot] * s - want_k[row]).abs() <= bound).all(), (b, i)
     rest = ~written[:, None, :, None].expand_as(got)  # older tokens, brought to the new scale, and slots of nobody
     assert torch.equal(got[rest], want[rest])
+
+
+def test_workspace_of_heads_that_are_refused_is_zero(seq, rng):  # noqa: F811
+    batch = Batch(seq, [1], [5000], 32, rng)
+    cache = Cache(seq, batch.pages, 32, 1, 64)
+    assert seq.cache_attention_workspace_bytes(cache.desc, batch.desc, 1 << 16) > 0
+    assert seq.cache_attention_workspace_bytes(cache.desc, batch.desc, (1 << 16) + 16) == 0
