@@ -88,6 +88,9 @@ int check_rotation(const char* op, const cck_rotation* r, int rows, int dim) {
     if (r->dims < 0 || r->dims % 2 || r->dims > dim || r->axes < 1 || r->axes > 4) {
         return refuse(CCK_E_SHAPE, op, "rotation: dims is even and at most a head's, axes 1 to 4");
     }
+    if (r->pos_stride < 0) {
+        return refuse(CCK_E_SHAPE, op, "rotation: the positions' stride is negative");
+    }
     int64_t pairs = 0;
     for (int a = 0; a < r->axes; a++) {
         if (r->section[a] < 0) {

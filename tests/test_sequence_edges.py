@@ -32,3 +32,12 @@ def test_frequencies_of_no_rows_may_be_null(seq, op):  # noqa: F811
     a["rows"] = a["batch"].rows = 0
     with pytest.raises(RuntimeError, match="device"):
         call(seq, op, a)
+
+
+@pytest.mark.parametrize("op", ["rotary", "append"])
+def test_negative_stride_of_positions(seq, op):  # noqa: F811
+    """As those of tensors and tables."""
+    a = good(seq)
+    a["rotation"].pos_stride = -5
+    with pytest.raises(ValueError, match="stride"):
+        call(seq, op, a)
