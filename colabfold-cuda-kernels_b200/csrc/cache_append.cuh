@@ -7,8 +7,8 @@
 // each (page, head) and as many heads at once as a block has groups; the angles of the page's rows are computed once, into shared memory,
 // for all heads that a block goes through. It wants 16-bit values and rotated parts that are whole vectors. append_kernel takes everything
 // else through shared memory, a block for each (page, head). Each row is read once, each code written once: bound by memory for
-// prompts (eight of about 900 tokens, 32 + 8 + 8 heads of 128: 49 us, 3.2 TB/s), by latency for single tokens (64: 10 us with the launch) and for small pages,
-// where a block is a chain of loads, angles, the largest value and the codes (2000 tokens of 3 x 20 heads of 64 in pages of 16: 16 us).
+// prompts (eight of about 900 tokens, 32 + 8 + 8 heads of 128: 51 us, 3.0 TB/s), by latency for single tokens (64: 11 us with the launch) and for small pages,
+// where a block is a chain of loads, angles, the largest value and the codes (2000 tokens of 3 x 20 heads of 64 in pages of 16: 18 us, 15.5 from a captured graph).
 #pragma once
 
 #include "rotary.cuh"
@@ -90,6 +90,26 @@ inline size_t append_smem(int rows, int dim, int size) {
     return size_t(rows) * (append_key_pitch(dim) * 4 + append_value_pitch(dim, size) * size + 4) + 128;
 }
 
+// ---- Codes of rotated keys that lie next to a rounding's border
+//
+// A rotation in 32 bits is off by less than 2^-21 (|a'| + |b'|): cosine and sine by 2^-23, a product by 2^-24, for |a| + |b|, which is at most 1.42 times
+// |a'| + |b'|, and the sum by 2^-24 of itself: 2.7 * 2^-23. Where both ends of that give the same code, it is the code of the rotation itself. Else, for
+// one value in 2^15, the pair is rotated again in 64 bits and rounded once, so that the codes are those of the definition. Without it 31 codes of 12
+// batches of 2000 rows of 20 heads of 64 were not. Those seldom values take some 0.6 us of a block, and so of a call of few tokens; from a captured
+// graph, 64 single tokens 6.4 -> 7.0 us, eight prompts of about 900 tokens 48.1 -> 50.1, 2000 tokens in pages of 16 14.3 -> 15.5.
+constexpr float kRotationOff = 1.f / 2097152.f;
+// the code of a pair's first or second value after rotation, times inv
+__device__ __forceinline__ uint32_t exact_code(const cck_rotation& R, int64_t row, int pair, float a, float b, bool second, float inv) {
+    const double2 cs = cos_sin_exactly(R.pos[axis_of(R, pair) * R.pos_stride + row], turns_of(R.freq[pair]));
+    const double x = (second ? fma(double(b), cs.x, double(a) * cs.y) : fma(double(a), cs.x, -double(b) * cs.y)) * double(inv);
+    const float f = __double2float_rz(x); // to odd, so that the second rounding does not see a border that x is beside
+    return pack_e4m3(double(f) == x || x != x ? f : __uint_as_float(__float_as_uint(f) | 1u), 0.f) & 0xFFu;
+}
+// the bytes in which two words differ, a bit each
+__device__ __forceinline__ uint32_t differing(uint32_t v, uint32_t w) {
+    return ((__vcmpne4(v, w) & 0x01010101u) * 0x10204080u) >> 28;
+}
+
 constexpr int kAppendSmem = 140 * 1024; // the most: 128 rows of 128 values in 32 bits
 
 __device__ __forceinline__ bool is_finite(float x) {
@@ -157,7 +177,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
         const float2 cs = cos_sin(A.rotation.pos[axis_of(A.rotation, p) * A.rotation.pos_stride + row0 + u], turns_of(A.rotation.freq[p]));
         float* a = fk + u * kp + (A.rotation.adjacent ? 2 * p : p);
         float* c = a + (A.rotation.adjacent ? 1 : half);
-        const float2 z = rotate_exactly(*a, *c, cs);
+        const float2 z = rotate(*a, *c, cs);
         *a = z.x, *c = z.y;
     }
     __syncthreads();
@@ -207,6 +227,15 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
             w[j] = bad[u] ? kNanCodes : pack_e4m3(x.x * inv_k, x.y * inv_k, x.z * inv_k, x.w * inv_k);
         }
         *reinterpret_cast<uint4*>(ck + key_offset(D, s0 + u, d)) = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll 1
+        for (int e = d; e < min(d + 16, A.rotation.dims) && !bad[u]; e++) {
+            const int pair = A.rotation.adjacent ? e >> 1 : e < half ? e : e - half, i0 = A.rotation.adjacent ? 2 * pair : pair, i1 = A.rotation.adjacent ? i0 + 1 : i0 + half;
+            const float x = fk[u * kp + e], off = (fabsf(fk[u * kp + i0]) + fabsf(fk[u * kp + i1])) * (kRotationOff * inv_k);
+            if (pack_e4m3(fmaf(x, inv_k, -off), 0.f) != pack_e4m3(fmaf(x, inv_k, off), 0.f)) {
+                const T* k = static_cast<const T*>(A.k) + (row0 + u) * A.kr + head * A.kh;
+                ck[key_offset(D, s0 + u, e)] = (unsigned char)exact_code(A.rotation, row0 + u, pair, to_f32(k[i0]), to_f32(k[i1]), e == i1, inv_k);
+            }
+        }
     }
     // values: a dimension's 16 tokens are 16 bytes
     const int g0 = lower_v < 1.f ? 0 : s0 / 16, g1 = ceil_div(s1, 16);
@@ -236,6 +265,21 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
             w[j] = pack_e4m3(x[0], x[1], x[2], x[3]);
         }
         *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// Codes of a thread's two key items (as below) anew where `which` has a bit, 16 for each
+template <class T, int D, bool kAdjacent>
+__device__ __noinline__ void exact_codes(const AppendArgs& A, unsigned char* codes, int s0, int row0, int head, int gt, int GT, uint32_t which, float inv) {
+#pragma unroll 1
+    for (; which; which &= which - 1) {
+        const int bit = __ffs(which) - 1, i = bit & 15, it = gt + (bit >> 4) * GT, c = it % (D / 16), slot = s0 + it / (D / 16);
+        const int64_t row = row0 + it / (D / 16);
+        const T* k = static_cast<const T*>(A.k) + row * A.kr + head * A.kh;
+        const int pair = kAdjacent ? 8 * c + (i >> 1) : 8 * c + (i & 7);
+        const bool second = kAdjacent ? i & 1 : i >> 3;
+        const int i0 = kAdjacent ? 2 * pair : pair, i1 = kAdjacent ? i0 + 1 : i0 + A.rotation.dims / 2;
+        codes[key_offset(D, slot, second ? i1 : i0)] = (unsigned char)exact_code(A.rotation, row, pair, to_f32(k[i0]), to_f32(k[i1]), second, inv);
     }
 }
 
@@ -327,7 +371,7 @@ __global__ void __launch_bounds__(kPageThreads, 1) append_pages_kernel(const __g
                     const float4 w = cs[e];
                     float &a0 = kAdjacent ? x[n][4 * e] : x[n][2 * e], &b0 = kAdjacent ? x[n][4 * e + 1] : x[n][8 + 2 * e];
                     float &a1 = kAdjacent ? x[n][4 * e + 2] : x[n][2 * e + 1], &b1 = kAdjacent ? x[n][4 * e + 3] : x[n][9 + 2 * e];
-                    const float2 z0 = rotate_exactly(a0, b0, make_float2(w.x, w.y)), z1 = rotate_exactly(a1, b1, make_float2(w.z, w.w));
+                    const float2 z0 = rotate(a0, b0, make_float2(w.x, w.y)), z1 = rotate(a1, b1, make_float2(w.z, w.w));
                     a0 = z0.x, b0 = z0.y, a1 = z1.x, b1 = z1.y;
                 }
             }
@@ -433,19 +477,30 @@ __global__ void __launch_bounds__(kPageThreads, 1) append_pages_kernel(const __g
         }
         unsigned char* ck = static_cast<unsigned char*>(C.k) + at * P * D;
         unsigned char* cv = static_cast<unsigned char*>(C.v) + at * P * D;
+        static_assert(kKeyItems == 2, "bits of later");
+        uint32_t later = 0; // values next to a border, 16 bits an item
 #pragma unroll
         for (int n = 0; n < kKeyItems; n++) {
             const int it = gt + n * GT, u = it / strips, c = it % strips;
             if (u >= rows) {
                 continue;
             }
-            uint32_t w[4];
+            uint32_t w[4], beside = 0;
+            const float off = c < turned ? kRotationOff * sc.inv_k : 0.f;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                w[e] = pack_e4m3(x[n][4 * e] * sc.inv_k, x[n][4 * e + 1] * sc.inv_k, x[n][4 * e + 2] * sc.inv_k, x[n][4 * e + 3] * sc.inv_k);
+                float lo[4], hi[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int i = 4 * e + j, other = kAdjacent ? i ^ 1 : i ^ 8;
+                    const float m = (fabsf(x[n][i]) + fabsf(x[n][other])) * off;
+                    lo[j] = fmaf(x[n][i], sc.inv_k, -m), hi[j] = fmaf(x[n][i], sc.inv_k, m);
+                }
+                w[e] = pack_e4m3(lo[0], lo[1], lo[2], lo[3]);
+                beside |= differing(w[e], pack_e4m3(hi[0], hi[1], hi[2], hi[3])) << (4 * e);
             }
             if (some_bad && (bad[group][u / 32] >> (u % 32) & 1)) {
-                w[0] = w[1] = w[2] = w[3] = kNanCodes;
+                w[0] = w[1] = w[2] = w[3] = kNanCodes, beside = 0;
             }
             if (c < turned && !kAdjacent) {
                 *reinterpret_cast<uint2*>(ck + key_offset(D, s0 + u, 8 * c)) = make_uint2(w[0], w[1]);
@@ -453,6 +508,7 @@ __global__ void __launch_bounds__(kPageThreads, 1) append_pages_kernel(const __g
             } else {
                 *reinterpret_cast<uint4*>(ck + key_offset(D, s0 + u, 16 * c)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
+            later |= beside << (16 * n);
         }
 #pragma unroll
         for (int n = 0; n < kValueItems; n++) {
@@ -506,6 +562,9 @@ __global__ void __launch_bounds__(kPageThreads, 1) append_pages_kernel(const __g
                 w.x = lowered(w.x, sc.lower_v), w.y = lowered(w.y, sc.lower_v), w.z = lowered(w.z, sc.lower_v), w.w = lowered(w.w, sc.lower_v);
                 *p = w;
             }
+        }
+        if (later) { // last, when nothing is held in registers over the call
+            exact_codes<T, D, kAdjacent>(A, ck, s0, pr.row0, head, gt, GT, later, sc.inv_k);
         }
     }
 }

@@ -40,9 +40,8 @@ __device__ __forceinline__ Turns turns_of(float freq) {
 // The nearest quarter turn is taken off in integers; what is left, at most pi / 4, goes through the Taylor series of sine and cosine about
 // zero to the ninth and tenth power (the terms after them are below 2e-9 of the result). It is held in two floats, x + e, down to 2^-58 of a turn,
 // so that a small angle keeps its digits, and the last additions carry what they round off: both come out within a few units of the last place of
-// themselves, however small the sine is, as far as the angle itself is known (2^-52 of position times frequency). Keys turned with them are rounded to 4
-// bits: of 12 batches of 2000 rows of 20 heads of 64, 31 codes are not the ones of 64 bits. With 2^-32 of a turn it took the same time, and a sine of 1e-4
-// was off by 1e-5 of itself.
+// themselves, however small the sine is, as far as the angle itself is known (2^-52 of position times frequency). With 2^-32 of a turn it took the same
+// time, and a sine of 1e-4 was off by 1e-5 of itself.
 __device__ __forceinline__ float2 cos_sin(int pos, Turns t) {
     const uint64_t angle = t.per * uint64_t(int64_t(pos)); // of a turn, in 2^-64
     const uint32_t top = uint32_t(angle >> 32);
@@ -68,10 +67,19 @@ __device__ __forceinline__ float2 cos_sin(int pos, Turns t) {
     const float2 cs = make_float2(__uint_as_float(__float_as_uint(u) ^ flip_c << 30), __uint_as_float(__float_as_uint(v) ^ flip_s << 30));
     return t.finite ? cs : make_float2(__int_as_float(0x7fffffff), __int_as_float(0x7fffffff));
 }
-// the same with what the products lose, for a result that is rounded to few bits
-__device__ __forceinline__ float2 rotate_exactly(float a, float b, float2 cs) {
-    const float p = b * cs.y, q = a * cs.y;
-    return make_float2(fmaf(a, cs.x, -p) - fmaf(b, cs.y, -p), fmaf(b, cs.x, q) + fmaf(a, cs.y, -q));
+// the same in 64 bits, to the eighteenth power: the terms after them are below 2^-58 of the result
+__device__ __forceinline__ double2 cos_sin_exactly(int pos, Turns t) {
+    const uint64_t angle = t.per * uint64_t(int64_t(pos));
+    const int quarter = int(int64_t(angle + (1ull << 61)) >> 62);
+    const double x = double(int64_t(angle - (uint64_t(int64_t(quarter)) << 62))) * (6.283185307179586477 / 18446744073709551616.0), y = x * x;
+    double s = 1.0, c = 1.0;
+#pragma unroll
+    for (int n = 18; n > 0; n -= 2) { // cosine 1 - y / (1 2) (1 - y / (3 4) (1 - ...)), sine over x 1 - y / (2 3) (1 - ...)
+        s = n == 18 ? 1.0 : fma(y * (-1.0 / double(n * (n + 1))), s, 1.0), c = fma(y * (-1.0 / double(n * (n - 1))), c, 1.0);
+    }
+    s *= x;
+    const double u = quarter & 1 ? s : c, v = quarter & 1 ? c : s;
+    return make_double2(quarter == 1 || quarter == -2 ? -u : u, quarter < 0 ? -v : v);
 }
 __device__ __forceinline__ float2 rotate(float a, float b, float2 cs) {
     return make_float2(fmaf(a, cs.x, -b * cs.y), fmaf(b, cs.x, a * cs.y));

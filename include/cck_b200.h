@@ -134,7 +134,8 @@ int cck_rotary(void* stream, const cck_rotation* rotation, int rows, int dim, co
  * cache, the keys rotated if `rotation` is given. q (may be null; any number of heads) is rotated into q_out (which may be q) by
  * the same call.
  * A page's scale is the smallest power of two that holds the values put into it, at least the one it has if older tokens of the
- * sequence share the page: those are then brought to the new scale. Rounded to nearest even; magnitudes over 448 * 2^40 saturate,
+ * sequence share the page: those are then brought to the new scale. Rounded to nearest even, a rotated key as its
+ * rotation in 64 bits is; magnitudes over 448 * 2^40 saturate,
  * what is far below 2^-40 is lost. A token that holds NaN or an infinity in a head's key or value becomes NaN in whole: its key's
  * codes are NaN, its value's are zero, and the rows of that head that attend to it come out as NaN, the others untouched.
  * Pages that a call writes to belong to one sequence of the batch; full pages may be shared. Slots past len[b] keep their codes.
