@@ -7,8 +7,8 @@
 // each (page, head) and as many heads at once as a block has groups; the angles of the page's rows are computed once, into shared memory,
 // for all heads that a block goes through. It wants 16-bit values and rotated parts that are whole vectors. append_kernel takes everything
 // else through shared memory, a block for each (page, head). Each row is read once, each code written once: bound by memory for
-// prompts (eight of about 900 tokens, 32 + 8 + 8 heads of 128: 51 us, 3.0 TB/s), by latency for single tokens (64: 11 us with the launch) and for small pages,
-// where a block is a chain of loads, angles, the largest value and the codes (2000 tokens of 3 x 20 heads of 64 in pages of 16: 18 us, 15.5 from a captured graph).
+// prompts (eight of about 900 tokens, 32 + 8 + 8 heads of 128: 49 us, 3.2 TB/s), by latency for single tokens (64: 11 us with the launch) and for small pages,
+// where a block is a chain of loads, angles, the largest value and the codes (2000 tokens of 3 x 20 heads of 64 in pages of 16: 17 us, 15.2 from a captured graph).
 #pragma once
 
 #include "rotary.cuh"
@@ -95,8 +95,9 @@ inline size_t append_smem(int rows, int dim, int size) {
 // A rotation in 32 bits is off by less than 2^-21 (|a'| + |b'|): cosine and sine by 2^-23, a product by 2^-24, for |a| + |b|, which is at most 1.42 times
 // |a'| + |b'|, and the sum by 2^-24 of itself: 2.7 * 2^-23. Where both ends of that give the same code, it is the code of the rotation itself. Else, for
 // one value in 2^15, the pair is rotated again in 64 bits and rounded once, so that the codes are those of the definition. Without it 31 codes of 12
-// batches of 2000 rows of 20 heads of 64 were not. Those seldom values take some 0.6 us of a block, and so of a call of few tokens; from a captured
-// graph, 64 single tokens 6.4 -> 7.0 us, eight prompts of about 900 tokens 48.1 -> 50.1, 2000 tokens in pages of 16 14.3 -> 15.5.
+// batches of 2000 rows of 20 heads of 64 were not. From a captured graph: 64 single tokens 6.4 us as before, eight prompts of about 900 tokens
+// 47.4 -> 47.6, 2000 tokens in pages of 16 14.4 -> 15.2. Values at position 0 stay as they are and often lie on a border (of bf16's, one in 16): they
+// are told apart by their sines, else a batch of such rows took 64 us instead of 46.
 constexpr float kRotationOff = 1.f / 2097152.f;
 // the code of a pair's first or second value after rotation, times inv
 __device__ __forceinline__ uint32_t exact_code(const cck_rotation& R, int64_t row, int pair, float a, float b, bool second, float inv) {
@@ -231,7 +232,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
         for (int e = d; e < min(d + 16, A.rotation.dims) && !bad[u]; e++) {
             const int pair = A.rotation.adjacent ? e >> 1 : e < half ? e : e - half, i0 = A.rotation.adjacent ? 2 * pair : pair, i1 = A.rotation.adjacent ? i0 + 1 : i0 + half;
             const float x = fk[u * kp + e], off = (fabsf(fk[u * kp + i0]) + fabsf(fk[u * kp + i1])) * (kRotationOff * inv_k);
-            if (pack_e4m3(fmaf(x, inv_k, -off), 0.f) != pack_e4m3(fmaf(x, inv_k, off), 0.f)) {
+            if (pack_e4m3(fmaf(x, inv_k, -off), 0.f) != pack_e4m3(fmaf(x, inv_k, off), 0.f) &&
+                A.rotation.pos[axis_of(A.rotation, pair) * A.rotation.pos_stride + row0 + u]) {
                 const T* k = static_cast<const T*>(A.k) + (row0 + u) * A.kr + head * A.kh;
                 ck[key_offset(D, s0 + u, e)] = (unsigned char)exact_code(A.rotation, row0 + u, pair, to_f32(k[i0]), to_f32(k[i1]), e == i1, inv_k);
             }
@@ -351,7 +353,7 @@ __global__ void __launch_bounds__(kPageThreads, 1) append_pages_kernel(const __g
             __syncthreads();
         }
         // keys rotated, in f32
-        float x[kKeyItems][16];
+        float x[kKeyItems][16], moved[kKeyItems] = {}; // moved: an item's largest sine; zero at position 0, where values stay as they are
         float top_k = 0.f, top_v = 0.f;
         // of the values as they came, two in a word, without their signs: the largest tells whether all are finite
         uint32_t most = 0, most_v = 0;
@@ -373,6 +375,7 @@ __global__ void __launch_bounds__(kPageThreads, 1) append_pages_kernel(const __g
                     float &a1 = kAdjacent ? x[n][4 * e + 2] : x[n][2 * e + 1], &b1 = kAdjacent ? x[n][4 * e + 3] : x[n][9 + 2 * e];
                     const float2 z0 = rotate(a0, b0, make_float2(w.x, w.y)), z1 = rotate(a1, b1, make_float2(w.z, w.w));
                     a0 = z0.x, b0 = z0.y, a1 = z1.x, b1 = z1.y;
+                    moved[n] = fmaxf(moved[n], fmaxf(fabsf(w.y), fabsf(w.w)));
                 }
             }
 #pragma unroll
@@ -486,7 +489,7 @@ __global__ void __launch_bounds__(kPageThreads, 1) append_pages_kernel(const __g
                 continue;
             }
             uint32_t w[4], beside = 0;
-            const float off = c < turned ? kRotationOff * sc.inv_k : 0.f;
+            const float off = moved[n] > 0.f ? kRotationOff * sc.inv_k : 0.f;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 float lo[4], hi[4];
