@@ -219,20 +219,29 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
             *p = w;
         }
     }
+    const float most_off = 2.f * top_k * (kRotationOff * inv_k); // of all values, for a first look
     for (int i = tid; i < rows * strips; i += kAppendThreads) {
         const int u = i / strips, d = i % strips * 16;
-        uint32_t w[4];
+        const float off = d < A.rotation.dims ? most_off : 0.f;
+        uint32_t w[4], beside = 0;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const float4 x = *reinterpret_cast<const float4*>(fk + u * kp + d + 4 * j);
             w[j] = bad[u] ? kNanCodes : pack_e4m3(x.x * inv_k, x.y * inv_k, x.z * inv_k, x.w * inv_k);
+            beside |= differing(pack_e4m3(fmaf(x.x, inv_k, -off), fmaf(x.y, inv_k, -off), fmaf(x.z, inv_k, -off), fmaf(x.w, inv_k, -off)),
+                                pack_e4m3(fmaf(x.x, inv_k, off), fmaf(x.y, inv_k, off), fmaf(x.z, inv_k, off), fmaf(x.w, inv_k, off)))
+                      << (4 * j);
         }
         *reinterpret_cast<uint4*>(ck + key_offset(D, s0 + u, d)) = make_uint4(w[0], w[1], w[2], w[3]);
 #pragma unroll 1
-        for (int e = d; e < min(d + 16, A.rotation.dims) && !bad[u]; e++) {
+        for (beside = bad[u] ? 0 : beside; beside; beside &= beside - 1) {
+            const int e = d + __ffs(beside) - 1;
+            if (e >= A.rotation.dims) {
+                break;
+            }
             const int pair = A.rotation.adjacent ? e >> 1 : e < half ? e : e - half, i0 = A.rotation.adjacent ? 2 * pair : pair, i1 = A.rotation.adjacent ? i0 + 1 : i0 + half;
-            const float x = fk[u * kp + e], off = (fabsf(fk[u * kp + i0]) + fabsf(fk[u * kp + i1])) * (kRotationOff * inv_k);
-            if (pack_e4m3(fmaf(x, inv_k, -off), 0.f) != pack_e4m3(fmaf(x, inv_k, off), 0.f) &&
+            const float x = fk[u * kp + e], own = (fabsf(fk[u * kp + i0]) + fabsf(fk[u * kp + i1])) * (kRotationOff * inv_k);
+            if (pack_e4m3(fmaf(x, inv_k, -own), 0.f) != pack_e4m3(fmaf(x, inv_k, own), 0.f) &&
                 A.rotation.pos[axis_of(A.rotation, pair) * A.rotation.pos_stride + row0 + u]) {
                 const T* k = static_cast<const T*>(A.k) + (row0 + u) * A.kr + head * A.kh;
                 ck[key_offset(D, s0 + u, e)] = (unsigned char)exact_code(A.rotation, row0 + u, pair, to_f32(k[i0]), to_f32(k[i1]), e == i1, inv_k);
