@@ -20,7 +20,7 @@
 // gives p in the order in which a word of V holds four keys.
 // The running maximum is only a reference: it moves when a score is 2^8 over the largest it was set by, so that shuffles and the
 // rescaling of the sums are rare; p is at most 2^14, the largest at least 2^6, and what f16 loses (2^-25) lies below 2^-30 of that.
-// 64 sequences of up to 8192 tokens, 32 heads on 8 of 128: 140 us, 5.7 TB/s, 0.87 of a copy's rate. One sequence of 700 in pages of 16: 14 us, a
+// 64 sequences of up to 8192 tokens, 32 heads on 8 of 128: 141 us, 5.7 TB/s, 0.87 of a copy's rate. One sequence of 700 in pages of 16: 14 us, a
 // chain of a launch, a look at the table, a copy, six granules a warp, each fetching its instructions anew, and the way out.
 #pragma once
 

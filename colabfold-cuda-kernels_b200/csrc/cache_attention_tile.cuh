@@ -14,8 +14,8 @@
 // products from the issue to the waiting thread, so that a tile whose S, softmax and p V follow one another takes 4800 cycles for 128 keys
 // whatever the rates are. With a buffer ahead, the softmax is the chain: 4200 cycles for 128 keys, half of them the exponentials of two warps on
 // one unit. (Every fourth pair of them by a polynomial instead took as long.) A unit's queries, first S and way out are 10000 cycles more.
-// 4 pieces of up to 1024 tokens before contexts of up to 8192, 32 heads on 8 of 128, bf16: 337 us, 0.92 PFLOP/s, 0.56 of the bf16 rate
-// measured for a library product; prompts of 4096 with a window of 1024, 16 heads on 4 of 64, f16: 93 us, 0.18 of it: nine steps a unit.
+// 4 pieces of up to 1024 tokens before contexts of up to 8192, 32 heads on 8 of 128, bf16: 333 us, 0.93 PFLOP/s, 0.56 of the bf16 rate
+// measured for a library product (364 us and 0.51 among other calls, at lower clocks); prompts of 4096 with a window of 1024, 16 heads on 4 of 64, f16: 93 us, 0.18 of it: nine steps a unit.
 #pragma once
 
 #include <cstddef>
