@@ -235,7 +235,7 @@ template <class T>
 cudaError_t launch_append(cudaStream_t st, const AppendArgs& a, bool pages, int v, unsigned blocks, size_t smem) {
     const int threads = pages && a.group_threads > kAppendThreads ? a.group_threads : kAppendThreads;
     auto go = [&](auto kernel, std::atomic<bool>* ready) {
-        if (smem > 48 * 1024) {
+        if (smem > 47 * 1024) { // 48 with the kernel's own arrays
             if (cudaError_t e = allow_shared(kernel, kAppendSmem, ready)) {
                 return e;
             }

@@ -284,6 +284,22 @@ def test_append_rotates_every_size(seq, rng, new, lens, page, dim, rot, adjacent
     assert torch.equal(got[rest], want[rest])
 
 
+@pytest.mark.parametrize("adjacent", [False, True])
+@pytest.mark.parametrize("rot", [96, 80, 64])
+def test_append_full_pages_of_every_table(seq, rng, rot, adjacent):  # noqa: F811
+    """A page of 128 new tokens whose angles take 48 KB, all that a block has without asking for more: beside them it has arrays of its own."""
+    batch = Batch(seq, [141, 300], [141, 400], 128, rng)
+    cache = Cache(seq, batch.pages, 128, 3, 96).random(rng)
+    before = cache.views()[0].view(torch.float8_e4m3fn).double(), cache.ks.double().clone()
+    k = torch.randn(batch.rows, 3, 96, device="cuda", generator=rng).bfloat16()
+    pos = torch.randint(0, 5000, (1, batch.rows), device="cuda", generator=rng, dtype=torch.int32)
+    freq = torch.rand(rot // 2, device="cuda", generator=rng)
+    r = seq.Rotation(rot, [rot // 2], freq.data_ptr(), pos.data_ptr(), adjacent=adjacent)
+    seq.cache_append(stream(), cache.desc, batch.desc, rows_of(seq, k), rows_of(seq, k), r)
+    want, scale = append_plain(cache, batch, turned(k, pos, freq, [rot // 2], adjacent), before)
+    assert torch.equal(cache.ks.double(), scale) and torch.equal(cache.views()[0].view(torch.float8_e4m3fn).double(), want)
+
+
 def test_workspace_of_heads_that_are_refused_is_zero(seq, rng):  # noqa: F811
     batch = Batch(seq, [1], [5000], 32, rng)
     cache = Cache(seq, batch.pages, 32, 1, 64)
