@@ -106,9 +106,9 @@ __device__ __forceinline__ uint32_t exact_code(const cck_rotation& R, int64_t ro
     const float f = __double2float_rz(x); // to odd, so that the second rounding does not see a border that x is beside
     return pack_e4m3(double(f) == x || x != x ? f : __uint_as_float(__float_as_uint(f) | 1u), 0.f) & 0xFFu;
 }
-// the bytes in which two words differ, a bit each
+// the bytes in which two words of codes differ as values, a bit each: zero has two codes
 __device__ __forceinline__ uint32_t differing(uint32_t v, uint32_t w) {
-    return ((__vcmpne4(v, w) & 0x01010101u) * 0x10204080u) >> 28;
+    return ((__vcmpne4(v, w) & __vcmpne4((v | w) & 0x7F7F7F7Fu, 0u) & 0x01010101u) * 0x10204080u) >> 28;
 }
 
 constexpr int kAppendSmem = 140 * 1024; // the most: 128 rows of 128 values in 32 bits
@@ -511,6 +511,7 @@ __global__ void __launch_bounds__(kPageThreads, 1) append_pages_kernel(const __g
                 w[e] = pack_e4m3(lo[0], lo[1], lo[2], lo[3]);
                 beside |= differing(w[e], pack_e4m3(hi[0], hi[1], hi[2], hi[3])) << (4 * e);
             }
+            beside = off > 0.f ? beside : 0; // other items have no pairs to rotate
             if (some_bad && (bad[group][u / 32] >> (u % 32) & 1)) {
                 w[0] = w[1] = w[2] = w[3] = kNanCodes, beside = 0;
             }

@@ -327,3 +327,30 @@ def test_rotated_codes_bit_for_bit(seq, rng, dtype, adjacent, page, dim):  # noq
     assert torch.equal(cache.ks.double(), scale)
     got = cache.views()[0].view(torch.float8_e4m3fn).double()
     assert (got != want).sum().item() == 0
+
+
+@pytest.mark.parametrize("rot", [None, 0, 32, 96])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_append_of_zeros_of_both_signs(seq, rng, dtype, rot):  # noqa: F811
+    """Zero has two codes and is one value: nothing lies on a border there, rotated or not."""
+    batch = Batch(seq, [40, 1, 70], [60, 33, 70], 32, rng)
+    cache = Cache(seq, batch.pages, 32, 3, 96).random(rng)
+    before = [(c.view(torch.float8_e4m3fn).double(), s.double().clone()) for c, s in zip(cache.views(), (cache.ks, cache.vs))]
+    k, v = (torch.randn(batch.rows, 3, 96, device="cuda", generator=rng) for _ in range(2))
+    for x in (k, v):
+        x[torch.rand(x.shape, device="cuda", generator=rng) < 0.5] = 0.0
+        x[torch.rand(x.shape, device="cuda", generator=rng) < 0.3] = -0.0
+        x[::5], x[1::7] = 0.0, -0.0
+    k, v = k.to(T[dtype]), v.to(T[dtype])
+    want_k, r = k.double(), None
+    if rot is not None:
+        pos = torch.randint(0, 3, (2, batch.rows), device="cuda", generator=rng, dtype=torch.int32)
+        freq = torch.rand(rot // 2, device="cuda", generator=rng)
+        sections = [rot // 2 - 7, 7] if rot else [0, 0]
+        r = seq.Rotation(rot, sections, freq.data_ptr(), pos.data_ptr(), batch.rows)
+        want_k = turned(k, pos, freq, sections, False)
+    seq.cache_append(stream(), cache.desc, batch.desc, rows_of(seq, k), rows_of(seq, v), r)
+    for x, codes, scale, old in zip((want_k, v.double()), cache.views(), (cache.ks, cache.vs), before):
+        want, want_scale = append_plain(cache, batch, x, old)
+        assert torch.equal(scale.double(), want_scale)
+        assert torch.equal(codes.view(torch.float8_e4m3fn).double(), want)
