@@ -26,21 +26,23 @@ __device__ __forceinline__ int axis_of(const cck_rotation& r, int p) {
     }
     return r.axes == 3 || p < edge + r.section[2] ? 2 : 3;
 }
-// A frequency as turns per position modulo one, in units of 2^-64: position times this, modulo 2^64, is the angle reduced without an error but
-// the frequency's (the product in 64 bits and this rounding: 2^-25 of a turn at a position times frequency of 2^31). An f32 product
-// would leave 0.03 radians open at a position of a million.
+// A frequency as turns per position modulo one, in units of 2^-64: position times this, modulo 2^64, is the angle, reduced without an error but this
+// rounding, 2^-65 of a turn times the position. 1 / 2 pi is in two doubles: in one, an angle of 2^20 radians would be off by 2^-32, and codes of rotated
+// keys with it. An f32 product would leave 0.03 radians open at a position of a million.
 struct Turns {
     uint64_t per;
     bool finite;
 };
 __device__ __forceinline__ Turns turns_of(float freq) {
-    const double x = double(freq) * 0.15915494309189533577, f = x - floor(x);
-    return {f < 1.0 ? __double2ull_rn(f * 18446744073709551616.0) : 0, freq - freq == 0.f};
+    constexpr double kHigh = 0.15915494309189535, kLow = -9.839338337591243e-18;
+    const double x = double(freq) * kHigh, rest = fma(double(freq), kHigh, -x) + double(freq) * kLow;
+    const long long per = __double2ll_rn((x - rint(x)) * 18446744073709551616.0), more = __double2ll_rn((rest - rint(rest)) * 18446744073709551616.0);
+    return {uint64_t(per) + uint64_t(more), freq - freq == 0.f};
 }
 // The nearest quarter turn is taken off in integers; what is left, at most pi / 4, goes through the Taylor series of sine and cosine about
 // zero to the ninth and tenth power (the terms after them are below 2e-9 of the result). It is held in two floats, x + e, down to 2^-58 of a turn,
 // so that a small angle keeps its digits, and the last additions carry what they round off: both come out within a few units of the last place of
-// themselves, however small the sine is, as far as the angle itself is known (2^-52 of position times frequency). With 2^-32 of a turn it took the same
+// themselves, however small the sine is, as far as the angle itself is known (2^-62 of the position). With 2^-32 of a turn it took the same
 // time, and a sine of 1e-4 was off by 1e-5 of itself.
 __device__ __forceinline__ float2 cos_sin(int pos, Turns t) {
     const uint64_t angle = t.per * uint64_t(int64_t(pos)); // of a turn, in 2^-64

@@ -34,8 +34,8 @@ def test_small_sines_have_their_digits(seq, rng, far, freq, adjacent):  # noqa: 
 
     Each is good to 10 roundings of 2^-24 of itself: where the coarse part of the angle is zero or as small as the fine one, five of the fine part
     (its conversion, the constant, their product, two additions) and, in the series, the factor 1 - y / 2, its product, two additions; one is spare.
-    Beside that the angle, in radians: |position * frequency| 2^-51 (the constant 1 / 2 pi, its product and the one of the 64-bit form here, 2^-53
-    each, and a margin of 4/3), |position| 2^-62 (a frequency's last place, half of 2^-64 of a turn) and 2^-55 (an angle's: 2^-58 of a turn)."""
+    Beside that the angle, in radians: |position * frequency| 2^-52 (the product of the 64-bit form here, 2^-53 where it has more than 53 bits, and its
+    cosine), |position| 2^-61 (a frequency's last place, one of 2^-64 of a turn: 2^-61.3) and 2^-55 (an angle's: 2^-58 of a turn)."""
     rows, pairs = 4096, 32
     pos = torch.randint(-far, far, (1, rows), device="cuda", generator=rng, dtype=torch.int32)
     f = (torch.rand(pairs, device="cuda", generator=rng) * 0.9 + 0.1) * freq
@@ -47,7 +47,7 @@ def test_small_sines_have_their_digits(seq, rng, far, freq, adjacent):  # noqa: 
     r = seq.Rotation(2 * pairs, [pairs], f.data_ptr(), pos.data_ptr(), adjacent=adjacent)
     seq.rotary(stream(), r, rows, 2 * pairs, rows_of(seq, x), rows_of(seq, y))
     angle = pos[0].double()[:, None] * f.double()
-    off = angle.abs() * 2.0**-51 + pos[0].double().abs()[:, None] * 2.0**-62 + 2.0**-55
+    off = angle.abs() * 2.0**-52 + pos[0].double().abs()[:, None] * 2.0**-61 + 2.0**-55
     for got, want in ((y[:, 0, a], angle.cos()), (y[:, 0, b], angle.sin())):
         err = (got.double() - want).abs()
         assert (err <= 10 * 2.0**-24 * want.abs() + off).all(), (err / (2.0**-24 * want.abs() + off)).max().item()
@@ -307,16 +307,17 @@ def test_workspace_of_heads_that_are_refused_is_zero(seq, rng):  # noqa: F811
     assert seq.cache_attention_workspace_bytes(cache.desc, batch.desc, (1 << 16) + 16) == 0
 
 
+@pytest.mark.parametrize("far", [8192, 1 << 28])
 @pytest.mark.parametrize("dtype, adjacent, page, dim", [("f16", True, 16, 64), ("bf16", False, 64, 128), ("bf16", True, 32, 96), ("f32", False, 64, 64), ("f16", False, 128, 32)])
-def test_rotated_codes_bit_for_bit(seq, rng, dtype, adjacent, page, dim):  # noqa: F811
+def test_rotated_codes_bit_for_bit(seq, rng, dtype, adjacent, page, dim, far):  # noqa: F811
     """The codes of rotated keys are those of the rotation in 64 bits, rounded once: of several million values, none differs. (64 bits leave 2^-50 of a
-    value open beside a border, which none of so many comes near to.)"""
+    value open beside a border, which none of so many comes near to; a position of 28 bits times a frequency of 24 is exact in 64.)"""
     heads, lens = 20, [1500, 1100, 2000, 900]
     batch = Batch(seq, lens, [n + 13 * b for b, n in enumerate(lens)], page, rng)
     cache = Cache(seq, batch.pages, page, heads, dim).random(rng)
     before = cache.views()[0].view(torch.float8_e4m3fn).double(), cache.ks.double().clone()
     k = torch.randn(batch.rows, heads, dim, device="cuda", generator=rng).to(T[dtype])
-    pos = torch.randint(0, 8192, (2, batch.rows), device="cuda", generator=rng, dtype=torch.int32)
+    pos = torch.randint(0, far, (2, batch.rows), device="cuda", generator=rng, dtype=torch.int32)
     pos[:, ::50] = 0  # exact values, many of them on a border
     pos[1, 1::50] = 0
     freq = (10000.0 ** (-torch.arange(dim // 2, device="cuda") / (dim // 2))).float()
